@@ -4,7 +4,7 @@ over such a cache (ops.kvq_attention), causal or with a sliding window and a few
 
 The cache. A head row of D values is cut into groups of 32. A group has one scale s: its largest magnitude over the
 largest code (7 in 4 bits, 127 in 8 bits), rounded up to five significant bits (4 bits) or to a power of two (8 bits),
-in bfloat16; a value is held as c = round(x / s), half to even, and stands for c * s, which bfloat16 holds exactly.
+in bfloat16; a value is held as c = round(x / s), half to even, and stands for c * s, which bfloat16 holds exactly. A group with a magnitude of 2^100 and more (or none: NaN) is held as NaN.
 codes [B, Hk, capacity, D * bits / 8] hold c + 8 (two in a byte, the even column in the low half) or c + 128.
 
 Attention. Query t of a sequence whose first new position is p sits at i = p + t and sees the positions j <= i with
@@ -139,7 +139,7 @@ def _quantise(x, bits):
     most = g.abs().amax(-1)
     s = (most / top).view(torch.int32)
     s = ((s + ((1 << cut) - 1)) >> cut << cut).view(torch.float32)
-    s = torch.where(most < 2.0 ** 120, s, torch.full_like(s, math.nan))
+    s = torch.where(most < 2.0 ** 100, s, torch.full_like(s, math.nan))
     c = (g.double() / s.double().unsqueeze(-1)).round()     # 64 bits: next to a half, 32 would decide otherwise
     c = torch.where(s.unsqueeze(-1) > 0, c.clamp(-top, top), torch.zeros_like(c))
     return (c.flatten(-2) + (1 << (bits - 1))).to(torch.uint8), s.bfloat16()
