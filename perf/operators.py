@@ -3,7 +3,7 @@ writing new rows and reading them back (ops.kvq_write, ops.kvq_read), and attent
 over such a cache (ops.kvq_attention), causal or with a sliding window and a few first tokens that stay visible.
 
 The cache. A head row of D values is cut into groups of 32. A group has one scale s: its largest magnitude over the
-largest code (7 in 4 bits, 127 in 8 bits), rounded up to five significant bits (4 bits) or to a power of two (8 bits),
+largest code (7 in 4 bits, 127 in 8 bits), rounded up to four significant bits (4 bits) or to a power of two (8 bits),
 in bfloat16; a value is held as c = round(x / s), half to even, and stands for c * s, which bfloat16 holds exactly. A group with a magnitude of 2^100 and more (or none: NaN) is held as NaN.
 codes [B, Hk, capacity, D * bits / 8] hold c + 8 (two in a byte, the even column in the low half) or c + 128.
 
@@ -134,7 +134,7 @@ def work(c):
 # ---- the plain form -----------------------------------------------------------------------------
 def _quantise(x, bits):
     """Codes (whole numbers, as bytes from 0) and scales (bfloat16) of the rows of x."""
-    top, cut = (7, 19) if bits == 4 else (127, 23)
+    top, cut = (7, 20) if bits == 4 else (127, 23)
     g = x.float().unflatten(-1, (-1, GROUP))
     most = g.abs().amax(-1)
     s = (most / top).view(torch.int32)
@@ -251,7 +251,7 @@ def _held64(x, bits):
     most = x.abs().amax(-1, keepdim=True)
     ratio = (most.float() / (2 ** (bits - 1) - 1)).double()       # formed in 32 bits, as the definition has it
     part, power = torch.frexp(ratio)
-    keep = 32.0 if bits == 4 else 1.0
+    keep = 16.0 if bits == 4 else 1.0
     if bits == 8:
         power = torch.where(part == 0.5, power - 1, power)        # a power of two stays
         step = torch.where(most > 0, torch.ldexp(torch.ones_like(part), power), torch.zeros_like(part))
