@@ -1,0 +1,262 @@
+// Writing rows into a key/value cache of 4 or 8 bits, and reading them back (layout: kv_quant.cuh). Beside the
+// fp32 cache's ctdk_kv_write / ctdk_kv_read_expanded (emberlm src/ops/kv_cache.cu:14-109).
+//
+// Both are bound by memory: a thread takes eight neighbouring values, four threads a group; a row's threads are
+// neighbours and consecutive rows are consecutive positions of one head, so that the cache side is contiguous and
+// the other side comes in whole head rows of 128 to 512 bytes.
+#include "kv_quant.cuh"
+
+namespace ctdk {
+namespace kvq {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct RowArgs {
+  const void* src[2];
+  int64_t row_stride, batch_stride;      // elements between tokens, between sequences
+  uint8_t* codes[2];
+  __nv_bfloat16* scales[2];
+  const int32_t *pos, *count;            // per sequence, or null
+  int64_t pos_all, capacity;
+  int64_t rows;                          // B * Hk * T
+  int T, Hk;
+};
+
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
+  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+// Code of x in [-top, top] for the scale s, to nearest, half to even, decided exactly: n is the product with a rounded
+// reciprocal, at most one step off and only next to a half; x - n * s is exact (both are whole multiples of the smaller
+// one's last place and the difference is short), so comparing it with half a step says which side of the half x is on.
+__device__ __forceinline__ float nearest(float x, float s, float inv) {
+  const float magic = 12582912.0f;       // 1.5 * 2^23: adding it rounds to a whole number
+  float n = __fadd_rn(__fmaf_rn(x, inv, magic), -magic);
+  const float r = __fmaf_rn(-n, s, x), h = 0.5f * s;
+  if (fabsf(r) >= h) {                   // rare
+    const float far = n + copysignf(1.0f, r);
+    const bool odd = (static_cast<int>(n) & 1) != 0;
+    if (fabsf(r) > h || odd) n = far;
+  }
+  return n;
+}
+
+template <typename T, int BITS, int D>
+__global__ void __launch_bounds__(kThreads) kvq_write_kernel(const RowArgs a) {
+  constexpr int kPerRow = D / 8, kRowBytes = D * BITS / 8;
+  constexpr float kPart = 1.0f / (BITS == 4 ? 7.0f : 127.0f);
+  constexpr int kCut = BITS == 4 ? 20 : 23;   // low bits of the fp32 scale that rounding up clears
+  pdl_launch();
+  pdl_wait();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, r = i / kPerRow;
+  const int lane8 = static_cast<int>(i % kPerRow), which = blockIdx.y;
+  bool live = r < a.rows;
+  float x[8] = {};
+  int64_t at = 0;
+  if (live) {
+    const int64_t bh = r / a.T;
+    const int t = static_cast<int>(r - bh * a.T);
+    const int64_t b = bh / a.Hk;
+    const int h = static_cast<int>(bh - b * a.Hk);
+    const int64_t p = (a.pos != nullptr ? static_cast<int64_t>(a.pos[b]) : a.pos_all) + t;
+    live = p >= 0 && p < a.capacity && (a.count == nullptr || t < a.count[b]);
+    at = bh * a.capacity + p;
+    if (live) load8(static_cast<const T*>(which ? a.src[1] : a.src[0]) + b * a.batch_stride + t * a.row_stride + h * D + lane8 * 8, x);
+  }
+  float most = 0.0f;
+  bool nan = false;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    most = fmaxf(most, fabsf(x[k]));
+    nan |= isnan(x[k]);
+  }
+  if (nan) most = __int_as_float(0x7f800000);
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  if (!live) return;
+  const bool fine = most < kMost;
+  float s = __uint_as_float(((__float_as_uint(__fmul_rn(most, kPart)) + ((1u << kCut) - 1u)) >> kCut) << kCut);
+  uint32_t u[8];
+  if (!fine || s == 0.0f) {
+    if (!fine) s = __int_as_float(0x7fc00000);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) u[k] = 1u << (BITS - 1);
+  } else if (BITS == 8) {
+    const float inv = __fdiv_rn(1.0f, s);     // a power of two from 2^-126 on: exact, and so is the product
+#pragma unroll
+    for (int k = 0; k < 8; ++k) u[k] = __float_as_uint(__fmaf_rn(x[k], inv, 12582912.0f + 128.0f)) & 0xffu;
+  } else if (s < 0x1p-100f) {                 // a reciprocal could overflow: 64 bits, where the quotient's half is safe
+#pragma unroll
+    for (int k = 0; k < 8; ++k) u[k] = static_cast<uint32_t>(static_cast<int>(fmin(fmax(rint(static_cast<double>(x[k]) / s), -7.0), 7.0)) + 8);
+  } else {
+    const float inv = __fdiv_rn(1.0f, s);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) u[k] = static_cast<uint32_t>(static_cast<int>(nearest(x[k], s, inv)) + 8);
+  }
+  uint8_t* dst = (which ? a.codes[1] : a.codes[0]) + at * kRowBytes + lane8 * BITS;
+  if (BITS == 8) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(u[0] | u[1] << 8 | u[2] << 16 | u[3] << 24, u[4] | u[5] << 8 | u[6] << 16 | u[7] << 24);
+  } else {
+    *reinterpret_cast<uint32_t*>(dst) =
+        u[0] | u[1] << 4 | u[2] << 8 | u[3] << 12 | u[4] << 16 | u[5] << 20 | u[6] << 24 | u[7] << 28;
+  }
+  if ((lane8 & 3) == 0) (which ? a.scales[1] : a.scales[0])[at * (D / kGroup) + lane8 / 4] = __ushort_as_bfloat16(static_cast<unsigned short>(__float_as_uint(s) >> 16));
+}
+
+struct ReadArgs {
+  Cache c;
+  void* out[2];                          // [B, Hk * group, length, D]
+  int64_t start, length, rows;           // rows = B * Hk * length
+  int group;
+};
+
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {   // exact
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+}
+
+template <typename T, int BITS, int D>
+__global__ void __launch_bounds__(kThreads) kvq_read_kernel(const ReadArgs a) {
+  constexpr int kPerRow = D / 8, kRowBytes = D * BITS / 8;
+  pdl_launch();
+  pdl_wait();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, r = i / kPerRow;
+  const int lane8 = static_cast<int>(i % kPerRow), which = blockIdx.y;
+  if (r >= a.rows) return;
+  const int64_t bh = r / a.length, t = r - bh * a.length, at = bh * a.c.capacity + a.start + t;
+  const float s = __bfloat162float((which ? a.c.scales[1] : a.c.scales[0])[at * (D / kGroup) + lane8 / 4]);
+  const uint8_t* src = (which ? a.c.codes[1] : a.c.codes[0]) + at * kRowBytes + lane8 * BITS;
+  float x[8];
+  if (BITS == 8) {
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      x[k] = static_cast<float>(static_cast<int>(w.x >> (8 * k) & 0xffu) - 128) * s;
+      x[4 + k] = static_cast<float>(static_cast<int>(w.y >> (8 * k) & 0xffu) - 128) * s;
+    }
+  } else {
+    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(src));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = static_cast<float>(static_cast<int>(w >> (4 * k) & 0xfu) - 8) * s;
+  }
+  T* dst = static_cast<T*>(which ? a.out[1] : a.out[0]) + (bh * a.group * a.length + t) * D + lane8 * 8;
+  for (int g = 0; g < a.group; ++g) store8(dst + g * a.length * D, x);
+}
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+template <typename K, typename A>
+int launch_rows(K kernel, const A& a, int64_t rows, int D, cudaStream_t s, const char* what) {
+  const int64_t blocks = (rows * (D / 8) + kThreads - 1) / kThreads;
+  CTDK_REQUIRE(blocks <= INT32_MAX, "%s: too many rows", what);
+  const cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(blocks), 2), dim3(kThreads), 0, s, a);
+  if (e != cudaSuccess) return fail(CTDK_ELAUNCH, "%s: %s", what, cudaGetErrorString(e));
+  return check_launch(what);
+}
+
+}  // namespace
+
+int check_cache(const ctdk_kvq_cache* c, const char* what) {
+  CTDK_REQUIRE(c != nullptr, "%s: no cache", what);
+  CTDK_REQUIRE(c->bits == 4 || c->bits == 8, "%s: bits must be 4 or 8", what);
+  CTDK_REQUIRE(c->D == 64 || c->D == 128, "%s: D must be 64 or 128", what);
+  CTDK_REQUIRE(c->B >= 0 && c->B <= INT32_MAX && c->Hk > 0, "%s: bad batch or head count", what);
+  CTDK_REQUIRE(c->capacity > 0 && c->capacity % kCapacityStep == 0 && c->capacity <= INT32_MAX - 2 * kCapacityStep,
+               "%s: capacity must be a multiple of %d below 2^31", what, kCapacityStep);
+  if (c->B == 0) return CTDK_OK;
+  CTDK_REQUIRE(c->k_codes != nullptr && c->k_scales != nullptr && c->v_codes != nullptr && c->v_scales != nullptr, "%s: null cache pointer", what);
+  CTDK_REQUIRE(aligned(c->k_codes, 16) && aligned(c->k_scales, 16) && aligned(c->v_codes, 16) && aligned(c->v_scales, 16),
+               "%s: the cache's pointers must be 16-byte aligned", what);
+  return CTDK_OK;
+}
+
+}  // namespace kvq
+}  // namespace ctdk
+
+using namespace ctdk;
+
+extern "C" {
+
+int ctdk_kvq_write(const ctdk_kvq_cache* cache, const void* k, const void* v, int dtype, int64_t row_stride, int64_t batch_stride, int64_t T,
+                   const int32_t* pos, int64_t pos_all, const int32_t* count, void* stream) {
+  if (const int rc = kvq::check_cache(cache, "kvq_write"); rc != CTDK_OK) return rc;
+  CTDK_REQUIRE(dtype == CTDK_DTYPE_F32 || dtype == CTDK_DTYPE_BF16, "kvq_write: dtype must be CTDK_DTYPE_F32 or CTDK_DTYPE_BF16");
+  CTDK_REQUIRE(T >= 0 && T <= INT32_MAX, "kvq_write: bad T");
+  CTDK_REQUIRE(pos != nullptr || (pos_all >= 0 && pos_all + T <= cache->capacity), "kvq_write: positions %lld..%lld exceed the capacity %lld",
+               static_cast<long long>(pos_all), static_cast<long long>(pos_all + T), static_cast<long long>(cache->capacity));
+  if (T == 0 || cache->B == 0) return CTDK_OK;
+  const int64_t unit = dtype == CTDK_DTYPE_F32 ? 4 : 8;   // elements in 16 bytes
+  CTDK_REQUIRE(k != nullptr && v != nullptr && kvq::aligned(k, 16) && kvq::aligned(v, 16), "kvq_write: k and v must be 16-byte aligned");
+  CTDK_REQUIRE(row_stride % unit == 0 && batch_stride % unit == 0 && row_stride >= 0 && batch_stride >= 0,
+               "kvq_write: strides must be multiples of 16 bytes");
+  kvq::RowArgs a;
+  a.src[0] = k;
+  a.src[1] = v;
+  a.row_stride = row_stride;
+  a.batch_stride = batch_stride;
+  a.codes[0] = static_cast<uint8_t*>(cache->k_codes);
+  a.codes[1] = static_cast<uint8_t*>(cache->v_codes);
+  a.scales[0] = static_cast<__nv_bfloat16*>(cache->k_scales);
+  a.scales[1] = static_cast<__nv_bfloat16*>(cache->v_scales);
+  a.pos = pos;
+  a.count = count;
+  a.pos_all = pos_all;
+  a.capacity = cache->capacity;
+  a.rows = cache->B * cache->Hk * T;
+  a.T = static_cast<int>(T);
+  a.Hk = cache->Hk;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool f32 = dtype == CTDK_DTYPE_F32;
+  auto go = [&](auto* kernel) { return kvq::launch_rows(kernel, a, a.rows, cache->D, s, "kvq_write"); };
+  if (cache->bits == 4) {
+    if (cache->D == 64) return f32 ? go(kvq::kvq_write_kernel<float, 4, 64>) : go(kvq::kvq_write_kernel<__nv_bfloat16, 4, 64>);
+    return f32 ? go(kvq::kvq_write_kernel<float, 4, 128>) : go(kvq::kvq_write_kernel<__nv_bfloat16, 4, 128>);
+  }
+  if (cache->D == 64) return f32 ? go(kvq::kvq_write_kernel<float, 8, 64>) : go(kvq::kvq_write_kernel<__nv_bfloat16, 8, 64>);
+  return f32 ? go(kvq::kvq_write_kernel<float, 8, 128>) : go(kvq::kvq_write_kernel<__nv_bfloat16, 8, 128>);
+}
+
+int ctdk_kvq_read(const ctdk_kvq_cache* cache, int64_t start, int64_t length, int group, int dtype, void* k_out, void* v_out, void* stream) {
+  if (const int rc = kvq::check_cache(cache, "kvq_read"); rc != CTDK_OK) return rc;
+  CTDK_REQUIRE(dtype == CTDK_DTYPE_F32 || dtype == CTDK_DTYPE_BF16, "kvq_read: dtype must be CTDK_DTYPE_F32 or CTDK_DTYPE_BF16");
+  CTDK_REQUIRE(start >= 0 && length >= 0 && start <= cache->capacity - length, "kvq_read: positions out of range");
+  CTDK_REQUIRE(group > 0, "kvq_read: group must be > 0");
+  if (length == 0 || cache->B == 0) return CTDK_OK;
+  CTDK_REQUIRE(k_out != nullptr && v_out != nullptr && kvq::aligned(k_out, 16) && kvq::aligned(v_out, 16),
+               "kvq_read: outputs must be 16-byte aligned");
+  kvq::ReadArgs a;
+  a.c = kvq::Cache{{static_cast<const uint8_t*>(cache->k_codes), static_cast<const uint8_t*>(cache->v_codes)},
+                   {static_cast<const __nv_bfloat16*>(cache->k_scales), static_cast<const __nv_bfloat16*>(cache->v_scales)},
+                   cache->capacity, static_cast<int>(cache->B), cache->Hk};
+  a.out[0] = k_out;
+  a.out[1] = v_out;
+  a.start = start;
+  a.length = length;
+  a.rows = cache->B * cache->Hk * length;
+  a.group = group;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool f32 = dtype == CTDK_DTYPE_F32;
+  auto go = [&](auto* kernel) { return kvq::launch_rows(kernel, a, a.rows, cache->D, s, "kvq_read"); };
+  if (cache->bits == 4) {
+    if (cache->D == 64) return f32 ? go(kvq::kvq_read_kernel<float, 4, 64>) : go(kvq::kvq_read_kernel<__nv_bfloat16, 4, 64>);
+    return f32 ? go(kvq::kvq_read_kernel<float, 4, 128>) : go(kvq::kvq_read_kernel<__nv_bfloat16, 4, 128>);
+  }
+  if (cache->D == 64) return f32 ? go(kvq::kvq_read_kernel<float, 8, 64>) : go(kvq::kvq_read_kernel<__nv_bfloat16, 8, 64>);
+  return f32 ? go(kvq::kvq_read_kernel<float, 8, 128>) : go(kvq::kvq_read_kernel<__nv_bfloat16, 8, 128>);
+}
+
+}  // extern "C"

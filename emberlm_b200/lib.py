@@ -10,6 +10,7 @@ LIB_PATH = HERE / "libctdk.so"
 HEADER = HERE.parent / "include" / "ctdk.h"
 
 CTDK_OK, CTDK_EINVAL, CTDK_ELAUNCH, CTDK_ETIMEOUT, CTDK_ENOMEM = 0, -1, -2, -3, -4
+DTYPE_F32, DTYPE_BF16 = 0, 1
 GEMM_TF32, GEMM_3XTF32, GEMM_FP32_SIMT = 0, 1, 2
 EPI_STORE, EPI_ACCUMULATE, EPI_RESIDUAL = 0, 1, 2
 
@@ -30,6 +31,11 @@ class RopeParams(C.Structure):
 class AdamWParams(C.Structure):
     _fields_ = [("lr", C.c_float), ("beta1", C.c_float), ("beta2", C.c_float),
                 ("eps", C.c_float), ("wd", C.c_float), ("bc1", C.c_float), ("bc2", C.c_float)]
+
+
+class KvqCacheDesc(C.Structure):
+    _fields_ = [("k_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_codes", C.c_void_p), ("v_scales", C.c_void_p),
+                ("B", C.c_int64), ("capacity", C.c_int64), ("Hk", C.c_int), ("D", C.c_int), ("bits", C.c_int)]
 
 
 def declared_symbols() -> list[str]:
@@ -97,6 +103,10 @@ _SIGS = {
     "ctdk_mse_bwd": [_p, _p, _p, _p, _l, _p],
     "ctdk_kv_write": [_p, _p, _l, _l, _i, _i, _l, _l, _p],
     "ctdk_kv_read_expanded": [_p, _p, _l, _i, _i, _l, _i, _l, _p],
+    "ctdk_kvq_write": [_p, _p, _p, _i, _l, _l, _l, _p, _l, _p, _p],
+    "ctdk_kvq_read": [_p, _l, _l, _i, _i, _p, _p, _p],
+    "ctdk_kvq_attn_workspace_bytes": [_p, _l, _i],
+    "ctdk_kvq_attn": [_p, _p, _i, _l, _l, _l, _i, _p, _l, _p, _l, _l, _f, _p, _p, _l, _p],
     "ctdk_loss_ratio": [_p, _p, _p],
     "ctdk_sample": [_p, _l, _l, _f, _i, _f, _p, _p, _p, _p],
     "ctdk_ce_row_weight": [_p, _p, _p, _l, _p, _p],
@@ -105,6 +115,7 @@ for _name, _args in _SIGS.items():
     _fn = getattr(_lib, _name)
     _fn.argtypes = _args
     _fn.restype = C.c_int
+_lib.ctdk_kvq_attn_workspace_bytes.restype = C.c_int64
 _lib.ctdk_last_error.restype = C.c_char_p
 _lib.ctdk_last_error.argtypes = []
 _lib.ctdk_sm_count.restype = C.c_int

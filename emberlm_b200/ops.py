@@ -299,6 +299,120 @@ def attention_backward(qkv, out, dout, lse, B, T, H, Hk, D, precision=lib.GEMM_T
     return dqkv
 
 
+class KvqCache:
+    """A key/value cache held in 4 or 8 bits (layout and rounding: ctdk.h, ctdk_kvq_*), over tensors of the caller:
+    codes uint8 [B, Hk, capacity, D * bits / 8] and scales bfloat16 [B, Hk, capacity, D / 32] of keys and values.
+    Keeps the tensors; one object serves as long as the cache."""
+
+    def __init__(self, k_codes, k_scales, v_codes, v_scales):
+        for t, dt in ((k_codes, torch.uint8), (k_scales, torch.bfloat16), (v_codes, torch.uint8), (v_scales, torch.bfloat16)):
+            _chk(t, "KvqCache", dt)
+            if t.dim() != 4 or t.device != k_codes.device:
+                raise RuntimeError("KvqCache: expected four 4D tensors on one device")
+        if v_codes.shape != k_codes.shape or v_scales.shape != k_scales.shape or k_codes.shape[:3] != k_scales.shape[:3]:
+            raise RuntimeError("KvqCache: shape mismatch")
+        B, Hk, capacity, row = k_codes.shape
+        D = k_scales.shape[3] * 32
+        if D not in (64, 128) or row * 8 not in (4 * D, 8 * D):
+            raise RuntimeError("KvqCache: head size must be 64 or 128, held in 4 or 8 bits")
+        if capacity == 0 or capacity % 64:
+            raise RuntimeError("KvqCache: capacity must be a multiple of 64")
+        self.tensors = (k_codes, k_scales, v_codes, v_scales)
+        self.device, self.B, self.Hk, self.capacity, self.D, self.bits = k_codes.device, B, Hk, capacity, D, row * 8 // D
+        self.desc = lib.KvqCacheDesc(*(t.data_ptr() for t in self.tensors), B, capacity, Hk, D, self.bits)
+        self.ref = C.addressof(self.desc)
+
+
+def kvq_cache(B, Hk, max_seq, D, bits, device="cuda"):
+    """An empty cache for max_seq positions (rounded up to a multiple of 64)."""
+    if bits not in (4, 8) or D not in (64, 128):
+        raise RuntimeError("kvq_cache: bits must be 4 or 8, D 64 or 128")
+    room = -(-max(int(max_seq), 1) // 64) * 64
+    held = []
+    for _ in range(2):
+        held += [torch.zeros(B, Hk, room, D * bits // 8, dtype=torch.uint8, device=device),
+                 torch.zeros(B, Hk, room, D // 32, dtype=torch.bfloat16, device=device)]
+    return KvqCache(*held)
+
+
+_KVQ_DTYPES = {torch.float32: lib.DTYPE_F32, torch.bfloat16: lib.DTYPE_BF16}
+
+
+def _kvq_rows(x, name, cache, heads):
+    """Checks rows [B, T, heads, D] (heads side by side; slices of a packed projection qualify); returns their strides."""
+    if x.dtype not in _KVQ_DTYPES:
+        raise RuntimeError(f"{name}: expected float32 or bfloat16")
+    if x.device != cache.device:
+        raise RuntimeError(f"{name}: expected a tensor on {cache.device}")
+    if x.dim() != 4 or x.shape[0] != cache.B or x.shape[3] != cache.D or (heads and x.shape[2] != heads):
+        raise RuntimeError(f"{name}: expected [B, T, heads, D] that fits the cache")
+    sb, st, sh, sd = x.stride()
+    if x.numel() and ((sd != 1) or (sh != cache.D and x.shape[2] > 1)):
+        raise RuntimeError(f"{name}: a token's heads must be contiguous")
+    return (st if x.shape[1] > 1 else 0), (sb if x.shape[0] > 1 else 0)
+
+
+def _kvq_places(pos, count, cache, name):
+    """(pos pointer, position of all, count pointer): pos an int or int32 [B] on the device, count None or the latter."""
+    at = [None, 0, None]
+    for i, t in ((0, pos), (2, count)):
+        if isinstance(t, torch.Tensor):
+            if t.dtype != torch.int32 or t.device != cache.device or tuple(t.shape) != (cache.B,) or not t.is_contiguous():
+                raise RuntimeError(f"{name}: positions and counts are int32 [B] on the cache's device")
+            at[i] = t.data_ptr()
+        elif i == 0:
+            at[1] = int(t)
+        elif t is not None:
+            raise RuntimeError(f"{name}: count must be a tensor or None")
+    return at
+
+
+def _kvq_stream(cache):
+    return torch.cuda.current_stream(cache.device).cuda_stream
+
+
+def kvq_write(cache, k, v, pos, count=None):
+    """Holds the rows k, v [B, T, Hk, D] (float32 or bfloat16) at positions pos .. of each sequence. pos: an int, or int32 [B]
+    on the device; count (int32 [B], optional): how many of a sequence's T rows are there."""
+    strides = _kvq_rows(k, "kvq_write", cache, cache.Hk)
+    if v.shape != k.shape or v.dtype != k.dtype or _kvq_rows(v, "kvq_write", cache, cache.Hk) != strides:
+        raise RuntimeError("kvq_write: k and v must have the same shape, type and strides")
+    p, at, n = _kvq_places(pos, count, cache, "kvq_write")
+    with torch.cuda.device(cache.device):
+        lib.call("ctdk_kvq_write", cache.ref, k.data_ptr(), v.data_ptr(), _KVQ_DTYPES[k.dtype], *strides, k.shape[1], p, at, n, _kvq_stream(cache))
+
+
+def kvq_read(cache, start, length, group=1, dtype=torch.float32):
+    """(k, v) [B, Hk * group, length, D]: what the cache holds at positions start .., each KV head `group` times (both types exact)."""
+    if dtype not in _KVQ_DTYPES:
+        raise RuntimeError("kvq_read: expected float32 or bfloat16")
+    if start < 0 or length < 0 or start + length > cache.capacity or group < 1:
+        raise RuntimeError("kvq_read: positions out of range, or a group below 1")
+    out = torch.empty(2, cache.B, cache.Hk * group, length, cache.D, device=cache.device, dtype=dtype)
+    k, v = out[0], out[1]
+    with torch.cuda.device(cache.device):
+        lib.call("ctdk_kvq_read", cache.ref, start, length, group, _KVQ_DTYPES[dtype], k.data_ptr(), v.data_ptr(), _kvq_stream(cache))
+    return k, v
+
+
+def kvq_attention(q, cache, pos, count=None, window=0, sinks=0, scale=None):
+    """Attention of q [B, T, H, D] (float32 or bfloat16), whose rows sit at positions pos .. of each sequence, over the cache:
+    causal, with window > 0 over the last `window` positions and the first `sinks`. Returns [B, T, H, D]; padding (rows from
+    count on) is zeros. pos and count as for kvq_write; scale: 1 / sqrt(D) unless given."""
+    strides = _kvq_rows(q, "kvq_attention", cache, 0)
+    T, H = q.shape[1], q.shape[2]
+    if H == 0 or H % cache.Hk:
+        raise RuntimeError("kvq_attention: heads must be a multiple of kv heads")
+    p, at, n = _kvq_places(pos, count, cache, "kvq_attention")
+    with torch.cuda.device(cache.device):
+        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        need = lib.raw().ctdk_kvq_attn_workspace_bytes(cache.ref, T, H)
+        work = torch.empty(need, device=q.device, dtype=torch.uint8) if need > 0 else None
+        lib.call("ctdk_kvq_attn", cache.ref, q.data_ptr(), _KVQ_DTYPES[q.dtype], *strides, T, H, p, at, n, window, sinks,
+                 cache.D ** -0.5 if scale is None else scale, out.data_ptr(), work.data_ptr() if need > 0 else None, max(need, 0), _kvq_stream(cache))
+    return out
+
+
 def sumsq(g, out=None):
     out = torch.zeros(1, device=g.device) if out is None else out
     lib.call("ctdk_sumsq", g.data_ptr(), g.numel(), out.data_ptr(), _s())

@@ -317,6 +317,52 @@ int ctdk_ce_row_weight(const float* loss_mask, const float* dy, const float* mas
                        float* row_weight, void* stream);
 
 /* ------------------------------------------------------------------------------------
+ * A key/value cache held in 4 or 8 bits, and attention over it: the fp32 cache above (ctdk_kv_write,
+ * ctdk_kv_read_expanded) in 4.5 or 8.5 bits a value, for batches of sequences of their own lengths
+ * (no counterpart in the reference, whose cache is fp32).
+ *   codes   [B, Hk, capacity, D * bits / 8] bytes, scales [B, Hk, capacity, D / 32] bfloat16; 16-byte
+ *           aligned; capacity (positions) a multiple of 64; D 64 or 128.
+ *   held    32 neighbouring values of a head row are a group with one scale s: the group's largest
+ *           magnitude times the fp32 number nearest 1/7 (4 bits) or 1/127 (8 bits), in fp32, rounded up to four
+ *           significant bits (4 bits) or to a power of two (8 bits). A value is the code
+ *           c = x / s rounded to the nearest whole number, half to even, stored as c + 8 (the even
+ *           column in the low half of its byte) or c + 128, and stands for c * s, which bfloat16 holds
+ *           exactly. A group with a NaN, or a magnitude of 2^100 and more, is held as NaN.
+ * pos (device, [B]) is the position of each sequence's first new row, or NULL: pos_all for all of them.
+ * count (device, [B], or NULL: T) is how many of its T rows are there; the others are padding.
+ *
+ * ctdk_kvq_write holds k and v (fp32 or bfloat16; row t of sequence b at b * batch_stride +
+ * t * row_stride, its Hk heads of D values side by side; 16-byte aligned pointers and strides) at
+ * positions pos .. pos + count - 1. Padding, and rows whose position is outside the cache, leave it as it was.
+ * ctdk_kvq_read gives positions start .. start + length - 1 of every sequence back, each KV head
+ * repeated `group` times: k_out, v_out [B, Hk * group, length, D], fp32 or bfloat16 (both exact).
+ * ctdk_kvq_attn: query t of sequence b sits at i = pos + t and sees the positions j <= i (of the
+ * cache) with i - j < window (window 0: all of them) or j < sinks:
+ *   out[b, t, h] = sum_j softmax_j(scale * q[b, t, h] . k[b, h / (H / Hk), j]) v[b, h / (H / Hk), j]
+ * q, out: fp32 or bfloat16, both of the same type; out is [B, T, H, D]. A row that sees nothing (padding,
+ * and a row whose own position is outside the cache, among them) is zeros. Scores, maxima and sums are fp32; fp32 queries and the probabilities of fp32 outputs enter the products as
+ * two bfloat16 terms (within 2^-16 of the value), bfloat16 queries as they are. The result does not depend on what lies at
+ * positions that no query sees. workspace: device memory, 16-byte aligned, of ctdk_kvq_attn_workspace_bytes(cache, T, H) bytes
+ * (0: none needed), whose contents need not be kept; calls that may overlap need one each.
+ * ------------------------------------------------------------------------------------ */
+typedef struct {
+  void *k_codes, *k_scales, *v_codes, *v_scales;
+  int64_t B, capacity;
+  int Hk, D, bits;
+} ctdk_kvq_cache;
+
+int ctdk_kvq_write(const ctdk_kvq_cache* cache, const void* k, const void* v, int dtype,
+                   int64_t row_stride, int64_t batch_stride, int64_t T, const int32_t* pos,
+                   int64_t pos_all, const int32_t* count, void* stream);
+int ctdk_kvq_read(const ctdk_kvq_cache* cache, int64_t start, int64_t length, int group, int dtype,
+                  void* k_out, void* v_out, void* stream);
+int64_t ctdk_kvq_attn_workspace_bytes(const ctdk_kvq_cache* cache, int64_t T, int H);
+int ctdk_kvq_attn(const ctdk_kvq_cache* cache, const void* q, int dtype, int64_t row_stride,
+                  int64_t batch_stride, int64_t T, int H, const int32_t* pos, int64_t pos_all,
+                  const int32_t* count, int64_t window, int64_t sinks, float scale, void* out,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------
  * Optimizer. ctdk_sumsq adds sum(g^2) into out[0] (sum_sq_kernel_f32,
  * src/core/optim.cu:221-239). ctdk_adamw is one launch over a flat range of parameters:
  *   g' = g * grad_scale            (clip_grad_norm_'s scale, optim.cu:276-290; read from
