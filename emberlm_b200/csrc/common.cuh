@@ -49,6 +49,10 @@ int encode_tensor_map(CUtensorMap* map, const float* base, int rank, const uint6
 int encode_tensor_map_bf16(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
                            const uint32_t* box);
 
+// The same for bytes, rows of 32, 64 or 128 of them, swizzled within the row.
+int encode_tensor_map_u8(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                         const uint32_t* box);
+
 // Operands of a 3xTF32 product and their high and low parts (na and nb floats, multiples of four, 16-byte aligned).
 struct SplitOperands {
   const float *a, *b;

@@ -1174,6 +1174,25 @@ int encode_tensor_map_bf16(CUtensorMap* map, const void* base, int rank, const u
   return CTDK_OK;
 }
 
+int encode_tensor_map_u8(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                         const uint32_t* box) {
+  auto enc = encode_fn();
+  if (enc == nullptr) return fail(CTDK_ELAUNCH, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t d[5], st[4];
+  cuuint32_t bx[5], es[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+    es[i] = 1u;
+    if (i + 1 < rank) st[i] = strides_bytes[i];
+  }
+  const CUtensorMapSwizzle swizzle = box[0] == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : box[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, st, bx, es,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(CTDK_ELAUNCH, "cuTensorMapEncodeTiled failed (%d) for bytes", static_cast<int>(r));
+  return CTDK_OK;
+}
+
 int gemm_tcgen05_2cta_bf16(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, int tma_out, float* C,
                            int64_t ldc, int M, int N, int K, int vec_ok, int splits, int* status, cudaStream_t stream);
 

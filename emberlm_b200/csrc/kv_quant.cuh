@@ -32,37 +32,75 @@ __device__ __forceinline__ bool is_nan_scale(uint32_t bits) { return (bits & 0x7
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 
-// x * s + c on two bfloat16 values, one rounding.
-__device__ __forceinline__ uint32_t hfma2_bf16(uint32_t x, uint32_t s, uint32_t c) {
-  uint32_t d;
-  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(x), "r"(s), "r"(c));
-  return d;
-}
-__device__ __forceinline__ uint32_t hmul2_bf16(uint32_t x, uint32_t s) { return hfma2_bf16(x, s, 0x80008000u); }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// x * s + c on two bfloat16 (fp16) values, one rounding.
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t x, uint32_t s, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(x), "r"(s), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t x, uint32_t s) { return fma_bf16x2(x, s, 0x80008000u); }
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t x, uint32_t s, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(x), "r"(s), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t add_f16x2(uint32_t x, uint32_t c) {
+  uint32_t d;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(c));
+  return d;
+}
 
-// 4 bits: the codes at bits 4k and 4k + 16 of w, times the scales s2, as two bfloat16 values. The nibble under the
-// exponent of 128 is the number 128 + u; (128 + u) * s - 136 * s is rounded once and exact. b2 = bias4(s2).
-__device__ __forceinline__ uint32_t bias4(uint32_t s2) { return hmul2_bf16(s2, 0xc308c308u); }   // -136 * s
-template <int K>
-__device__ __forceinline__ uint32_t value4(uint32_t w, uint32_t s2, uint32_t b2) {
-  return hfma2_bf16(((w >> (4 * K)) & 0x000f000fu) | 0x43004300u, s2, b2);
+#endif  // __CUDACC__
+
+// Every conversion below is exact, one operation behind the extraction of the bits.
+// Bit patterns that the conversions need, as values that the compiler does not know: with two constants known in one
+// operation it spends a second one on it.
+struct Patterns {
+  uint32_t x43, x3f;                     // bfloat16 128, 1 / 2
+  uint32_t up15, up11, less4, less8;     // fp16 2^15, 2^11, -8 * 2^-9, -128 * 2^-9
+};
+inline Patterns patterns() { return {0x43004300u, 0x3f003f00u, 0x78007800u, 0x68006800u, 0xa400a400u, 0xb400b400u}; }
+
+#ifdef __CUDACC__
+// Codes times 2^-9 as fp16 numbers: the bits alone are the subnormal number u * 2^-24 (or 2^-20), which needs no exponent put over them.
+// 4-bit codes: of w's nibbles, pair i of out holds i and i + 4.
+constexpr int kCodeShift = 9;
+__device__ __forceinline__ void codes4_f16(uint32_t w, const Patterns& c, uint32_t (&out)[4]) {
+  const uint32_t v = w >> 8;
+  out[0] = fma_f16x2(w & 0x000f000fu, c.up15, c.less4);
+  out[1] = fma_f16x2(w & 0x00f000f0u, c.up11, c.less4);
+  out[2] = fma_f16x2(v & 0x000f000fu, c.up15, c.less4);
+  out[3] = fma_f16x2(v & 0x00f000f0u, c.up11, c.less4);
 }
-// 8 bits: byte K of w, as the fp32 number 2^23 + u.
-template <int K>
-__device__ __forceinline__ float magic8(uint32_t w) {
-  return __uint_as_float(prmt(w, 0x4b000000u, 0x7650u + K));
+// 8-bit codes: bytes 0, 1 and 2, 3.
+__device__ __forceinline__ void codes8_f16(uint32_t w, const Patterns& c, uint32_t (&out)[2]) {
+  out[0] = fma_f16x2(prmt(w, 0, 0x4140), c.up15, c.less8);
+  out[1] = fma_f16x2(prmt(w, 0, 0x4342), c.up15, c.less8);
 }
-// (2^23 + u) * s - (2^23 + 128) * s, exact, for two codes with scales s0, s1 and biases b = -(2^23 + 128) * s.
-__device__ __forceinline__ uint32_t values8(float f0, float f1, float s0, float s1, float b0, float b1) {
-  float x, y;
-  ffma2(x, y, f0, f1, s0, s1, b0, b1);
-  return pack_bf16(x, y);
+// Codes times their scales as bfloat16 numbers: the bits go under the exponent of a power of two.
+// 4 bits: nibble i of both halves of w, the halves' scales in s2.
+__device__ __forceinline__ uint32_t bias4(uint32_t s2) { return mul_bf16x2(s2, 0xc308c308u); }   // -136 s
+__device__ __forceinline__ void values4_bf16(uint32_t w, uint32_t s2, uint32_t b2, const Patterns& c, uint32_t (&out)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = fma_bf16x2(((w >> (4 * i)) & 0x000f000fu) | c.x43, s2, b2);   // (128 + u) s - 136 s
 }
-__device__ __forceinline__ float bias8(float s) { return s * -8388736.0f; }
+// 8 bits: byte i of both halves of w. The mantissa takes seven bits; the eighth moves the exponent of a half.
+struct Scale8 {
+  uint32_t s, b, t;                      // s, -384 s, 256 s
+};
+__device__ __forceinline__ Scale8 scale8(uint32_t s2) { return {s2, mul_bf16x2(s2, 0xc3c0c3c0u), mul_bf16x2(s2, 0x43804380u)}; }
+__device__ __forceinline__ void values8_bf16(uint32_t w, const Scale8& s, const Patterns& c, uint32_t (&out)[2]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t v = w >> (8 * i);
+    const uint32_t low = fma_bf16x2((v & 0x007f007fu) | c.x43, s.s, s.b);   // (128 + u mod 128) s - 384 s
+    out[i] = fma_bf16x2((v & 0x00800080u) | c.x3f, s.t, low);               // + 128 s or 256 s
+  }
+}
 
 #endif  // __CUDACC__
 

@@ -2,18 +2,20 @@
 // groups. out = sum_j softmax_j(scale * q . k_j) v_j, over the positions that a row sees.
 //
 // A block of R <= 8 * NT rows (the query heads of one key/value head times the new tokens) shares the cache rows, which
-// are read once. Warps work alone, each on tiles of 2 KB of key codes (16 to 64 positions), which bulk copies
-// bring into the warp's two stages of shared memory; the codes become exact bfloat16 values in registers, in the layout
+// are read once. Warps work alone, each on tiles of 2 KB of key codes (16 to 64 positions), which TMA brings
+// into the warp's two stages of shared memory; the codes become exact 16-bit floating numbers in registers, in the layout
 // that mma.sync wants, without another trip through shared memory:
-//   scores   S^T[16 positions, 8 rows] = K Q^T: a lane takes a quarter of the columns of two positions; which columns meet in
-//            which step of the product is free, as long as Q is laid out the same, so a lane's codes are consecutive bytes;
+//   scores   S^T[16 positions, 8 rows] = K Q^T: ldmatrix gives a lane a word of codes of one group and position; which columns meet
+//            in which step of the product is free, as long as Q is laid out the same. The codes enter as fp16 numbers, unscaled, a
+//            group at a time, and the group's scale joins in fp32 afterwards: that saves half of the shifts of a bfloat16
+//            conversion, and fp32 queries keep 22 bits in two fp16 terms (after a power of two has brought the row near 64);
 //   softmax  maximum, exponentials and sums in fp32, in the log2 domain; the reference point moves only when a score exceeds it
 //            by more than 2^8, so that most tiles need one vote instead of a reduction over the warp;
-//   output   O^T[16 columns, 8 rows] += V^T P^T: V's fragments pair the codes of two positions (byte permutes), P comes from the
-//            scores' fragments by an 8 x 8 transposition (movmatrix).
-// fp32 queries and, for fp32 outputs, the probabilities enter as two bfloat16 terms: what that leaves out, at most 2^-16 of a
-// term (2^-18 on average), is within the bound of rounding an fp32 sum of 256 terms.
+//   output   O^T[16 columns, 8 rows] += V^T P^T: ldmatrix.trans pairs the codes of two positions, which become c * s in bfloat16; P
+//            comes from the scores' fragments by an 8 x 8 transposition (movmatrix). For fp32 outputs it enters as three bfloat16
+//            terms (24 bits), for bfloat16 outputs as one.
 #include <climits>
+#include <type_traits>
 
 #include "kv_quant_attn.h"
 #include "mma_bf16.cuh"
@@ -30,40 +32,84 @@ struct Tile {
   static constexpr int kRow = D * BITS / 8, kScaleRow = D / kGroup * 2;   // bytes of a position
   static constexpr int kKeys = 2048 / kRow;                               // positions of a tile
   static constexpr int kCodes = kKeys * kRow, kScales = kKeys * kScaleRow;
-  static constexpr int kStage = 2 * (kCodes + kScales);                   // key codes, value codes, key scales, value scales
+  static constexpr int kStage = 2 * (kCodes + kScales);                   // bytes that one tile brings
   static constexpr int kPitch = D + 4;                                    // floats of a row in the exchange of partial results
   static constexpr int kExchange = kWarps * 8 * kPitch * 4;
-  static constexpr int kSmem = kWarps * kStages * kStage + kExchange;
+  static constexpr int kSmem = 1024 + kWarps * kStages * kStage + kExchange;
 };
-
-// Row m of a block of 16 positions holds position place(m): neighbours in m differ in parity, and so do m and m + 2, which
-// keeps the keys' and the values' reads of 64-byte rows off each other's banks.
-__device__ __forceinline__ int place(int m) { return m ^ ((m >> 1) & 1); }
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same without a third operand.
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t lds16(uint32_t a) {
   unsigned short v;
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
   return v;
 }
+__device__ __forceinline__ void lds_words(uint32_t (&w)[1], uint32_t a) { asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(a)); }
+__device__ __forceinline__ void lds_words(uint32_t (&w)[2], uint32_t a) {
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
+}
+__device__ __forceinline__ void lds_words(uint32_t (&w)[4], uint32_t a) {
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ void unpack_f16(uint32_t w, float& lo, float& hi) {
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.f32.f16 %0, a;\n cvt.f32.f16 %1, b;\n}" : "=f"(lo), "=f"(hi) : "r"(w));
+}
+// (x, y) as N packed terms, each the rest of the ones before, rounded.
 template <int N>
-__device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t a) {
-  static_assert(N == 1 || N == 2 || N == 4 || N == 8, "words");
-  if constexpr (N == 1) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(a));
-  if constexpr (N == 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
-  if constexpr (N >= 4)
+__device__ __forceinline__ void terms_f16(float x, float y, uint32_t (&t)[N]) {
 #pragma unroll
-    for (int i = 0; i < N; i += 4)
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "r"(a + 4 * i));
+  for (int i = 0; i < N; ++i) {
+    t[i] = pack_f16(x, y);
+    if (i + 1 < N) {
+      float u, v;
+      unpack_f16(t[i], u, v);
+      x -= u, y -= v;
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ void terms_bf16(float x, float y, uint32_t (&t)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    t[i] = pack_bf16(x, y);
+    if (i + 1 < N) {
+      x -= __uint_as_float(t[i] << 16);
+      y -= __uint_as_float(t[i] & 0xffff0000u);
+    }
+  }
 }
 
 struct Span {
   int64_t lo, hi;      // tiles of all units, numbered through
 };
+// As bulk_load of common.cuh, without a cache hint.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
+               "r"(smem_u32(bar))
+               : "memory");
+}
 // A CTA's place in the list of units (sequence, key/value head): the unit it is at, and where that unit's tiles lie.
 struct Unit {
   int b, h;
@@ -75,6 +121,19 @@ struct TokenArgs {
   AttnArgs a;
   int rows;            // T * group
   int split;           // 0: one CTA a unit (and a block of 8 * NT rows); 1: equal spans of all tiles
+  Patterns bits;
+};
+
+// What a warp's loads go by. A run: its tiles of one unit that lie evenly spaced (all sink tiles, or all others).
+struct Feed {
+  int j, n, bh, left;                    // next position, tiles left in the run; key/value head; tiles left after the run
+  int plain_lo, plain_hi, loaded, pad;   // tiles from position plain_lo to plain_hi are seen whole by every row
+  Unit u;
+  int64_t hi;
+  int at, end;                           // tile of the unit behind the run; tiles of the unit that are this CTA's
+};
+struct Maps {
+  CUtensorMap m[2];                      // codes of keys, of values
 };
 
 __device__ __forceinline__ int64_t pos_of(const AttnArgs& a, int b) { return a.pos != nullptr ? static_cast<int64_t>(a.pos[b]) : a.pos_all; }
@@ -101,6 +160,26 @@ __device__ __forceinline__ void next_unit(const AttnArgs& a, Unit& u) {
   } while (u.v.tiles == 0 && u.b + 1 < a.c.B);
   u.begin = u.end;
   u.end += u.v.tiles;
+}
+
+// The next run of a warp's tiles.
+template <int KEYS>
+__device__ __forceinline__ void next_run(const AttnArgs& a, Feed& f) {
+  while (f.at >= f.end) {
+    f.at -= static_cast<int>(f.u.end - f.u.begin);
+    next_unit<KEYS>(a, f.u);
+    f.end = static_cast<int>(min(f.u.end, f.hi) - f.u.begin);
+  }
+  const Visit& v = f.u.v;
+  const bool sink = f.at < v.sink_tiles;
+  const int behind = sink ? min(v.sink_tiles, f.end) : f.end;
+  f.n = (behind - f.at + kWarps - 1) / kWarps;
+  f.left -= f.n;
+  f.j = v.tile_at(f.at) * KEYS;
+  f.bh = f.u.b * a.c.Hk + f.u.h;
+  f.at += f.n * kWarps;
+  f.plain_lo = sink || a.window == 0 ? 0 : v.hi_row - a.window;
+  f.plain_hi = sink ? min(a.sinks - KEYS, v.lo_row - KEYS + 1) : v.lo_row - KEYS + 1;
 }
 
 __device__ __forceinline__ int64_t span_start(int64_t all, int i, int n) { return all * i / n; }
@@ -180,20 +259,28 @@ struct Part {
 };
 
 template <typename QT, int D, int BITS, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kvq_token_kernel(const TokenArgs ta) {
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
+    kvq_token_kernel(const __grid_constant__ Maps maps, const TokenArgs ta) {
   using TL = Tile<D, BITS>;
-  constexpr int KEYS = TL::kKeys, BLOCKS = KEYS / 16;
-  constexpr bool kSplitQ = sizeof(QT) == 4;            // two bfloat16 terms
-  constexpr int NS = kSplitQ ? 2 : 1;
-  constexpr int KW = TL::kRow / 16, VW = TL::kRow / 32;   // words of a lane's share of a position: a quarter of the keys', an eighth of the values'
-  extern __shared__ __align__(128) unsigned char smem[];
+  constexpr int KEYS = TL::kKeys, BLOCKS = KEYS / 16, GROUPS = D / kGroup, STEPS = D / 16, ROW = TL::kRow;
+  constexpr int NQ = sizeof(QT) == 4 ? 2 : 1, NP = sizeof(QT) == 4 ? 3 : 1;   // terms of a query, of a probability
+  constexpr int SW = GROUPS / 2;                       // words of a position's scales
+  extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t bars[kWarps * kStages];
   __shared__ int64_t scan[kWarps];
   __shared__ float row_m[kWarps][8 * NT], row_l[kWarps][8 * NT];
+  __shared__ Feed feed[kWarps];
+  __shared__ int place[kWarps][kStages];               // a stage's first position, its complement where not every row sees all of it
+  __shared__ Unit unit;                                // that the CTA is at
   const AttnArgs& a = ta.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3;
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   if (threadIdx.x < kWarps * kStages) mbar_init(&bars[threadIdx.x], 1);
-  if (threadIdx.x == 0) mbar_fence_init();
+  if (threadIdx.x == 0) {
+    mbar_fence_init();
+    tma_prefetch_desc(&maps.m[0]);
+    tma_prefetch_desc(&maps.m[1]);
+  }
   pdl_launch();
   __syncthreads();
   pdl_wait();
@@ -223,73 +310,103 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kvq_token_kernel
   }
   const int rows = min(8 * NT, ta.rows - r0);
 
-  unsigned char* mine = smem + warp * kStages * TL::kStage;
-  uint64_t* bar = &bars[warp * kStages];
   float* exchange = reinterpret_cast<float*>(smem + kWarps * kStages * TL::kStage);
 
-  // Loads run ahead of the products, over the units' borders.
-  Unit lu = u;
-  int64_t load_at = span.lo + warp;
-  int loaded = 0;
-  uint64_t policy;
-  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  // Loads run ahead of the products, over the units' borders. What they go by lies in shared memory: only lane 0 needs it, and
+  // the products need the registers. Tile numbers count from the unit's first.
+  if (lane == 0) {
+    Feed& f = feed[warp];
+    f.u = u;
+    f.hi = span.hi;
+    f.left = static_cast<int>((span.hi - span.lo - warp + kWarps - 1) / kWarps);   // of this warp's tiles (it may be <= 0)
+    f.at = static_cast<int>(span.lo - u.begin) + warp;
+    f.end = static_cast<int>(min(u.end, span.hi) - u.begin);
+    f.n = f.loaded = 0;
+  }
+  if (threadIdx.x == 0) unit = u;
+  __syncwarp();
   auto load = [&]() {
-    if (load_at >= span.hi) return;
-    while (load_at >= lu.end) next_unit<KEYS>(a, lu);
-    if (lane == 0) {
-      const int64_t j = (static_cast<int64_t>(lu.b) * a.c.Hk + lu.h) * a.c.capacity + static_cast<int64_t>(lu.v.tile_at(static_cast<int>(load_at - lu.begin))) * KEYS;
-      unsigned char* dst = mine + (loaded % kStages) * TL::kStage;
-      uint64_t* full = &bar[loaded % kStages];
-      mbar_expect_tx(full, TL::kStage);
-      bulk_load(dst, a.c.codes[0] + j * TL::kRow, TL::kCodes, full, policy);
-      bulk_load(dst + 2 * TL::kCodes, a.c.scales[0] + j * (D / kGroup), TL::kScales, full, policy);
-      bulk_load(dst + TL::kCodes, a.c.codes[1] + j * TL::kRow, TL::kCodes, full, policy);
-      bulk_load(dst + 2 * TL::kCodes + TL::kScales, a.c.scales[1] + j * (D / kGroup), TL::kScales, full, policy);
+    Feed& f = feed[warp];
+    if (f.n == 0) {                                    // the same for all lanes
+      if (f.left <= 0) return;
+      __syncwarp();
+      if (lane == 0) next_run<KEYS>(a, f);
+      __syncwarp();
     }
-    ++loaded;
-    load_at += kWarps;
+    const int j = f.j, bh = f.bh, st = f.loaded % kStages;
+    __syncwarp();
+    uint64_t* full = &bars[warp * kStages + st];
+    if (lane == 0) {
+      f.j = j + kWarps * KEYS;
+      --f.n;
+      ++f.loaded;
+      place[warp][st] = j >= f.plain_lo && j <= f.plain_hi ? j : ~j;
+      mbar_expect_tx(full, TL::kStage);
+    }
+    __syncwarp();
+    if (lane < 2) {                                    // keys, values
+      tma_load_3d(smem + ((warp * kStages + st) * 2 + lane) * TL::kCodes, &maps.m[lane], full, 0, j, bh);
+      bulk_load(smem + kWarps * kStages * 2 * TL::kCodes + ((warp * kStages + st) * 2 + lane) * TL::kScales,
+                (lane ? a.c.scales[1] : a.c.scales[0]) + (static_cast<int64_t>(bh) * a.c.capacity + j) * GROUPS, TL::kScales, full);
+    }
+    __syncwarp();
   };
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < kStages; ++i) load();
+  __syncthreads();
+
+  // A lane's row address for ldmatrix (16 rows, two neighbouring chunks of 16 bytes), swizzled as TMA has written it.
+  const uint32_t row16 = static_cast<uint32_t>(lane & 15) * ROW;
+  const uint32_t lane_at = row16 + ((static_cast<uint32_t>(lane >> 4) * 16u) ^ ((row16 >> 3) & (ROW - 16u)));
 
   int used = 0;
   bool ok = true;
-  int64_t at = span.lo + warp;
-  for (int64_t seg = span.lo;;) {                      // one unit after the other
-    const int64_t seg_end = min(u.end, span.hi);
-    const int64_t pos = pos_of(a, u.b), count = count_of(a, u.b);
-    // Q's fragments: column (a row of queries) g of tile n; b0, b1 of product step ks in the lane's own order of columns.
-    uint32_t qf[NT][D / 16][NS][2];
+  int ck = static_cast<int>(span.lo - unit.begin) + warp;
+  for (;;) {                                           // one unit after the other
+    const int cend = static_cast<int>(min(unit.end, span.hi) - unit.begin), ub = unit.b, uh = unit.h;
+    const int64_t pos = pos_of(a, ub), count = count_of(a, ub);
+    // Q's fragments: column (a row of queries) g of tile n; b0, b1 of product step ks in the order in which the codes come.
+    uint32_t qf[NT][STEPS][NQ][2];
+    float factor[NT][2];                               // of rows 2 tig, 2 tig + 1: score to log2 domain
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int r = r0 + 8 * n + g, t = r / a.group;
       const bool live = 8 * n + g < rows;
-      const QT* src = static_cast<const QT*>(a.q) + u.b * a.batch_stride + static_cast<int64_t>(t) * a.row_stride +
-                      static_cast<int64_t>(u.h * a.group + (r - t * a.group)) * D + tig * (D / 4);
+      const QT* src = static_cast<const QT*>(a.q) + ub * a.batch_stride + static_cast<int64_t>(t) * a.row_stride +
+                      static_cast<int64_t>(uh * a.group + (r - t * a.group)) * D;
+      float x[STEPS][4], most = 0.0f;
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        int d[4];
-        if (BITS == 4) {                               // words of eight codes: two steps, pairs (c, c + 4)
-          const int w = 8 * (ks / 2) + 2 * (ks & 1);
-          d[0] = w, d[1] = w + 4, d[2] = w + 1, d[3] = w + 5;
-        } else {
-          d[0] = 4 * ks, d[1] = 4 * ks + 1, d[2] = 4 * ks + 2, d[3] = 4 * ks + 3;
-        }
-        float x[4];
+      for (int ks = 0; ks < STEPS; ++ks)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = live ? static_cast<float>(src[d[i]]) : 0.0f;
-        if constexpr (kSplitQ) {
-          split_bf16x2(x[0], x[1], qf[n][ks][0][0], qf[n][ks][1][0]);
-          split_bf16x2(x[2], x[3], qf[n][ks][0][1], qf[n][ks][1][1]);
-        } else {
-          qf[n][ks][0][0] = pack_bf16(x[0], x[1]);
-          qf[n][ks][0][1] = pack_bf16(x[2], x[3]);
+        for (int i = 0; i < 4; ++i) {
+          // 4 bits: a word of eight codes gives two steps, pairs (c, c + 4); 8 bits: a word of four gives one
+          const int d = BITS == 4 ? 32 * (ks / 2) + 8 * tig + 2 * (ks & 1) + (i >> 1) + 4 * (i & 1) : 16 * ks + 4 * tig + i;
+          x[ks][i] = live ? static_cast<float>(src[d]) : 0.0f;
+          most = fmaxf(most, fabsf(x[ks][i]));
         }
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const int e = static_cast<int>(__float_as_uint(most) >> 23) - 127;           // 128: not finite
+      const int up = most == 0.0f || e == 128 ? 0 : max(min(6 - e, 126), -110);    // most * 2^up is in [64, 128), or near it
+      const float f = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+#pragma unroll
+      for (int ks = 0; ks < STEPS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t tt[NQ];
+          terms_f16<NQ>(x[ks][2 * i] * f, x[ks][2 * i + 1] * f, tt);
+#pragma unroll
+          for (int y = 0; y < NQ; ++y) qf[n][ks][y][i] = tt[y];
+        }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int other = __shfl_sync(0xffffffffu, up, (2 * tig + c) * 4);
+        factor[n][c] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + kCodeShift - other) << 23);   // other is 126 at most
       }
     }
     // Rows 2 tig and 2 tig + 1 of tile n: their positions, reference points (log2 domain) and sums.
     int at_row[NT][2];
-    float m[NT][2], l[NT][2], o[NT][D / 16][4];
+    float m[NT][2], l[NT][2], o[NT][STEPS][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -300,75 +417,74 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kvq_token_kernel
         l[n][c] = 0.0f;
       }
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i)
+      for (int i = 0; i < STEPS; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[n][i][c] = 0.0f;
     }
 
-    for (; at < seg_end; at += kWarps) {
-      const int j0 = u.v.tile_at(static_cast<int>(at - u.begin)) * KEYS;
-      const int stage = used % kStages;
-      ok = ok && mbar_wait_bounded_w(&bar[stage], (used / kStages) & 1, a.status, 210);
-      if (!ok) break;
-      const uint32_t base = smem_u32(mine + stage * TL::kStage), vbase = base + TL::kCodes;
-      const uint32_t ksc = base + 2 * TL::kCodes, vsc = ksc + TL::kScales;
-      // every valid row sees every position of most tiles
-      const bool plain = j0 + KEYS - 1 <= u.v.lo_row && (a.window == 0 || u.v.hi_row - 1 - j0 < a.window || j0 + KEYS <= a.sinks);
+    // One tile; PLAIN: every valid row sees all of it.
+    auto tile = [&](auto plain, int j0, uint32_t kbase, uint32_t ksc) {
+      constexpr bool PLAIN = decltype(plain)::value;
+      const uint32_t vbase = kbase + TL::kCodes, vsc = ksc + TL::kScales;
       float s[BLOCKS][NT][4];
       // ---- scores
 #pragma unroll
       for (int k = 0; k < BLOCKS; ++k) {
-        uint32_t w[2][KW], s2[2], b2[2];
-        float sf[2], bf[2];
+        uint32_t sc[2][SW];
+        lds_words(sc[0], ksc + (16 * k + g) * TL::kScaleRow);
+        lds_words(sc[1], ksc + (16 * k + 8 + g) * TL::kScaleRow);
+        float acc[NT][4];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const int tok = 16 * k + place(g + 8 * hf);
-          lds_words(w[hf], base + tok * TL::kRow + tig * (TL::kRow / 4));
-          const uint32_t sc = lds16(ksc + tok * TL::kScaleRow + (tig * (D / 4) / kGroup) * 2);
-          if (BITS == 4) {
-            s2[hf] = prmt(sc, 0, 0x1010);
-            b2[hf] = bias4(s2[hf]);
-          } else {
-            sf[hf] = __uint_as_float(sc << 16);
-            bf[hf] = bias8(sf[hf]);
-          }
-        }
+        for (int x = 0; x < ROW / 32; ++x) {           // two chunks of 16 bytes: two groups of 4-bit codes, one of 8-bit codes
+          uint32_t w[4];                               // chunk 2 x of positions g, g + 8; chunk 2 x + 1 of both
+          ldsm4(w, kbase + k * 16 * ROW + (lane_at ^ (32u * x)));
+          auto step = [&](int ks, const uint32_t (&f)[4]) {   // a group is two steps
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) s[k][n][c] = 0.0f;
-        float lo[NT][4] = {};
-#pragma unroll
-        for (int x = 0; x < KW; ++x) {
-          uint32_t f[2][4];
-          if constexpr (BITS == 4) {
-            f[0][0] = value4<0>(w[0][x], s2[0], b2[0]), f[0][1] = value4<0>(w[1][x], s2[1], b2[1]);
-            f[0][2] = value4<1>(w[0][x], s2[0], b2[0]), f[0][3] = value4<1>(w[1][x], s2[1], b2[1]);
-            f[1][0] = value4<2>(w[0][x], s2[0], b2[0]), f[1][1] = value4<2>(w[1][x], s2[1], b2[1]);
-            f[1][2] = value4<3>(w[0][x], s2[0], b2[0]), f[1][3] = value4<3>(w[1][x], s2[1], b2[1]);
-          } else {
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-              f[0][hf] = values8(magic8<0>(w[hf][x]), magic8<1>(w[hf][x]), sf[hf], sf[hf], bf[hf], bf[hf]);
-              f[0][2 + hf] = values8(magic8<2>(w[hf][x]), magic8<3>(w[hf][x]), sf[hf], sf[hf], bf[hf], bf[hf]);
-            }
-          }
-#pragma unroll
-          for (int y = 0; y < (BITS == 4 ? 2 : 1); ++y) {
-            const int ks = BITS == 4 ? 2 * x + y : x;
+              for (int y = 0; y < NQ; ++y) {
+                if ((ks & 1) == 0 && y == 0) mma_f16_first(acc[n], f, qf[n][ks][y][0], qf[n][ks][y][1]);
+                else mma_f16(acc[n], f, qf[n][ks][y][0], qf[n][ks][y][1]);
+              }
+          };
+          auto scaled = [&](int gr) {
+            const float s0 = __uint_as_float(gr & 1 ? sc[0][gr / 2] & 0xffff0000u : sc[0][gr / 2] << 16);
+            const float s1 = __uint_as_float(gr & 1 ? sc[1][gr / 2] & 0xffff0000u : sc[1][gr / 2] << 16);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              mma_bf16(s[k][n], f[y], qf[n][ks][0][0], qf[n][ks][0][1]);
-              if constexpr (kSplitQ) mma_bf16(lo[n], f[y], qf[n][ks][NS - 1][0], qf[n][ks][NS - 1][1]);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) s[k][n][c] = gr == 0 ? acc[n][c] * (c < 2 ? s0 : s1) : fmaf(acc[n][c], c < 2 ? s0 : s1, s[k][n][c]);
             }
+          };
+          if constexpr (BITS == 4) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              uint32_t p[4], q[4];
+              codes4_f16(w[2 * y], ta.bits, p);
+              codes4_f16(w[2 * y + 1], ta.bits, q);
+              const uint32_t f0[4] = {p[0], q[0], p[1], q[1]}, f1[4] = {p[2], q[2], p[3], q[3]};
+              step(4 * x + 2 * y, f0);
+              step(4 * x + 2 * y + 1, f1);
+              scaled(2 * x + y);
+            }
+          } else {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              uint32_t p[2], q[2];
+              codes8_f16(w[2 * y], ta.bits, p);
+              codes8_f16(w[2 * y + 1], ta.bits, q);
+              const uint32_t f[4] = {p[0], q[0], p[1], q[1]};
+              step(2 * x + y, f);
+            }
+            scaled(x);
           }
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            s[k][n][c] = (s[k][n][c] + lo[n][c]) * a.scale_log2;
-            if (!plain && !sees(at_row[n][c & 1], j0 + 16 * k + place(g + 8 * (c >> 1)), a.window, a.sinks)) s[k][n][c] = -INFINITY;
+            s[k][n][c] *= factor[n][c & 1];
+            if (!PLAIN && !sees(at_row[n][c & 1], j0 + 16 * k + g + 8 * (c >> 1), a.window, a.sinks)) s[k][n][c] = -INFINITY;
           }
       }
       // ---- reference points
@@ -396,7 +512,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kvq_token_kernel
             m[n][c] = x;
             l[n][c] *= f;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
+            for (int i = 0; i < STEPS; ++i) {
               o[n][i][c] *= f;
               o[n][i][c + 2] *= f;
             }
@@ -410,7 +526,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kvq_token_kernel
         for (int c = 0; c < 2; ++c) ref[n][c] = m[n][c] == -INFINITY ? 0.0f : m[n][c];
 #pragma unroll
       for (int k = 0; k < BLOCKS; ++k) {
-        uint32_t pf[NT][NS][2];
+        uint32_t pf[NT][NP][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float p[4];
@@ -418,91 +534,98 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kvq_token_kernel
           for (int c = 0; c < 4; ++c) p[c] = ex2(s[k][n][c] - ref[n][c & 1]);
           l[n][0] += p[0] + p[2];
           l[n][1] += p[1] + p[3];
-          if constexpr (kSplitQ) {
-            split_bf16x2(p[0], p[1], pf[n][0][0], pf[n][NS - 1][0]);
-            split_bf16x2(p[2], p[3], pf[n][0][1], pf[n][NS - 1][1]);
-          } else {
-            pf[n][0][0] = pack_bf16(p[0], p[1]);
-            pf[n][0][1] = pack_bf16(p[2], p[3]);
-          }
 #pragma unroll
-          for (int x = 0; x < NS; ++x) {
-            pf[n][x][0] = movmatrix(pf[n][x][0]);
-            pf[n][x][1] = movmatrix(pf[n][x][1]);
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t tt[NP];
+            terms_bf16<NP>(p[2 * hf], p[2 * hf + 1], tt);
+#pragma unroll
+            for (int y = 0; y < NP; ++y) pf[n][y][hf] = movmatrix(tt[y]);
           }
         }
-        uint32_t w[4][VW], sc[4];                      // positions 2 tig, 2 tig + 1, 2 tig + 8, 2 tig + 9 of the block
+        uint32_t s2[2][GROUPS];                        // scales of positions (2 tig, 2 tig + 1) and (2 tig + 8, 2 tig + 9)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int m16 = 2 * tig + (i & 1) + 8 * (i >> 1), tok = 16 * k + place(m16);
-          lds_words(w[i], vbase + tok * TL::kRow + g * (TL::kRow / 8));
-          sc[i] = lds16(vsc + tok * TL::kScaleRow + (g * (D / 8) / kGroup) * 2);
-          if (!plain) {
+        for (int hf = 0; hf < 2; ++hf) {
+          const int tok = 16 * k + 2 * tig + 8 * hf;
+          uint32_t sc[2 * SW];
+          lds_words(sc, vsc + tok * TL::kScaleRow);
+          if (!PLAIN) {
             // A probability of zero must not meet a NaN: positions that no row sees count as zeros, and so, here, do
             // groups that are NaN themselves; the rows that see one of those get their NaN below.
-            if (j0 + tok >= u.v.hi_row || is_nan_scale(sc[i])) sc[i] = 0;
-          }
-        }
-        uint32_t s2[2], b2[2];
-        float sf[4], bf[4];
-        if (BITS == 4) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            s2[i] = prmt(sc[2 * i], sc[2 * i + 1], 0x5410);
-            b2[i] = bias4(s2[i]);
+            for (int i = 0; i < 2 * SW; ++i) {
+              if (j0 + tok + i / SW >= unit.v.hi_row) sc[i] = 0;
+              if (is_nan_scale(sc[i])) sc[i] &= 0xffff0000u;
+              if (is_nan_scale(sc[i] >> 16)) sc[i] &= 0x0000ffffu;
+            }
           }
-        } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            sf[i] = __uint_as_float(sc[i] << 16);
-            bf[i] = bias8(sf[i]);
-          }
+          for (int gr = 0; gr < GROUPS; ++gr) s2[hf][gr] = prmt(sc[gr / 2], sc[SW + gr / 2], gr & 1 ? 0x7632 : 0x5410);
         }
         auto product = [&](int i, const uint32_t (&f)[4]) {
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int x = 0; x < NS; ++x) mma_bf16(o[n][i], f, pf[n][x][0], pf[n][x][1]);
+            for (int y = 0; y < NP; ++y) mma_bf16(o[n][i], f, pf[n][y][0], pf[n][y][1]);
         };
 #pragma unroll
-        for (int x = 0; x < VW; ++x) {
+        for (int x = 0; x < ROW / 32; ++x) {
+          uint32_t w[4];                               // chunk 2 x of both pairs of positions, chunk 2 x + 1 of both
+          ldsm4_trans(w, vbase + k * 16 * ROW + (lane_at ^ (32u * x)));
           if constexpr (BITS == 4) {
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {              // halves of the words: codes 4 y .. 4 y + 3 of both positions
-              const uint32_t e = prmt(w[0][x], w[1][x], y ? 0x7632 : 0x5410), f = prmt(w[2][x], w[3][x], y ? 0x7632 : 0x5410);
-              const uint32_t f0[4] = {value4<0>(e, s2[0], b2[0]), value4<1>(e, s2[0], b2[0]), value4<0>(f, s2[1], b2[1]), value4<1>(f, s2[1], b2[1])};
-              const uint32_t f1[4] = {value4<2>(e, s2[0], b2[0]), value4<3>(e, s2[0], b2[0]), value4<2>(f, s2[1], b2[1]), value4<3>(f, s2[1], b2[1])};
-              product(4 * x + 2 * y, f0);
-              product(4 * x + 2 * y + 1, f1);
+            for (int y = 0; y < 2; ++y) {              // a chunk is a group: columns 4 g .. 4 g + 3 of it
+              const int gr = 2 * x + y;
+              uint32_t p[4], q[4];
+              values4_bf16(w[2 * y], s2[0][gr], bias4(s2[0][gr]), ta.bits, p);
+              values4_bf16(w[2 * y + 1], s2[1][gr], bias4(s2[1][gr]), ta.bits, q);
+              const uint32_t f0[4] = {p[0], p[1], q[0], q[1]}, f1[4] = {p[2], p[3], q[2], q[3]};
+              product(2 * gr, f0);
+              product(2 * gr + 1, f1);
             }
           } else {
-            const uint32_t f0[4] = {values8(magic8<0>(w[0][x]), magic8<0>(w[1][x]), sf[0], sf[1], bf[0], bf[1]),
-                                    values8(magic8<1>(w[0][x]), magic8<1>(w[1][x]), sf[0], sf[1], bf[0], bf[1]),
-                                    values8(magic8<0>(w[2][x]), magic8<0>(w[3][x]), sf[2], sf[3], bf[2], bf[3]),
-                                    values8(magic8<1>(w[2][x]), magic8<1>(w[3][x]), sf[2], sf[3], bf[2], bf[3])};
-            const uint32_t f1[4] = {values8(magic8<2>(w[0][x]), magic8<2>(w[1][x]), sf[0], sf[1], bf[0], bf[1]),
-                                    values8(magic8<3>(w[0][x]), magic8<3>(w[1][x]), sf[0], sf[1], bf[0], bf[1]),
-                                    values8(magic8<2>(w[2][x]), magic8<2>(w[3][x]), sf[2], sf[3], bf[2], bf[3]),
-                                    values8(magic8<3>(w[2][x]), magic8<3>(w[3][x]), sf[2], sf[3], bf[2], bf[3])};
-            product(2 * x, f0);
-            product(2 * x + 1, f1);
+            const Scale8 c0 = scale8(s2[0][x]), c1 = scale8(s2[1][x]);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {              // a chunk is half a group: columns 2 g, 2 g + 1 of it
+              uint32_t p[2], q[2];
+              values8_bf16(w[2 * y], c0, ta.bits, p);
+              values8_bf16(w[2 * y + 1], c1, ta.bits, q);
+              const uint32_t f[4] = {p[0], p[1], q[0], q[1]};
+              product(2 * x + y, f);
+            }
           }
         }
       }
-      if (!plain) {                                    // NaN groups of values: the rows that see them
+      if (!PLAIN) {                                    // NaN groups of values: the rows that see them
         bool nan = false;
-        for (int i = lane; i < KEYS * (D / kGroup); i += 32) nan |= is_nan_scale(lds16(vsc + 2 * i)) && j0 + i / (D / kGroup) < u.v.hi_row;
+        for (int i = lane; i < KEYS * GROUPS; i += 32) nan |= is_nan_scale(lds16(vsc + 2 * i)) && j0 + i / GROUPS < unit.v.hi_row;
         if (__any_sync(0xffffffffu, nan)) {
+#pragma unroll 1
           for (int i = 0; i < KEYS; ++i)
-            if (is_nan_scale(lds16(vsc + i * TL::kScaleRow + (g * (D / 8) / kGroup) * 2)))
 #pragma unroll
-              for (int n = 0; n < NT; ++n)
+            for (int gr = 0; gr < GROUPS; ++gr)
+              if (is_nan_scale(lds16(vsc + i * TL::kScaleRow + gr * 2)))
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
-                  if (sees(at_row[n][c], j0 + i, a.window, a.sinks))
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int x = 0; x < D / 16; ++x) o[n][x][c] = o[n][x][c + 2] = __int_as_float(0x7fc00000);
+                  for (int c = 0; c < 2; ++c)
+                    if (sees(at_row[n][c], j0 + i, a.window, a.sinks))
+#pragma unroll
+                      for (int x = 2 * gr; x < 2 * gr + 2; ++x) o[n][x][c] = o[n][x][c + 2] = __int_as_float(0x7fc00000);
         }
+      }
+    };
+
+    for (; ck < cend; ck += kWarps) {
+      const int stage = used % kStages;
+      ok = ok && mbar_wait_bounded_w(&bars[warp * kStages + stage], (used / kStages) & 1, a.status, 210);
+      if (!ok) break;
+      const uint32_t kbase = smem_u32(smem) + (warp * kStages + stage) * 2 * TL::kCodes;
+      const uint32_t ksc = smem_u32(smem) + kWarps * kStages * 2 * TL::kCodes + (warp * kStages + stage) * 2 * TL::kScales;
+      const int j0 = place[warp][stage];
+      if (j0 >= 0) {
+        tile(std::true_type{}, j0, kbase, ksc);
+      } else {
+        tile(std::false_type{}, ~j0, kbase, ksc);
       }
       __syncwarp();
       ++used;
@@ -522,13 +645,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kvq_token_kernel
           row_l[warp][8 * n + 2 * tig + c] = x;
         }
       }
-    const bool whole = u.begin >= span.lo && u.end <= span.hi;
+    const bool whole = unit.begin >= span.lo && unit.end <= span.hi;
     float* part = nullptr;
-    if (!whole) part = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (u.begin < span.lo ? 0 : 1)) * Part<D, NT>::kFloats;
+    if (!whole) part = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (unit.begin < span.lo ? 0 : 1)) * Part<D, NT>::kFloats;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
+      for (int i = 0; i < STEPS; ++i) {
         float* e = exchange + (warp * 8 + 2 * tig) * TL::kPitch + 16 * i + g;
         e[0] = o[n][i][0];
         e[TL::kPitch] = o[n][i][1];
@@ -550,8 +673,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kvq_token_kernel
           ll += f * row_l[w][rr];
           sum += f * exchange[(w * 8 + r) * TL::kPitch + e];
         }
-        // column of slot e: tile i of 16 holds columns 2 i and 2 i + 1 of each eighth of the head
-        const int gi = e & 7, d = gi * (D / 8) + 2 * (e >> 4) + ((e >> 3) & 1);
+        // the column that lane e & 7 had in half (e >> 3) & 1 of tile e >> 4
+        const int ti = e >> 4, gi = e & 7, hf = (e >> 3) & 1;
+        const int d = BITS == 4 ? 32 * (ti / 2) + 4 * gi + 2 * (ti & 1) + hf : 16 * ti + 2 * gi + hf;
         if (part != nullptr) {
           part[rr * D + d] = sum;
           if (e == 0) {
@@ -561,16 +685,20 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kvq_token_kernel
         } else {
           const int t = (r0 + rr) / a.group, hg = (r0 + rr) - t * a.group;
           const bool valid = row_position(pos, count, t, a.c.capacity) >= 0;
-          store_out(static_cast<QT*>(a.out) + ((static_cast<int64_t>(u.b) * a.T + t) * a.H + u.h * a.group + hg) * D + d, valid ? sum / ll : 0.0f);
+          store_out(static_cast<QT*>(a.out) + ((static_cast<int64_t>(ub) * a.T + t) * a.H + uh * a.group + hg) * D + d, valid ? sum / ll : 0.0f);
         }
       }
       __syncthreads();
     }
-    seg = seg_end;
-    if (seg >= span.hi) break;
-    next_unit<KEYS>(a, u);
+    if (unit.end >= span.hi) break;
+    ck -= static_cast<int>(unit.end - unit.begin);
+    __syncthreads();
+    if (threadIdx.x == 0) next_unit<KEYS>(a, unit);
+    __syncthreads();
   }
-  for (; !ok && used < loaded; ++used) mbar_wait_bounded_w(&bar[used % kStages], (used / kStages) & 1, a.status, 211);   // copies still on their way
+  if (!ok)
+    for (; used < feed[warp].loaded; ++used)           // copies still on their way
+      mbar_wait_bounded_w(&bars[warp * kStages + used % kStages], (used / kStages) & 1, a.status, 211);
 }
 
 // Joins the parts of the units that several CTAs worked on, in the order of their positions, and writes zeros for the units that
@@ -647,10 +775,18 @@ bool split_wanted(int64_t rows, int64_t tiles) { return rows <= 16 && tiles > 2 
 
 template <typename QT, int D, int BITS, int NT>
 int launch_token(const TokenArgs& ta, int ctas, cudaStream_t s) {
-  constexpr int kSmem = Tile<D, BITS>::kSmem;
+  using TL = Tile<D, BITS>;
+  constexpr int kSmem = TL::kSmem;
   auto* kernel = kvq_token_kernel<QT, D, BITS, NT>;
+  Maps maps;
+  const Cache& c = ta.a.c;
+  const uint64_t dims[3] = {TL::kRow, static_cast<uint64_t>(c.capacity), static_cast<uint64_t>(c.B) * c.Hk};
+  const uint64_t strides[2] = {TL::kRow, static_cast<uint64_t>(c.capacity) * TL::kRow};
+  const uint32_t box[3] = {TL::kRow, TL::kKeys, 1};
+  for (int i = 0; i < 2; ++i)
+    if (const int rc = encode_tensor_map_u8(&maps.m[i], c.codes[i], 3, dims, strides, box); rc != CTDK_OK) return rc;
   cudaError_t e = raise_dynamic_smem(reinterpret_cast<const void*>(kernel), kSmem);
-  if (e == cudaSuccess) e = launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kWarps * 32), kSmem, s, ta);
+  if (e == cudaSuccess) e = launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kWarps * 32), kSmem, s, maps, ta);
   if (e != cudaSuccess) return fail(CTDK_ELAUNCH, "kvq_attn: %s", cudaGetErrorString(e));
   if (const int rc = check_launch("kvq_attn"); rc != CTDK_OK || !ta.split) return rc;
   e = launch_pdl(kvq_join_kernel<QT, D, BITS, NT>, dim3(static_cast<unsigned>(ta.a.c.B * ta.a.c.Hk)), dim3(D), 0, s, ta, ctas);
@@ -726,6 +862,7 @@ int ctdk_kvq_attn(const ctdk_kvq_cache* cache, const void* q, int dtype, int64_t
   if (a.status == nullptr) return fail(CTDK_ELAUNCH, "kvq_attn: no status word");
   const int64_t rows = T * a.group, units = cache->B * cache->Hk;
   ta.rows = static_cast<int>(rows);
+  ta.bits = kvq::patterns();
   const int nt = rows <= 8 ? 1 : 2;
   const int64_t tiles = kvq::most_tiles(a, cache->D, cache->bits);
   ta.split = kvq::split_wanted(rows, tiles) ? 1 : 0;
