@@ -2,8 +2,9 @@
 // groups. out = sum_j softmax_j(scale * q . k_j) v_j, over the positions that a row sees.
 //
 // A block of R <= 8 * NT rows (the query heads of one key/value head times the new tokens) shares the cache rows, which
-// are read once. Warps work alone, each on tiles of 2 KB of key codes (16 to 64 positions), which TMA brings
-// into the warp's two stages of shared memory; the codes become exact 16-bit floating numbers in registers, in the layout
+// are read once. Each of a CTA's eight warps takes tiles of 2 KB of key codes (16 to 64 positions); TMA brings a stage of eight
+// tiles with few, large copies (issuing one takes longer than 2 KB take to arrive: a copy a tile fell behind), two stages in shared
+// memory, and the warp that leaves a stage last has it filled again. The codes become exact 16-bit floating numbers in registers, in the layout
 // that mma.sync wants, without another trip through shared memory:
 //   scores   S^T[16 positions, 8 rows] = K Q^T: ldmatrix gives a lane a word of codes of one group and position; which columns meet
 //            in which step of the product is free, as long as Q is laid out the same. The codes enter as fp16 numbers, unscaled, a
@@ -32,10 +33,11 @@ struct Tile {
   static constexpr int kRow = D * BITS / 8, kScaleRow = D / kGroup * 2;   // bytes of a position
   static constexpr int kKeys = 2048 / kRow;                               // positions of a tile
   static constexpr int kCodes = kKeys * kRow, kScales = kKeys * kScaleRow;
-  static constexpr int kStage = 2 * (kCodes + kScales);                   // bytes that one tile brings
+  static constexpr int kBytes = 2 * (kCodes + kScales);                   // that one tile brings
+  static constexpr int kBox = kWarps * kKeys < 256 ? kWarps * kKeys : 256;   // positions of a copy (a box has no more)
   static constexpr int kPitch = D + 4;                                    // floats of a row in the exchange of partial results
   static constexpr int kExchange = kWarps * 8 * kPitch * 4;
-  static constexpr int kSmem = 1024 + kWarps * kStages * kStage + kExchange;
+  static constexpr int kSmem = 1024 + kWarps * kStages * kBytes + kExchange;
 };
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
@@ -104,6 +106,12 @@ __device__ __forceinline__ void terms_bf16(float x, float y, uint32_t (&t)[N]) {
 struct Span {
   int64_t lo, hi;      // tiles of all units, numbered through
 };
+// Counts a warp that is done with a stage's contents; returns how many were before.
+__device__ __forceinline__ uint32_t leave(uint32_t* count) {
+  uint32_t n;
+  asm volatile("atom.acq_rel.cta.shared::cta.add.u32 %0, [%1], 1;" : "=r"(n) : "r"(smem_u32(count)) : "memory");
+  return n;
+}
 // As bulk_load of common.cuh, without a cache hint.
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
@@ -124,16 +132,19 @@ struct TokenArgs {
   Patterns bits;
 };
 
-// What a warp's loads go by. A run: its tiles of one unit that lie evenly spaced (all sink tiles, or all others).
+// What the loads go by.
 struct Feed {
-  int j, n, bh, left;                    // next position, tiles left in the run; key/value head; tiles left after the run
-  int plain_lo, plain_hi, loaded, pad;   // tiles from position plain_lo to plain_hi are seen whole by every row
   Unit u;
-  int64_t hi;
-  int at, end;                           // tile of the unit behind the run; tiles of the unit that are this CTA's
+  int64_t left;                          // tiles to come
+  int at, end;                           // next one, counted from the unit's first; the unit's tiles that are this CTA's
+};
+// A stage: n tiles of one unit, one a warp.
+struct Stage {
+  int j, n, last;                        // first position; last: it ends the unit's part here
+  int plain_lo, plain_hi;                // tiles from position plain_lo to plain_hi are seen whole by every row
 };
 struct Maps {
-  CUtensorMap m[2];                      // codes of keys, of values
+  CUtensorMap few[2], all[2];            // codes of keys and of values: boxes of one tile, of as many as one copy takes
 };
 
 __device__ __forceinline__ int64_t pos_of(const AttnArgs& a, int b) { return a.pos != nullptr ? static_cast<int64_t>(a.pos[b]) : a.pos_all; }
@@ -160,26 +171,6 @@ __device__ __forceinline__ void next_unit(const AttnArgs& a, Unit& u) {
   } while (u.v.tiles == 0 && u.b + 1 < a.c.B);
   u.begin = u.end;
   u.end += u.v.tiles;
-}
-
-// The next run of a warp's tiles.
-template <int KEYS>
-__device__ __forceinline__ void next_run(const AttnArgs& a, Feed& f) {
-  while (f.at >= f.end) {
-    f.at -= static_cast<int>(f.u.end - f.u.begin);
-    next_unit<KEYS>(a, f.u);
-    f.end = static_cast<int>(min(f.u.end, f.hi) - f.u.begin);
-  }
-  const Visit& v = f.u.v;
-  const bool sink = f.at < v.sink_tiles;
-  const int behind = sink ? min(v.sink_tiles, f.end) : f.end;
-  f.n = (behind - f.at + kWarps - 1) / kWarps;
-  f.left -= f.n;
-  f.j = v.tile_at(f.at) * KEYS;
-  f.bh = f.u.b * a.c.Hk + f.u.h;
-  f.at += f.n * kWarps;
-  f.plain_lo = sink || a.window == 0 ? 0 : v.hi_row - a.window;
-  f.plain_hi = sink ? min(a.sinks - KEYS, v.lo_row - KEYS + 1) : v.lo_row - KEYS + 1;
 }
 
 __device__ __forceinline__ int64_t span_start(int64_t all, int i, int n) { return all * i / n; }
@@ -266,20 +257,26 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
   constexpr int NQ = sizeof(QT) == 4 ? 2 : 1, NP = sizeof(QT) == 4 ? 3 : 1;   // terms of a query, of a probability
   constexpr int SW = GROUPS / 2;                       // words of a position's scales
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t bars[kWarps * kStages];
+  __shared__ uint64_t full[kStages];
+  __shared__ uint32_t done[kStages];                   // warps that have left a stage
+  __shared__ Stage stages[kStages];
+  __shared__ Feed feed;
   __shared__ int64_t scan[kWarps];
   __shared__ float row_m[kWarps][8 * NT], row_l[kWarps][8 * NT];
-  __shared__ Feed feed[kWarps];
-  __shared__ int place[kWarps][kStages];               // a stage's first position, its complement where not every row sees all of it
   __shared__ Unit unit;                                // that the CTA is at
   const AttnArgs& a = ta.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3;
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  if (threadIdx.x < kWarps * kStages) mbar_init(&bars[threadIdx.x], 1);
+  if (threadIdx.x < kStages) {
+    mbar_init(&full[threadIdx.x], 1);
+    done[threadIdx.x] = 0;
+  }
   if (threadIdx.x == 0) {
     mbar_fence_init();
-    tma_prefetch_desc(&maps.m[0]);
-    tma_prefetch_desc(&maps.m[1]);
+    for (int i = 0; i < 2; ++i) {
+      tma_prefetch_desc(&maps.few[i]);
+      tma_prefetch_desc(&maps.all[i]);
+    }
   }
   pdl_launch();
   __syncthreads();
@@ -310,49 +307,53 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
   }
   const int rows = min(8 * NT, ta.rows - r0);
 
-  float* exchange = reinterpret_cast<float*>(smem + kWarps * kStages * TL::kStage);
+  float* exchange = reinterpret_cast<float*>(smem + kWarps * kStages * TL::kBytes);
 
-  // Loads run ahead of the products, over the units' borders. What they go by lies in shared memory: only lane 0 needs it, and
-  // the products need the registers. Tile numbers count from the unit's first.
-  if (lane == 0) {
-    Feed& f = feed[warp];
-    f.u = u;
-    f.hi = span.hi;
-    f.left = static_cast<int>((span.hi - span.lo - warp + kWarps - 1) / kWarps);   // of this warp's tiles (it may be <= 0)
-    f.at = static_cast<int>(span.lo - u.begin) + warp;
-    f.end = static_cast<int>(min(u.end, span.hi) - u.begin);
-    f.n = f.loaded = 0;
-  }
-  if (threadIdx.x == 0) unit = u;
-  __syncwarp();
-  auto load = [&]() {
-    Feed& f = feed[warp];
-    if (f.n == 0) {                                    // the same for all lanes
-      if (f.left <= 0) return;
-      __syncwarp();
-      if (lane == 0) next_run<KEYS>(a, f);
-      __syncwarp();
+  // One thread asks for a stage's tiles; loads run ahead of the products, over the units' borders.
+  auto load = [&](int st) {
+    Feed& f = feed;
+    if (f.left <= 0) return;
+    while (f.at >= f.end) {
+      f.at -= static_cast<int>(f.u.end - f.u.begin);
+      next_unit<KEYS>(a, f.u);
+      f.end = static_cast<int>(min(f.u.end, span.hi) - f.u.begin);
     }
-    const int j = f.j, bh = f.bh, st = f.loaded % kStages;
-    __syncwarp();
-    uint64_t* full = &bars[warp * kStages + st];
-    if (lane == 0) {
-      f.j = j + kWarps * KEYS;
-      --f.n;
-      ++f.loaded;
-      place[warp][st] = j >= f.plain_lo && j <= f.plain_hi ? j : ~j;
-      mbar_expect_tx(full, TL::kStage);
+    const Visit& v = f.u.v;
+    const bool sink = f.at < v.sink_tiles;
+    const int n = min((sink ? min(v.sink_tiles, f.end) : f.end) - f.at, kWarps), j = v.tile_at(f.at) * KEYS, bh = f.u.b * a.c.Hk + f.u.h;
+    f.at += n;
+    f.left -= n;
+    Stage& g = stages[st];
+    g.j = j;
+    g.n = n;
+    g.last = f.at == f.end;
+    g.plain_lo = sink || a.window == 0 ? 0 : v.hi_row - a.window;
+    g.plain_hi = v.lo_row - KEYS + 1;
+    if (sink) g.plain_hi = min(g.plain_hi, a.sinks - KEYS);
+    const int64_t sc = (static_cast<int64_t>(bh) * a.c.capacity + j) * GROUPS;
+    unsigned char* codes = smem + st * 2 * kWarps * TL::kCodes;
+    unsigned char* scales = smem + kStages * 2 * kWarps * TL::kCodes + st * 2 * kWarps * TL::kScales;
+    mbar_expect_tx(&full[st], n * TL::kBytes);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      unsigned char* dst = codes + i * kWarps * TL::kCodes;
+      if (n == kWarps) {
+#pragma unroll
+        for (int x = 0; x < kWarps * KEYS; x += TL::kBox) tma_load_3d(dst + x * ROW, &maps.all[i], &full[st], 0, j + x, bh);
+      } else {
+        for (int x = 0; x < n; ++x) tma_load_3d(dst + x * TL::kCodes, &maps.few[i], &full[st], 0, j + x * KEYS, bh);
+      }
+      bulk_load(scales + i * kWarps * TL::kScales, a.c.scales[i] + sc, n * TL::kScales, &full[st]);
     }
-    __syncwarp();
-    if (lane < 2) {                                    // keys, values
-      tma_load_3d(smem + ((warp * kStages + st) * 2 + lane) * TL::kCodes, &maps.m[lane], full, 0, j, bh);
-      bulk_load(smem + kWarps * kStages * 2 * TL::kCodes + ((warp * kStages + st) * 2 + lane) * TL::kScales,
-                (lane ? a.c.scales[1] : a.c.scales[0]) + (static_cast<int64_t>(bh) * a.c.capacity + j) * GROUPS, TL::kScales, full);
-    }
-    __syncwarp();
   };
-#pragma unroll 1
-  for (int i = 0; i < kStages; ++i) load();
+  if (threadIdx.x == 0) {
+    unit = u;
+    feed.u = u;
+    feed.left = span.hi - span.lo;
+    feed.at = static_cast<int>(span.lo - u.begin);
+    feed.end = static_cast<int>(min(u.end, span.hi) - u.begin);
+    for (int i = 0; i < kStages; ++i) load(i);
+  }
   __syncthreads();
 
   // A lane's row address for ldmatrix (16 rows, two neighbouring chunks of 16 bytes), swizzled as TMA has written it.
@@ -361,9 +362,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
 
   int used = 0;
   bool ok = true;
-  int ck = static_cast<int>(span.lo - unit.begin) + warp;
   for (;;) {                                           // one unit after the other
-    const int cend = static_cast<int>(min(unit.end, span.hi) - unit.begin), ub = unit.b, uh = unit.h;
+    const int ub = unit.b, uh = unit.h;
     const int64_t pos = pos_of(a, ub), count = count_of(a, ub);
     // Q's fragments: column (a row of queries) g of tile n; b0, b1 of product step ks in the order in which the codes come.
     uint32_t qf[NT][STEPS][NQ][2];
@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
     // One tile; PLAIN: every valid row sees all of it.
     auto tile = [&](auto plain, int j0, uint32_t kbase, uint32_t ksc) {
       constexpr bool PLAIN = decltype(plain)::value;
-      const uint32_t vbase = kbase + TL::kCodes, vsc = ksc + TL::kScales;
+      const uint32_t vbase = kbase + kWarps * TL::kCodes, vsc = ksc + kWarps * TL::kScales;
       float s[BLOCKS][NT][4];
       // ---- scores
 #pragma unroll
@@ -615,21 +615,27 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
       }
     };
 
-    for (; ck < cend; ck += kWarps) {
-      const int stage = used % kStages;
-      ok = ok && mbar_wait_bounded_w(&bars[warp * kStages + stage], (used / kStages) & 1, a.status, 210);
+    for (bool more = span.lo < span.hi; more && ok; ++used) {
+      const int st = used % kStages;
+      ok = mbar_wait_bounded_w(&full[st], (used / kStages) & 1, a.status, 210);
       if (!ok) break;
-      const uint32_t kbase = smem_u32(smem) + (warp * kStages + stage) * 2 * TL::kCodes;
-      const uint32_t ksc = smem_u32(smem) + kWarps * kStages * 2 * TL::kCodes + (warp * kStages + stage) * 2 * TL::kScales;
-      const int j0 = place[warp][stage];
-      if (j0 >= 0) {
-        tile(std::true_type{}, j0, kbase, ksc);
-      } else {
-        tile(std::false_type{}, ~j0, kbase, ksc);
+      const Stage& f = stages[st];
+      more = f.last == 0;
+      if (warp < f.n) {
+        const uint32_t kbase = smem_u32(smem) + (st * 2 * kWarps + warp) * TL::kCodes;
+        const uint32_t ksc = smem_u32(smem) + kStages * 2 * kWarps * TL::kCodes + (st * 2 * kWarps + warp) * TL::kScales;
+        const int j0 = f.j + warp * KEYS;
+        if (j0 >= f.plain_lo && j0 <= f.plain_hi) {
+          tile(std::true_type{}, j0, kbase, ksc);
+        } else {
+          tile(std::false_type{}, j0, kbase, ksc);
+        }
       }
       __syncwarp();
-      ++used;
-      load();
+      if (lane == 0 && leave(&done[st]) == kWarps - 1) {   // the last warp to leave a stage has it filled again
+        done[st] = 0;
+        load(st);
+      }
     }
 
     // ---- the warps' results of this unit together
@@ -691,14 +697,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
       __syncthreads();
     }
     if (unit.end >= span.hi) break;
-    ck -= static_cast<int>(unit.end - unit.begin);
     __syncthreads();
     if (threadIdx.x == 0) next_unit<KEYS>(a, unit);
     __syncthreads();
   }
-  if (!ok)
-    for (; used < feed[warp].loaded; ++used)           // copies still on their way
-      mbar_wait_bounded_w(&bars[warp * kStages + used % kStages], (used / kStages) & 1, a.status, 211);
+  for (int i = 0; !ok && i < kStages; ++i, ++used)     // copies still on their way
+    mbar_wait_bounded_w(&full[used % kStages], (used / kStages) & 1, a.status, 211);
 }
 
 // Joins the parts of the units that several CTAs worked on, in the order of their positions, and writes zeros for the units that
@@ -782,9 +786,12 @@ int launch_token(const TokenArgs& ta, int ctas, cudaStream_t s) {
   const Cache& c = ta.a.c;
   const uint64_t dims[3] = {TL::kRow, static_cast<uint64_t>(c.capacity), static_cast<uint64_t>(c.B) * c.Hk};
   const uint64_t strides[2] = {TL::kRow, static_cast<uint64_t>(c.capacity) * TL::kRow};
-  const uint32_t box[3] = {TL::kRow, TL::kKeys, 1};
-  for (int i = 0; i < 2; ++i)
-    if (const int rc = encode_tensor_map_u8(&maps.m[i], c.codes[i], 3, dims, strides, box); rc != CTDK_OK) return rc;
+  const uint32_t few[3] = {TL::kRow, TL::kKeys, 1}, all[3] = {TL::kRow, TL::kBox, 1};
+  for (int i = 0; i < 2; ++i) {
+    int rc = encode_tensor_map_u8(&maps.few[i], c.codes[i], 3, dims, strides, few);
+    if (rc == CTDK_OK) rc = encode_tensor_map_u8(&maps.all[i], c.codes[i], 3, dims, strides, all);
+    if (rc != CTDK_OK) return rc;
+  }
   cudaError_t e = raise_dynamic_smem(reinterpret_cast<const void*>(kernel), kSmem);
   if (e == cudaSuccess) e = launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kWarps * 32), kSmem, s, maps, ta);
   if (e != cudaSuccess) return fail(CTDK_ELAUNCH, "kvq_attn: %s", cudaGetErrorString(e));
