@@ -61,25 +61,23 @@ __device__ __forceinline__ uint32_t add_f16x2(uint32_t x, uint32_t c) {
 // operation it spends a second one on it.
 struct Patterns {
   uint32_t x43, x3f;                     // bfloat16 128, 1 / 2
-  uint32_t up15, up11, less4, less8;     // fp16 2^15, 2^11, -8 * 2^-9, -128 * 2^-9
 };
-inline Patterns patterns() { return {0x43004300u, 0x3f003f00u, 0x78007800u, 0x68006800u, 0xa400a400u, 0xb400b400u}; }
+inline Patterns patterns() { return {0x43004300u, 0x3f003f00u}; }
 
 #ifdef __CUDACC__
-// Codes times 2^-9 as fp16 numbers: the bits alone are the subnormal number u * 2^-24 (or 2^-20), which needs no exponent put over them.
-// 4-bit codes: of w's nibbles, pair i of out holds i and i + 4.
-constexpr int kCodeShift = 9;
-__device__ __forceinline__ void codes4_f16(uint32_t w, const Patterns& c, uint32_t (&out)[4]) {
+// Stored codes u as fp16 numbers: the bits alone are the subnormal numbers u * 2^-24, or u * 2^-20 where they lie four places higher.
+// 4-bit codes: of w's nibbles, pair i of out holds i and i + 4; pairs 1 and 3 are the ones times 2^-20.
+__device__ __forceinline__ void codes4_f16(uint32_t w, uint32_t (&out)[4]) {
   const uint32_t v = w >> 8;
-  out[0] = fma_f16x2(w & 0x000f000fu, c.up15, c.less4);
-  out[1] = fma_f16x2(w & 0x00f000f0u, c.up11, c.less4);
-  out[2] = fma_f16x2(v & 0x000f000fu, c.up15, c.less4);
-  out[3] = fma_f16x2(v & 0x00f000f0u, c.up11, c.less4);
+  out[0] = w & 0x000f000fu;
+  out[1] = w & 0x00f000f0u;
+  out[2] = v & 0x000f000fu;
+  out[3] = v & 0x00f000f0u;
 }
 // 8-bit codes: bytes 0, 1 and 2, 3.
-__device__ __forceinline__ void codes8_f16(uint32_t w, const Patterns& c, uint32_t (&out)[2]) {
-  out[0] = fma_f16x2(prmt(w, 0, 0x4140), c.up15, c.less8);
-  out[1] = fma_f16x2(prmt(w, 0, 0x4342), c.up15, c.less8);
+__device__ __forceinline__ void codes8_f16(uint32_t w, uint32_t (&out)[2]) {
+  out[0] = prmt(w, 0, 0x4140);
+  out[1] = prmt(w, 0, 0x4342);
 }
 // Codes times their scales as bfloat16 numbers: the bits go under the exponent of a power of two.
 // 4 bits: nibble i of both halves of w, the halves' scales in s2.

@@ -25,7 +25,7 @@ namespace ctdk {
 namespace kvq {
 namespace {
 
-constexpr int kWarps = 8, kStages = 2;
+constexpr int kWarps = 8, kStages = 3;
 constexpr float kSlack = 8.0f;
 
 template <int D, int BITS>
@@ -36,8 +36,9 @@ struct Tile {
   static constexpr int kBytes = 2 * (kCodes + kScales);                   // that one tile brings
   static constexpr int kBox = kWarps * kKeys < 256 ? kWarps * kKeys : 256;   // positions of a copy (a box has no more)
   static constexpr int kPitch = D + 4;                                    // floats of a row in the exchange of partial results
-  static constexpr int kExchange = kWarps * 8 * kPitch * 4;
-  static constexpr int kSmem = 1024 + kWarps * kStages * kBytes + kExchange;
+  static constexpr int kExchange = kWarps * 8 * kPitch * 4;                // it takes the place of a stage that has been used
+  static_assert(kExchange <= kWarps * 2 * (kCodes + kScales), "exchange");
+  static constexpr int kSmem = 1024 + kWarps * kStages * kBytes;
 };
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
@@ -51,12 +52,12 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// The same without a third operand.
-__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+// The same on top of init[0] in the even columns, init[1] in the odd ones.
+__device__ __forceinline__ void mma_f16_from(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&init)[2]) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(init[0]), "f"(init[1]));
 }
 __device__ __forceinline__ uint32_t lds16(uint32_t a) {
   unsigned short v;
@@ -103,6 +104,25 @@ __device__ __forceinline__ void terms_bf16(float x, float y, uint32_t (&t)[N]) {
   }
 }
 
+// N neighbouring values (16 bytes or more, aligned) as floats.
+template <int N>
+__device__ __forceinline__ void load_row(const float* p, float* x) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(p + i));
+    x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_row(const __nv_bfloat16* p, float* x) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p + i));
+    x[i] = __uint_as_float(v.x << 16), x[i + 1] = __uint_as_float(v.x & 0xffff0000u);
+    x[i + 2] = __uint_as_float(v.y << 16), x[i + 3] = __uint_as_float(v.y & 0xffff0000u);
+  }
+}
+
 struct Span {
   int64_t lo, hi;      // tiles of all units, numbered through
 };
@@ -122,6 +142,7 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 struct Unit {
   int b, h;
   int64_t begin, end;
+  int64_t pos, count;
   Visit v;
 };
 
@@ -140,6 +161,7 @@ struct Feed {
 };
 // A stage: n tiles of one unit, one a warp.
 struct Stage {
+  Unit u;
   int j, n, last;                        // first position; last: it ends the unit's part here
   int plain_lo, plain_hi;                // tiles from position plain_lo to plain_hi are seen whole by every row
 };
@@ -155,6 +177,12 @@ template <int KEYS>
 __device__ __forceinline__ Visit visit(const AttnArgs& a, int b, int t0, int rows) {
   return visit_of(pos_of(a, b), count_of(a, b), t0, rows, a.c.capacity, a.window, a.sinks, KEYS);
 }
+template <int KEYS>
+__device__ __forceinline__ void visit_unit(const AttnArgs& a, Unit& u, int t0, int rows) {
+  u.pos = pos_of(a, u.b);
+  u.count = count_of(a, u.b);
+  u.v = visit_of(u.pos, u.count, t0, rows, a.c.capacity, a.window, a.sinks, KEYS);
+}
 // Moves to the next unit that has tiles.
 template <int KEYS>
 __device__ __forceinline__ void next_unit(const AttnArgs& a, Unit& u) {
@@ -167,7 +195,7 @@ __device__ __forceinline__ void next_unit(const AttnArgs& a, Unit& u) {
   u.h = 0;
   do {
     ++u.b;
-    u.v = visit<KEYS>(a, u.b, 0, a.T);
+    visit_unit<KEYS>(a, u, 0, a.T);
   } while (u.v.tiles == 0 && u.b + 1 < a.c.B);
   u.begin = u.end;
   u.end += u.v.tiles;
@@ -196,48 +224,51 @@ __device__ __forceinline__ int64_t cta_sum(int64_t x, int64_t* before, int64_t* 
   return all;
 }
 
-// Tiles of all sequences' units.
+// The CTA's part `i` of `n` of all units' tiles, and the unit that holds its first one. False: it has none.
 template <int KEYS>
-__device__ __forceinline__ int64_t all_tiles(const AttnArgs& a, int64_t* smem) {
-  if (a.pos == nullptr && a.count == nullptr) return static_cast<int64_t>(visit<KEYS>(a, 0, 0, a.T).tiles) * a.c.B * a.c.Hk;
-  int64_t n = 0;
-  for (int b = threadIdx.x; b < a.c.B; b += blockDim.x) n += visit<KEYS>(a, b, 0, a.T).tiles;
-  return cta_sum(n, nullptr, smem) * a.c.Hk;
-}
-
-// The unit that holds tile x (x < all tiles).
-template <int KEYS>
-__device__ __forceinline__ Unit unit_at(const AttnArgs& a, int64_t x, int64_t* smem) {
-  Unit u;
+__device__ __forceinline__ bool span_of(const AttnArgs& a, int i, int n, Span& span, Unit& u, int64_t* smem) {
+  u = {};
   if (a.pos == nullptr && a.count == nullptr) {
-    u.v = visit<KEYS>(a, 0, 0, a.T);
-    const int64_t n = x / u.v.tiles;
-    u.b = static_cast<int>(n / a.c.Hk);
-    u.h = static_cast<int>(n % a.c.Hk);
-    u.begin = n * u.v.tiles;
+    visit_unit<KEYS>(a, u, 0, a.T);
+    const int64_t all = static_cast<int64_t>(u.v.tiles) * a.c.B * a.c.Hk;
+    span = {span_start(all, i, n), span_start(all, i + 1, n)};
+    if (span.lo >= span.hi) return false;
+    const int64_t k = span.lo / u.v.tiles;
+    u.b = static_cast<int>(k / a.c.Hk);
+    u.h = static_cast<int>(k % a.c.Hk);
+    u.begin = k * u.v.tiles;
     u.end = u.begin + u.v.tiles;
-    return u;
+    return true;
   }
   __shared__ int64_t found[2];
+  // Tiles of a chunk of sequences, one a thread; more than one chunk: once for their sum, once more to find the place.
+  auto mine = [&](int b0) {
+    const int b = b0 + static_cast<int>(threadIdx.x);
+    return b < a.c.B ? static_cast<int64_t>(visit<KEYS>(a, b, 0, a.T).tiles) * a.c.Hk : 0;
+  };
+  const int step = static_cast<int>(blockDim.x);
+  int64_t x = mine(0), before, all = cta_sum(x, &before, smem);
+  for (int b0 = step; b0 < a.c.B; b0 += step) all += cta_sum(mine(b0), nullptr, smem);
+  span = {span_start(all, i, n), span_start(all, i + 1, n)};
+  if (span.lo >= span.hi) return false;
   int64_t base = 0;
-  for (int b0 = 0;; b0 += blockDim.x) {
-    const int b = b0 + threadIdx.x;
-    const int64_t n = b < a.c.B ? static_cast<int64_t>(visit<KEYS>(a, b, 0, a.T).tiles) * a.c.Hk : 0;
-    int64_t before;
-    const int64_t sum = cta_sum(n, &before, smem);
-    before += base;
-    if (x >= before && x < before + n) found[0] = b, found[1] = before;
-    base += sum;
-    __syncthreads();
-    if (x < base || b0 + static_cast<int>(blockDim.x) >= a.c.B) break;
+  for (int b0 = 0;;) {
+    if (span.lo >= base + before && span.lo < base + before + x) found[0] = b0 + threadIdx.x, found[1] = base + before;
+    if (a.c.B <= step) break;
+    base += cta_sum(x, &before, smem);
+    b0 += step;
+    if (span.lo < base || b0 >= a.c.B) break;
+    x = mine(b0);
+    cta_sum(x, &before, smem);
   }
+  __syncthreads();
   u.b = static_cast<int>(found[0]);
-  u.v = visit<KEYS>(a, u.b, 0, a.T);
-  const int64_t h = (x - found[1]) / u.v.tiles;
+  visit_unit<KEYS>(a, u, 0, a.T);
+  const int64_t h = (span.lo - found[1]) / u.v.tiles;
   u.h = static_cast<int>(h);
   u.begin = found[1] + h * u.v.tiles;
   u.end = u.begin + u.v.tiles;
-  return u;
+  return true;
 }
 
 __device__ __forceinline__ void store_out(float* p, float x) { *p = x; }
@@ -263,7 +294,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
   __shared__ Feed feed;
   __shared__ int64_t scan[kWarps];
   __shared__ float row_m[kWarps][8 * NT], row_l[kWarps][8 * NT];
-  __shared__ Unit unit;                                // that the CTA is at
   const AttnArgs& a = ta.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3;
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -287,11 +317,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
   Unit u = {};
   int r0 = 0;                                          // first row of the block of rows
   if (ta.split) {
-    const int64_t all = all_tiles<KEYS>(a, scan);
-    span.lo = span_start(all, blockIdx.x, gridDim.x);
-    span.hi = span_start(all, blockIdx.x + 1, gridDim.x);
-    if (span.lo >= span.hi) return;
-    u = unit_at<KEYS>(a, span.lo, scan);
+    if (!span_of<KEYS>(a, blockIdx.x, gridDim.x, span, u, scan)) return;
   } else {
     const int blocks = (ta.rows + 8 * NT - 1) / (8 * NT);
     const int64_t id = blockIdx.x, bh = id / blocks;
@@ -299,15 +325,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
     u.b = static_cast<int>(bh / a.c.Hk);
     u.h = static_cast<int>(bh - static_cast<int64_t>(u.b) * a.c.Hk);
     const int t0 = r0 / a.group, t1 = (min(r0 + 8 * NT, ta.rows) - 1) / a.group;
-    u.v = visit<KEYS>(a, u.b, t0, t1 - t0 + 1);
+    visit_unit<KEYS>(a, u, t0, t1 - t0 + 1);
     u.begin = 0;
     u.end = u.v.tiles;
     span.lo = 0;
     span.hi = u.v.tiles;
   }
   const int rows = min(8 * NT, ta.rows - r0);
-
-  float* exchange = reinterpret_cast<float*>(smem + kWarps * kStages * TL::kBytes);
 
   // One thread asks for a stage's tiles; loads run ahead of the products, over the units' borders.
   auto load = [&](int st) {
@@ -324,6 +348,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
     f.at += n;
     f.left -= n;
     Stage& g = stages[st];
+    g.u = f.u;
     g.j = j;
     g.n = n;
     g.last = f.at == f.end;
@@ -331,8 +356,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
     g.plain_hi = v.lo_row - KEYS + 1;
     if (sink) g.plain_hi = min(g.plain_hi, a.sinks - KEYS);
     const int64_t sc = (static_cast<int64_t>(bh) * a.c.capacity + j) * GROUPS;
-    unsigned char* codes = smem + st * 2 * kWarps * TL::kCodes;
-    unsigned char* scales = smem + kStages * 2 * kWarps * TL::kCodes + st * 2 * kWarps * TL::kScales;
+    unsigned char* codes = smem + st * kWarps * TL::kBytes;
+    unsigned char* scales = codes + 2 * kWarps * TL::kCodes;
     mbar_expect_tx(&full[st], n * TL::kBytes);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -347,7 +372,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
     }
   };
   if (threadIdx.x == 0) {
-    unit = u;
+    if (span.lo >= span.hi) stages[0].u = u;           // a unit without tiles (not split): zeros
     feed.u = u;
     feed.left = span.hi - span.lo;
     feed.at = static_cast<int>(span.lo - u.begin);
@@ -363,45 +388,65 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
   int used = 0;
   bool ok = true;
   for (;;) {                                           // one unit after the other
-    const int ub = unit.b, uh = unit.h;
-    const int64_t pos = pos_of(a, ub), count = count_of(a, ub);
+    const Unit& unit = stages[used % kStages].u;       // (of this stage's time: it is read before the stage is left)
+    const int ub = unit.b, uh = unit.h, hi_row = unit.v.hi_row;
+    const int64_t pos = unit.pos, count = unit.count;
+    const bool whole = unit.begin >= span.lo && unit.end <= span.hi, last_unit = unit.end >= span.hi;
+    float* part = whole ? nullptr : a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (unit.begin < span.lo ? 0 : 1)) * Part<D, NT>::kFloats;
     // Q's fragments: column (a row of queries) g of tile n; b0, b1 of product step ks in the order in which the codes come.
     uint32_t qf[NT][STEPS][NQ][2];
-    float factor[NT][2];                               // of rows 2 tig, 2 tig + 1: score to log2 domain
+    float factor[NT][2], init[NT][GROUPS][2];          // of rows 2 tig, 2 tig + 1: score to log2 domain; what takes the codes' bias off
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int r = r0 + 8 * n + g, t = r / a.group;
-      const bool live = 8 * n + g < rows;
       const QT* src = static_cast<const QT*>(a.q) + ub * a.batch_stride + static_cast<int64_t>(t) * a.row_stride +
                       static_cast<int64_t>(uh * a.group + (r - t * a.group)) * D;
-      float x[STEPS][4], most = 0.0f;
+      float x[D / 4], most = 0.0f;                     // a lane's columns: of every group eight (4 bits), or twice four
 #pragma unroll
-      for (int ks = 0; ks < STEPS; ++ks)
+      for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
+      if (8 * n + g < rows) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // 4 bits: a word of eight codes gives two steps, pairs (c, c + 4); 8 bits: a word of four gives one
-          const int d = BITS == 4 ? 32 * (ks / 2) + 8 * tig + 2 * (ks & 1) + (i >> 1) + 4 * (i & 1) : 16 * ks + 4 * tig + i;
-          x[ks][i] = live ? static_cast<float>(src[d]) : 0.0f;
-          most = fmaxf(most, fabsf(x[ks][i]));
+        for (int i = 0; i < D / 4; i += BITS == 4 ? 8 : 4) {
+          if constexpr (BITS == 4) load_row<8>(src + 4 * i + 8 * tig, x + i);
+          else load_row<4>(src + 4 * i + 4 * tig, x + i);
         }
+      }
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) most = fmaxf(most, fabsf(x[i]));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
       const int e = static_cast<int>(__float_as_uint(most) >> 23) - 127;           // 128: not finite
-      const int up = most == 0.0f || e == 128 ? 0 : max(min(6 - e, 126), -110);    // most * 2^up is in [64, 128), or near it
+      const int up = most == 0.0f || e == 128 ? 0 : max(min(6 - e, 126), -100);    // most * 2^up is in [64, 128), or near it
       const float f = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
+#pragma unroll
+      for (int i = 0; i < D / 4; ++i) x[i] *= f;
 #pragma unroll
       for (int ks = 0; ks < STEPS; ++ks)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+          // 4 bits: a word of eight codes gives two steps, pairs (c, c + 4); 8 bits: a word of four gives one
+          const float* y = x + (BITS == 4 ? 8 * (ks / 2) + 2 * (ks & 1) + i : 4 * ks + 2 * i);
+          const float w = BITS == 4 && i == 1 ? 0.0625f : 1.0f;
           uint32_t tt[NQ];
-          terms_f16<NQ>(x[ks][2 * i] * f, x[ks][2 * i + 1] * f, tt);
+          terms_f16<NQ>(y[0] * w, y[BITS == 4 ? 4 : 1] * w, tt);
 #pragma unroll
-          for (int y = 0; y < NQ; ++y) qf[n][ks][y][i] = tt[y];
+          for (int z = 0; z < NQ; ++z) qf[n][ks][z][i] = tt[z];
         }
+#pragma unroll
+      for (int gr = 0; gr < GROUPS; ++gr) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += x[8 * gr + i];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        sum *= BITS == 4 ? -8.0f * 0x1p-24f : -128.0f * 0x1p-24f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) init[n][gr][c] = __shfl_sync(0xffffffffu, sum, (2 * tig + c) * 4);
+      }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int other = __shfl_sync(0xffffffffu, up, (2 * tig + c) * 4);
-        factor[n][c] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + kCodeShift - other) << 23);   // other is 126 at most
+        factor[n][c] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + 24 - other) << 23);   // other is from -100 to 126
       }
     }
     // Rows 2 tig and 2 tig + 1 of tile n: their positions, reference points (log2 domain) and sums.
@@ -443,7 +488,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int y = 0; y < NQ; ++y) {
-                if ((ks & 1) == 0 && y == 0) mma_f16_first(acc[n], f, qf[n][ks][y][0], qf[n][ks][y][1]);
+                if ((ks & 1) == 0 && y == 0) mma_f16_from(acc[n], f, qf[n][ks][y][0], qf[n][ks][y][1], init[n][ks / 2]);
                 else mma_f16(acc[n], f, qf[n][ks][y][0], qf[n][ks][y][1]);
               }
           };
@@ -460,8 +505,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               uint32_t p[4], q[4];
-              codes4_f16(w[2 * y], ta.bits, p);
-              codes4_f16(w[2 * y + 1], ta.bits, q);
+              codes4_f16(w[2 * y], p);
+              codes4_f16(w[2 * y + 1], q);
               const uint32_t f0[4] = {p[0], q[0], p[1], q[1]}, f1[4] = {p[2], q[2], p[3], q[3]};
               step(4 * x + 2 * y, f0);
               step(4 * x + 2 * y + 1, f1);
@@ -471,8 +516,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               uint32_t p[2], q[2];
-              codes8_f16(w[2 * y], ta.bits, p);
-              codes8_f16(w[2 * y + 1], ta.bits, q);
+              codes8_f16(w[2 * y], p);
+              codes8_f16(w[2 * y + 1], q);
               const uint32_t f[4] = {p[0], q[0], p[1], q[1]};
               step(2 * x + y, f);
             }
@@ -553,7 +598,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
             // groups that are NaN themselves; the rows that see one of those get their NaN below.
 #pragma unroll
             for (int i = 0; i < 2 * SW; ++i) {
-              if (j0 + tok + i / SW >= unit.v.hi_row) sc[i] = 0;
+              if (j0 + tok + i / SW >= hi_row) sc[i] = 0;
               if (is_nan_scale(sc[i])) sc[i] &= 0xffff0000u;
               if (is_nan_scale(sc[i] >> 16)) sc[i] &= 0x0000ffffu;
             }
@@ -597,7 +642,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
       }
       if (!PLAIN) {                                    // NaN groups of values: the rows that see them
         bool nan = false;
-        for (int i = lane; i < KEYS * GROUPS; i += 32) nan |= is_nan_scale(lds16(vsc + 2 * i)) && j0 + i / GROUPS < unit.v.hi_row;
+        for (int i = lane; i < KEYS * GROUPS; i += 32) nan |= is_nan_scale(lds16(vsc + 2 * i)) && j0 + i / GROUPS < hi_row;
         if (__any_sync(0xffffffffu, nan)) {
 #pragma unroll 1
           for (int i = 0; i < KEYS; ++i)
@@ -615,15 +660,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
       }
     };
 
+    int st = used % kStages;
     for (bool more = span.lo < span.hi; more && ok; ++used) {
-      const int st = used % kStages;
+      st = used % kStages;
       ok = mbar_wait_bounded_w(&full[st], (used / kStages) & 1, a.status, 210);
       if (!ok) break;
       const Stage& f = stages[st];
       more = f.last == 0;
       if (warp < f.n) {
-        const uint32_t kbase = smem_u32(smem) + (st * 2 * kWarps + warp) * TL::kCodes;
-        const uint32_t ksc = smem_u32(smem) + kStages * 2 * kWarps * TL::kCodes + (st * 2 * kWarps + warp) * TL::kScales;
+        const uint32_t kbase = smem_u32(smem) + st * kWarps * TL::kBytes + warp * TL::kCodes;
+        const uint32_t ksc = smem_u32(smem) + st * kWarps * TL::kBytes + 2 * kWarps * TL::kCodes + warp * TL::kScales;
         const int j0 = f.j + warp * KEYS;
         if (j0 >= f.plain_lo && j0 <= f.plain_hi) {
           tile(std::true_type{}, j0, kbase, ksc);
@@ -634,7 +680,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
       __syncwarp();
       if (lane == 0 && leave(&done[st]) == kWarps - 1) {   // the last warp to leave a stage has it filled again
         done[st] = 0;
-        load(st);
+        if (more) load(st);                            // the unit's last stage is needed below first
       }
     }
 
@@ -651,9 +697,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
           row_l[warp][8 * n + 2 * tig + c] = x;
         }
       }
-    const bool whole = unit.begin >= span.lo && unit.end <= span.hi;
-    float* part = nullptr;
-    if (!whole) part = a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (unit.begin < span.lo ? 0 : 1)) * Part<D, NT>::kFloats;
+    // All warps have left the stage st: its room serves for the exchange.
+    __syncthreads();
+    float* exchange = reinterpret_cast<float*>(smem + st * kWarps * TL::kBytes);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -696,25 +742,30 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
       }
       __syncthreads();
     }
-    if (unit.end >= span.hi) break;
-    __syncthreads();
-    if (threadIdx.x == 0) next_unit<KEYS>(a, unit);
-    __syncthreads();
+    if (last_unit) break;
+    if (threadIdx.x == 0) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // copies may write where the exchange was
+      load(st);
+    }
   }
   for (int i = 0; !ok && i < kStages; ++i, ++used)     // copies still on their way
     mbar_wait_bounded_w(&full[used % kStages], (used / kStages) & 1, a.status, 211);
 }
 
 // Joins the parts of the units that several CTAs worked on, in the order of their positions, and writes zeros for the units that
-// have nothing to see.
+// have nothing to see. One CTA a unit: the parts' maxima and sums first, all at once, then every output as one sum of
+// independent loads (a chain of parts, one after the other, took 60 us for 37 parts of four rows).
+constexpr int kJoinThreads = 256, kJoinParts = 128;    // parts whose weights are held at a time
 template <typename QT, int D, int BITS, int NT>
-__global__ void __launch_bounds__(D) kvq_join_kernel(const TokenArgs ta, int ctas) {
-  constexpr int KEYS = Tile<D, BITS>::kKeys;
-  __shared__ int64_t scan[D / 32];
+__global__ void __launch_bounds__(kJoinThreads) kvq_join_kernel(const TokenArgs ta, int ctas) {
+  constexpr int KEYS = Tile<D, BITS>::kKeys, kRows = 8 * NT, kOut = (kRows * D + kJoinThreads - 1) / kJoinThreads;
+  __shared__ int64_t scan[kJoinThreads / 32];
+  __shared__ float weight[kJoinParts][kRows], row_m[kRows], row_l[kRows];
   const AttnArgs& a = ta.a;
   pdl_launch();
   pdl_wait();
   const int b = blockIdx.x / a.c.Hk, h = blockIdx.x - b * a.c.Hk;
+  const int64_t pos = pos_of(a, b), count = count_of(a, b);
   const Visit v = visit<KEYS>(a, b, 0, a.T);
   int64_t all, begin;
   if (a.pos == nullptr && a.count == nullptr) {
@@ -722,7 +773,7 @@ __global__ void __launch_bounds__(D) kvq_join_kernel(const TokenArgs ta, int cta
     begin = static_cast<int64_t>(v.tiles) * blockIdx.x;
   } else {
     int64_t n = 0, before = 0;
-    for (int i = threadIdx.x; i < a.c.B; i += D) {
+    for (int i = threadIdx.x; i < a.c.B; i += kJoinThreads) {
       const int64_t x = visit<KEYS>(a, i, 0, a.T).tiles;
       n += x;
       if (i < b) before += x;
@@ -730,32 +781,81 @@ __global__ void __launch_bounds__(D) kvq_join_kernel(const TokenArgs ta, int cta
     all = cta_sum(n, nullptr, scan) * a.c.Hk;
     begin = cta_sum(before, nullptr, scan) * a.c.Hk + static_cast<int64_t>(v.tiles) * h;
   }
-  const int d = threadIdx.x;
-  QT* out = static_cast<QT*>(a.out) + (static_cast<int64_t>(b) * a.T * a.H + h * a.group) * D + d;
+  QT* out = static_cast<QT*>(a.out) + (static_cast<int64_t>(b) * a.T * a.H + h * a.group) * D;
   if (v.tiles == 0) {
-    for (int r = 0; r < ta.rows; ++r) store_out(out + (static_cast<int64_t>(r / a.group) * a.H + r % a.group) * D, 0.0f);
+    for (int i = threadIdx.x; i < ta.rows * D; i += kJoinThreads) {
+      const int r = i / D, t = r / a.group;
+      store_out(out + (static_cast<int64_t>(t) * a.H + r - t * a.group) * D + i % D, 0.0f);
+    }
     return;
   }
   const int64_t end = begin + v.tiles;
   const int c0 = static_cast<int>(((begin + 1) * ctas - 1) / all), c1 = static_cast<int>((end * ctas - 1) / all);
   if (c0 == c1) return;
-  const int64_t pos = pos_of(a, b), count = count_of(a, b);
-  for (int r = 0; r < ta.rows; ++r) {
-    const int t = r / a.group;
-    float x = 0.0f;
-    if (row_position(pos, count, t, a.c.capacity) >= 0) {
-      float m = -INFINITY, l = 0.0f, s = 0.0f;
-      for (int c = c0; c <= c1; ++c) {
-        const float* p = a.part + (static_cast<int64_t>(c) * 2 + (begin < span_start(all, c, ctas) ? 0 : 1)) * Part<D, NT>::kFloats;
-        const float pm = p[8 * NT * D + r], pl = p[8 * NT * D + 8 * NT + r], ps = p[r * D + d];
-        const float nm = fmaxf(m, pm), ref = nm == -INFINITY ? 0.0f : nm, f = ex2(m - ref), e = ex2(pm - ref);
-        l = l * f + pl * e;
-        s = s * f + ps * e;
-        m = nm;
+  // The first part is its CTA's last unit (or its only one, which began before), the others are their CTAs' first.
+  const float* first = a.part + (static_cast<int64_t>(c0) * 2 + (begin < span_start(all, c0, ctas) ? 0 : 1)) * Part<D, NT>::kFloats;
+  auto part_of = [&](int c) { return c == c0 ? first : a.part + static_cast<int64_t>(c) * 2 * Part<D, NT>::kFloats; };
+  float sum[kOut];
+#pragma unroll
+  for (int i = 0; i < kOut; ++i) sum[i] = 0.0f;
+  if (threadIdx.x < kRows) {
+    row_m[threadIdx.x] = -INFINITY;
+    row_l[threadIdx.x] = 0.0f;
+  }
+  for (int p0 = c0; p0 <= c1; p0 += kJoinParts) {
+    const int n = min(kJoinParts, c1 - p0 + 1);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n * kRows; i += kJoinThreads) weight[i / kRows][i % kRows] = part_of(p0 + i / kRows)[kRows * D + i % kRows];
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float again[NT];                                   // what the sums of earlier parts are multiplied by (rows warp, warp + 8)
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      const int r = warp + 8 * x;
+      float m = row_m[r];
+      for (int i = lane; i < n; i += 32) m = fmaxf(m, weight[i][r]);
+      m = warp_max(m);
+      const float ref = m == -INFINITY ? 0.0f : m;
+      float l = 0.0f;
+      for (int i = lane; i < n; i += 32) {
+        const float w = ex2(weight[i][r] - ref);
+        weight[i][r] = w;
+        l += w * part_of(p0 + i)[kRows * D + kRows + r];
       }
-      x = s / l;
+      l = warp_sum(l);
+      again[x] = ex2(row_m[r] - ref);
+      __syncwarp();
+      if (lane == 0) {
+        row_l[r] = row_l[r] * again[x] + l;
+        row_m[r] = m;
+      }
     }
-    store_out(out + (static_cast<int64_t>(t) * a.H + r % a.group) * D, x);
+    if (p0 != c0) {                                    // (more parts than weights are held at a time)
+      __shared__ float scale[kRows];
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+        if (lane == 0) scale[warp + 8 * x] = again[x];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kOut; ++i)
+        if (threadIdx.x + i * kJoinThreads < kRows * D) sum[i] *= scale[(threadIdx.x + i * kJoinThreads) / D];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kOut; ++i) {
+      const int e = threadIdx.x + i * kJoinThreads, r = e / D;
+      if (r >= ta.rows) continue;
+#pragma unroll 8
+      for (int p = 0; p < n; ++p) sum[i] += weight[p][r] * part_of(p0 + p)[e];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kOut; ++i) {
+    const int e = threadIdx.x + i * kJoinThreads, r = e / D, t = r / a.group;
+    if (r >= ta.rows) continue;
+    const bool valid = row_position(pos, count, t, a.c.capacity) >= 0;
+    store_out(out + (static_cast<int64_t>(t) * a.H + r - t * a.group) * D + e % D, valid ? sum[i] / row_l[r] : 0.0f);
   }
 }
 
@@ -796,7 +896,7 @@ int launch_token(const TokenArgs& ta, int ctas, cudaStream_t s) {
   if (e == cudaSuccess) e = launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kWarps * 32), kSmem, s, maps, ta);
   if (e != cudaSuccess) return fail(CTDK_ELAUNCH, "kvq_attn: %s", cudaGetErrorString(e));
   if (const int rc = check_launch("kvq_attn"); rc != CTDK_OK || !ta.split) return rc;
-  e = launch_pdl(kvq_join_kernel<QT, D, BITS, NT>, dim3(static_cast<unsigned>(ta.a.c.B * ta.a.c.Hk)), dim3(D), 0, s, ta, ctas);
+  e = launch_pdl(kvq_join_kernel<QT, D, BITS, NT>, dim3(static_cast<unsigned>(ta.a.c.B * ta.a.c.Hk)), dim3(kJoinThreads), 0, s, ta, ctas);
   if (e != cudaSuccess) return fail(CTDK_ELAUNCH, "kvq_attn: %s", cudaGetErrorString(e));
   return check_launch("kvq_attn");
 }
