@@ -156,6 +156,7 @@ struct TokenArgs {
 // What the loads go by.
 struct Feed {
   Unit u;
+  int64_t lo, hi;                        // the CTA's tiles
   int64_t left;                          // tiles to come
   int at, end;                           // next one, counted from the unit's first; the unit's tiles that are this CTA's
 };
@@ -201,7 +202,12 @@ __device__ __forceinline__ void next_unit(const AttnArgs& a, Unit& u) {
   u.end += u.v.tiles;
 }
 
-__device__ __forceinline__ int64_t span_start(int64_t all, int i, int n) { return all * i / n; }
+// x / n for x >= 0, n > 0: 64-bit divisions are a hundred instructions, and the numbers are small as a rule.
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t n) {
+  if (((x | n) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(n);
+  return x / n;
+}
+__device__ __forceinline__ int64_t span_start(int64_t all, int i, int n) { return quotient(all * i, n); }
 
 // Sum over the CTA of one value a thread (all threads get it), and of the values of the threads before (exclusive).
 __device__ __forceinline__ int64_t cta_sum(int64_t x, int64_t* before, int64_t* smem) {
@@ -233,9 +239,9 @@ __device__ __forceinline__ bool span_of(const AttnArgs& a, int i, int n, Span& s
     const int64_t all = static_cast<int64_t>(u.v.tiles) * a.c.B * a.c.Hk;
     span = {span_start(all, i, n), span_start(all, i + 1, n)};
     if (span.lo >= span.hi) return false;
-    const int64_t k = span.lo / u.v.tiles;
-    u.b = static_cast<int>(k / a.c.Hk);
-    u.h = static_cast<int>(k % a.c.Hk);
+    const int64_t k = quotient(span.lo, u.v.tiles);
+    u.b = static_cast<int>(quotient(k, a.c.Hk));
+    u.h = static_cast<int>(k - static_cast<int64_t>(u.b) * a.c.Hk);
     u.begin = k * u.v.tiles;
     u.end = u.begin + u.v.tiles;
     return true;
@@ -264,7 +270,7 @@ __device__ __forceinline__ bool span_of(const AttnArgs& a, int i, int n, Span& s
   __syncthreads();
   u.b = static_cast<int>(found[0]);
   visit_unit<KEYS>(a, u, 0, a.T);
-  const int64_t h = (span.lo - found[1]) / u.v.tiles;
+  const int64_t h = quotient(span.lo - found[1], u.v.tiles);
   u.h = static_cast<int>(h);
   u.begin = found[1] + h * u.v.tiles;
   u.end = u.begin + u.v.tiles;
@@ -286,12 +292,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
   using TL = Tile<D, BITS>;
   constexpr int KEYS = TL::kKeys, BLOCKS = KEYS / 16, GROUPS = D / kGroup, STEPS = D / 16, ROW = TL::kRow;
   constexpr int NQ = sizeof(QT) == 4 ? 2 : 1, NP = sizeof(QT) == 4 ? 3 : 1;   // terms of a query, of a probability
+  static_assert(D / 4 * 8 <= kWarps * 32, "a row of queries is loaded by the threads of one pass");
   constexpr int SW = GROUPS / 2;                       // words of a position's scales
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t full[kStages];
   __shared__ uint32_t done[kStages];                   // warps that have left a stage
   __shared__ Stage stages[kStages];
   __shared__ Feed feed;
+  __shared__ Unit first_unit;
+  __shared__ __align__(16) uint32_t q_terms[NT][NQ][32][2 * STEPS + 4];   // (rows of odd numbers of 16 bytes: no bank conflicts)
+  __shared__ float q_factor[8 * NT], q_init[8 * NT][GROUPS];
   __shared__ int64_t scan[kWarps];
   __shared__ float row_m[kWarps][8 * NT], row_l[kWarps][8 * NT];
   const AttnArgs& a = ta.a;
@@ -340,7 +350,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
     while (f.at >= f.end) {
       f.at -= static_cast<int>(f.u.end - f.u.begin);
       next_unit<KEYS>(a, f.u);
-      f.end = static_cast<int>(min(f.u.end, span.hi) - f.u.begin);
+      f.end = static_cast<int>(min(f.u.end, f.hi) - f.u.begin);
     }
     const Visit& v = f.u.v;
     const bool sink = f.at < v.sink_tiles;
@@ -372,12 +382,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
     }
   };
   if (threadIdx.x == 0) {
-    if (span.lo >= span.hi) stages[0].u = u;           // a unit without tiles (not split): zeros
-    feed.u = u;
+    feed.u = first_unit = u;
+    feed.lo = span.lo;
+    feed.hi = span.hi;
     feed.left = span.hi - span.lo;
     feed.at = static_cast<int>(span.lo - u.begin);
     feed.end = static_cast<int>(min(u.end, span.hi) - u.begin);
-    for (int i = 0; i < kStages; ++i) load(i);
   }
   __syncthreads();
 
@@ -386,67 +396,82 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
   const uint32_t lane_at = row16 + ((static_cast<uint32_t>(lane >> 4) * 16u) ^ ((row16 >> 3) & (ROW - 16u)));
 
   int used = 0;
-  bool ok = true;
+  bool ok = true, first = true;
   for (;;) {                                           // one unit after the other
-    const Unit& unit = stages[used % kStages].u;       // (of this stage's time: it is read before the stage is left)
+    const Unit& unit = first ? first_unit : stages[used % kStages].u;   // (of that stage's time: it is read before the stage is left)
     const int ub = unit.b, uh = unit.h, hi_row = unit.v.hi_row;
     const int64_t pos = unit.pos, count = unit.count;
-    const bool whole = unit.begin >= span.lo && unit.end <= span.hi, last_unit = unit.end >= span.hi;
-    float* part = whole ? nullptr : a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (unit.begin < span.lo ? 0 : 1)) * Part<D, NT>::kFloats;
-    // Q's fragments: column (a row of queries) g of tile n; b0, b1 of product step ks in the order in which the codes come.
-    uint32_t qf[NT][STEPS][NQ][2];
-    float factor[NT][2], init[NT][GROUPS][2];          // of rows 2 tig, 2 tig + 1: score to log2 domain; what takes the codes' bias off
-#pragma unroll
+    const bool whole = unit.begin >= feed.lo && unit.end <= feed.hi, last_unit = unit.end >= feed.hi, any = feed.lo < feed.hi;
+    float* part = whole ? nullptr : a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (unit.begin < feed.lo ? 0 : 1)) * Part<D, NT>::kFloats;
+    // Q: a thread takes four columns of a row, a power of two brings the row's largest value near 64, and the terms go to
+    // shared memory in the order in which lanes need them: word 2 ks + i of lane 4 (row mod 8) + tig is b_i of product step ks.
     for (int n = 0; n < NT; ++n) {
-      const int r = r0 + 8 * n + g, t = r / a.group;
-      const QT* src = static_cast<const QT*>(a.q) + ub * a.batch_stride + static_cast<int64_t>(t) * a.row_stride +
-                      static_cast<int64_t>(uh * a.group + (r - t * a.group)) * D;
-      float x[D / 4], most = 0.0f;                     // a lane's columns: of every group eight (4 bits), or twice four
-#pragma unroll
-      for (int i = 0; i < D / 4; ++i) x[i] = 0.0f;
-      if (8 * n + g < rows) {
-#pragma unroll
-        for (int i = 0; i < D / 4; i += BITS == 4 ? 8 : 4) {
-          if constexpr (BITS == 4) load_row<8>(src + 4 * i + 8 * tig, x + i);
-          else load_row<4>(src + 4 * i + 4 * tig, x + i);
-        }
+      constexpr int kPer = D / 4;                      // threads of a row: 16 or 32
+      const int rr = 8 * n + static_cast<int>(threadIdx.x) / kPer, c4 = static_cast<int>(threadIdx.x) % kPer, r = r0 + rr;
+      if (rr >= 8 * n + 8) break;                      // whole warps
+      float x[4] = {};
+      if (rr < rows) {
+        const int t = r / a.group;
+        load_row<4>(static_cast<const QT*>(a.q) + ub * a.batch_stride + static_cast<int64_t>(t) * a.row_stride +
+                        static_cast<int64_t>(uh * a.group + (r - t * a.group)) * D + 4 * c4, x);
       }
+      if (first && n == 0 && threadIdx.x == 0) load(0);   // while the rows are on their way
+      float most = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
 #pragma unroll
-      for (int i = 0; i < D / 4; ++i) most = fmaxf(most, fabsf(x[i]));
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      for (int o = 1; o < kPer; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
       const int e = static_cast<int>(__float_as_uint(most) >> 23) - 127;           // 128: not finite
       const int up = most == 0.0f || e == 128 ? 0 : max(min(6 - e, 126), -100);    // most * 2^up is in [64, 128), or near it
       const float f = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
 #pragma unroll
-      for (int i = 0; i < D / 4; ++i) x[i] *= f;
+      for (int i = 0; i < 4; ++i) x[i] *= f;
+      float sum = (x[0] + x[1]) + (x[2] + x[3]);       // of a group: eight threads
 #pragma unroll
-      for (int ks = 0; ks < STEPS; ++ks)
+      for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if ((c4 & 7) == 0) q_init[rr][c4 / 8] = sum * (BITS == 4 ? -8.0f * 0x1p-24f : -128.0f * 0x1p-24f);
+      if (c4 == 0) q_factor[rr] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + 24 - up) << 23);   // up is from -100 to 126
+      if constexpr (BITS == 4) {                       // columns 8 tig + c of a group: pairs (c, c + 4); odd c times 2^-4
+        const int row_lane = (rr & 7) * 4 + ((c4 >> 1) & 3), half = c4 & 1, word = 4 * (c4 >> 3);
+        uint32_t t01[NQ], t23[NQ];
+        terms_f16<NQ>(x[0], x[1] * 0.0625f, t01);
+        terms_f16<NQ>(x[2], x[3] * 0.0625f, t23);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          // 4 bits: a word of eight codes gives two steps, pairs (c, c + 4); 8 bits: a word of four gives one
-          const float* y = x + (BITS == 4 ? 8 * (ks / 2) + 2 * (ks & 1) + i : 4 * ks + 2 * i);
-          const float w = BITS == 4 && i == 1 ? 0.0625f : 1.0f;
-          uint32_t tt[NQ];
-          terms_f16<NQ>(y[0] * w, y[BITS == 4 ? 4 : 1] * w, tt);
-#pragma unroll
-          for (int z = 0; z < NQ; ++z) qf[n][ks][z][i] = tt[z];
+        for (int z = 0; z < NQ; ++z) {
+          uint16_t* w = reinterpret_cast<uint16_t*>(&q_terms[n][z][row_lane][word]) + half;
+          w[0] = static_cast<uint16_t>(t01[z]);
+          w[2] = static_cast<uint16_t>(t01[z] >> 16);
+          w[4] = static_cast<uint16_t>(t23[z]);
+          w[6] = static_cast<uint16_t>(t23[z] >> 16);
         }
+      } else {                                         // columns 4 tig + c of a step: pairs of neighbours
+        const int row_lane = (rr & 7) * 4 + (c4 & 3), word = 2 * (c4 >> 2);
+        uint32_t t01[NQ], t23[NQ];
+        terms_f16<NQ>(x[0], x[1], t01);
+        terms_f16<NQ>(x[2], x[3], t23);
 #pragma unroll
-      for (int gr = 0; gr < GROUPS; ++gr) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum += x[8 * gr + i];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        sum *= BITS == 4 ? -8.0f * 0x1p-24f : -128.0f * 0x1p-24f;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) init[n][gr][c] = __shfl_sync(0xffffffffu, sum, (2 * tig + c) * 4);
+        for (int z = 0; z < NQ; ++z) {
+          q_terms[n][z][row_lane][word] = t01[z];
+          q_terms[n][z][row_lane][word + 1] = t23[z];
+        }
       }
+    }
+    __syncthreads();
+    if (first && threadIdx.x == 0)
+#pragma unroll 1
+      for (int i = 1; i < kStages; ++i) load(i);
+    first = false;
+    uint32_t qf[NT][NQ][2 * STEPS];
+    float factor[NT][2], init[NT][GROUPS][2];          // of rows 2 tig, 2 tig + 1: score to log2 domain; what takes the codes' bias off
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int z = 0; z < NQ; ++z)
+#pragma unroll
+        for (int i = 0; i < 2 * STEPS; ++i) qf[n][z][i] = q_terms[n][z][lane][i];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int other = __shfl_sync(0xffffffffu, up, (2 * tig + c) * 4);
-        factor[n][c] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + 24 - other) << 23);   // other is from -100 to 126
+        factor[n][c] = q_factor[8 * n + 2 * tig + c];
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr) init[n][gr][c] = q_init[8 * n + 2 * tig + c][gr];
       }
     }
     // Rows 2 tig and 2 tig + 1 of tile n: their positions, reference points (log2 domain) and sums.
@@ -488,8 +513,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int y = 0; y < NQ; ++y) {
-                if ((ks & 1) == 0 && y == 0) mma_f16_from(acc[n], f, qf[n][ks][y][0], qf[n][ks][y][1], init[n][ks / 2]);
-                else mma_f16(acc[n], f, qf[n][ks][y][0], qf[n][ks][y][1]);
+                if ((ks & 1) == 0 && y == 0) mma_f16_from(acc[n], f, qf[n][y][2 * ks], qf[n][y][2 * ks + 1], init[n][ks / 2]);
+                else mma_f16(acc[n], f, qf[n][y][2 * ks], qf[n][y][2 * ks + 1]);
               }
           };
           auto scaled = [&](int gr) {
@@ -661,7 +686,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
     };
 
     int st = used % kStages;
-    for (bool more = span.lo < span.hi; more && ok; ++used) {
+    for (bool more = any; more && ok; ++used) {
       st = used % kStages;
       ok = mbar_wait_bounded_w(&full[st], (used / kStages) & 1, a.status, 210);
       if (!ok) break;
@@ -760,7 +785,7 @@ template <typename QT, int D, int BITS, int NT>
 __global__ void __launch_bounds__(kJoinThreads) kvq_join_kernel(const TokenArgs ta, int ctas) {
   constexpr int KEYS = Tile<D, BITS>::kKeys, kRows = 8 * NT, kOut = (kRows * D + kJoinThreads - 1) / kJoinThreads;
   __shared__ int64_t scan[kJoinThreads / 32];
-  __shared__ float weight[kJoinParts][kRows], row_m[kRows], row_l[kRows];
+  __shared__ float weight[kJoinParts][kRows], part_l[kJoinParts][kRows], row_m[kRows], row_l[kRows];
   const AttnArgs& a = ta.a;
   pdl_launch();
   pdl_wait();
@@ -790,7 +815,7 @@ __global__ void __launch_bounds__(kJoinThreads) kvq_join_kernel(const TokenArgs 
     return;
   }
   const int64_t end = begin + v.tiles;
-  const int c0 = static_cast<int>(((begin + 1) * ctas - 1) / all), c1 = static_cast<int>((end * ctas - 1) / all);
+  const int c0 = static_cast<int>(quotient((begin + 1) * ctas - 1, all)), c1 = static_cast<int>(quotient(end * ctas - 1, all));
   if (c0 == c1) return;
   // The first part is its CTA's last unit (or its only one, which began before), the others are their CTAs' first.
   const float* first = a.part + (static_cast<int64_t>(c0) * 2 + (begin < span_start(all, c0, ctas) ? 0 : 1)) * Part<D, NT>::kFloats;
@@ -805,7 +830,11 @@ __global__ void __launch_bounds__(kJoinThreads) kvq_join_kernel(const TokenArgs 
   for (int p0 = c0; p0 <= c1; p0 += kJoinParts) {
     const int n = min(kJoinParts, c1 - p0 + 1);
     __syncthreads();
-    for (int i = threadIdx.x; i < n * kRows; i += kJoinThreads) weight[i / kRows][i % kRows] = part_of(p0 + i / kRows)[kRows * D + i % kRows];
+    for (int i = threadIdx.x; i < n * kRows; i += kJoinThreads) {
+      const float* p = part_of(p0 + i / kRows) + kRows * D + i % kRows;
+      weight[i / kRows][i % kRows] = p[0];
+      part_l[i / kRows][i % kRows] = p[kRows];
+    }
     __syncthreads();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float again[NT];                                   // what the sums of earlier parts are multiplied by (rows warp, warp + 8)
@@ -820,7 +849,7 @@ __global__ void __launch_bounds__(kJoinThreads) kvq_join_kernel(const TokenArgs 
       for (int i = lane; i < n; i += 32) {
         const float w = ex2(weight[i][r] - ref);
         weight[i][r] = w;
-        l += w * part_of(p0 + i)[kRows * D + kRows + r];
+        l += w * part_l[i][r];
       }
       l = warp_sum(l);
       again[x] = ex2(row_m[r] - ref);
