@@ -2,9 +2,9 @@
 // groups. out = sum_j softmax_j(scale * q . k_j) v_j, over the positions that a row sees.
 //
 // A block of R <= 8 * NT rows (the query heads of one key/value head times the new tokens) shares the cache rows, which
-// are read once. Each of a CTA's eight warps takes tiles of 2 KB of key codes (16 to 64 positions); TMA brings a stage of eight
-// tiles with few, large copies (issuing one takes longer than 2 KB take to arrive: a copy a tile fell behind), two stages in shared
-// memory, and the warp that leaves a stage last has it filled again. The codes become exact 16-bit floating numbers in registers, in the layout
+// are read once. Seven of a CTA's warps take tiles of 2 KB of key codes (16 to 64 positions); the eighth has TMA bring a stage of seven
+// tiles with few, large copies (issuing one takes longer than 2 KB take to arrive: a copy a tile fell behind), three stages in shared
+// memory. The codes become exact 16-bit floating numbers in registers, in the layout
 // that mma.sync wants, without another trip through shared memory:
 //   scores   S^T[16 positions, 8 rows] = K Q^T: ldmatrix gives a lane a word of codes of one group and position; which columns meet
 //            in which step of the product is free, as long as Q is laid out the same. The codes enter as fp16 numbers, unscaled, a
@@ -25,7 +25,8 @@ namespace ctdk {
 namespace kvq {
 namespace {
 
-constexpr int kWarps = 8, kStages = 3;
+constexpr int kWarps = 7, kStages = 3;   // warps that compute (an eighth one loads: with 128 registers a thread, two CTAs fill an SM)
+constexpr int kThreads = (kWarps + 1) * 32;
 constexpr float kSlack = 8.0f;
 
 template <int D, int BITS>
@@ -34,11 +35,13 @@ struct Tile {
   static constexpr int kKeys = 2048 / kRow;                               // positions of a tile
   static constexpr int kCodes = kKeys * kRow, kScales = kKeys * kScaleRow;
   static constexpr int kBytes = 2 * (kCodes + kScales);                   // that one tile brings
-  static constexpr int kBox = kWarps * kKeys < 256 ? kWarps * kKeys : 256;   // positions of a copy (a box has no more)
+  static constexpr int kBoxes = (kWarps * kKeys + 255) / 256, kBox = kWarps * kKeys / kBoxes;   // copies of a stage (a box is 256 positions at most)
+  static_assert(kWarps * kKeys % kBoxes == 0, "equal copies");
   static constexpr int kPitch = D + 4;                                    // floats of a row in the exchange of partial results
   static constexpr int kExchange = kWarps * 8 * kPitch * 4;                // it takes the place of a stage that has been used
   static_assert(kExchange <= kWarps * 2 * (kCodes + kScales), "exchange");
-  static constexpr int kSmem = 1024 + kWarps * kStages * kBytes;
+  static constexpr int kStageBytes = (kWarps * kBytes + 1023) / 1024 * 1024;   // (swizzled tiles start at multiples of 1 KB)
+  static constexpr int kSmem = 1024 + kStages * kStageBytes;
 };
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
@@ -126,12 +129,6 @@ __device__ __forceinline__ void load_row(const __nv_bfloat16* p, float* x) {
 struct Span {
   int64_t lo, hi;      // tiles of all units, numbered through
 };
-// Counts a warp that is done with a stage's contents; returns how many were before.
-__device__ __forceinline__ uint32_t leave(uint32_t* count) {
-  uint32_t n;
-  asm volatile("atom.acq_rel.cta.shared::cta.add.u32 %0, [%1], 1;" : "=r"(n) : "r"(smem_u32(count)) : "memory");
-  return n;
-}
 // As bulk_load of common.cuh, without a cache hint.
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
@@ -230,6 +227,12 @@ __device__ __forceinline__ int64_t cta_sum(int64_t x, int64_t* before, int64_t* 
   return all;
 }
 
+// CTAs that share `all` tiles: no more than get one for each of their warps, so none of them is left without (how many tiles
+// there are the host may not know).
+__device__ __forceinline__ int sharing(int64_t all, int ctas) {
+  const int64_t n = quotient(all + kWarps - 1, kWarps);
+  return n < ctas ? static_cast<int>(n) : ctas;
+}
 // The CTA's part `i` of `n` of all units' tiles, and the unit that holds its first one. False: it has none.
 template <int KEYS>
 __device__ __forceinline__ bool span_of(const AttnArgs& a, int i, int n, Span& span, Unit& u, int64_t* smem) {
@@ -237,8 +240,9 @@ __device__ __forceinline__ bool span_of(const AttnArgs& a, int i, int n, Span& s
   if (a.pos == nullptr && a.count == nullptr) {
     visit_unit<KEYS>(a, u, 0, a.T);
     const int64_t all = static_cast<int64_t>(u.v.tiles) * a.c.B * a.c.Hk;
+    n = sharing(all, n);
+    if (i >= n) return false;
     span = {span_start(all, i, n), span_start(all, i + 1, n)};
-    if (span.lo >= span.hi) return false;
     const int64_t k = quotient(span.lo, u.v.tiles);
     u.b = static_cast<int>(quotient(k, a.c.Hk));
     u.h = static_cast<int>(k - static_cast<int64_t>(u.b) * a.c.Hk);
@@ -255,8 +259,9 @@ __device__ __forceinline__ bool span_of(const AttnArgs& a, int i, int n, Span& s
   const int step = static_cast<int>(blockDim.x);
   int64_t x = mine(0), before, all = cta_sum(x, &before, smem);
   for (int b0 = step; b0 < a.c.B; b0 += step) all += cta_sum(mine(b0), nullptr, smem);
+  n = sharing(all, n);
+  if (i >= n) return false;
   span = {span_start(all, i, n), span_start(all, i + 1, n)};
-  if (span.lo >= span.hi) return false;
   int64_t base = 0;
   for (int b0 = 0;;) {
     if (span.lo >= base + before && span.lo < base + before + x) found[0] = b0 + threadIdx.x, found[1] = base + before;
@@ -287,29 +292,27 @@ struct Part {
 };
 
 template <typename QT, int D, int BITS, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
     kvq_token_kernel(const __grid_constant__ Maps maps, const TokenArgs ta) {
   using TL = Tile<D, BITS>;
   constexpr int KEYS = TL::kKeys, BLOCKS = KEYS / 16, GROUPS = D / kGroup, STEPS = D / 16, ROW = TL::kRow;
   constexpr int NQ = sizeof(QT) == 4 ? 2 : 1, NP = sizeof(QT) == 4 ? 3 : 1;   // terms of a query, of a probability
-  static_assert(D / 4 * 8 <= kWarps * 32, "a row of queries is loaded by the threads of one pass");
   constexpr int SW = GROUPS / 2;                       // words of a position's scales
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t full[kStages];
-  __shared__ uint32_t done[kStages];                   // warps that have left a stage
+  __shared__ uint64_t full[kStages], empty[kStages];
   __shared__ Stage stages[kStages];
   __shared__ Feed feed;
   __shared__ Unit first_unit;
   __shared__ __align__(16) uint32_t q_terms[NT][NQ][32][2 * STEPS + 4];   // (rows of odd numbers of 16 bytes: no bank conflicts)
   __shared__ float q_factor[8 * NT], q_init[8 * NT][GROUPS];
-  __shared__ int64_t scan[kWarps];
+  __shared__ int64_t scan[kWarps + 1];
   __shared__ float row_m[kWarps][8 * NT], row_l[kWarps][8 * NT];
   const AttnArgs& a = ta.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3;
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   if (threadIdx.x < kStages) {
     mbar_init(&full[threadIdx.x], 1);
-    done[threadIdx.x] = 0;
+    mbar_init(&empty[threadIdx.x], kWarps);
   }
   if (threadIdx.x == 0) {
     mbar_fence_init();
@@ -343,44 +346,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
   }
   const int rows = min(8 * NT, ta.rows - r0);
 
-  // One thread asks for a stage's tiles; loads run ahead of the products, over the units' borders.
-  auto load = [&](int st) {
-    Feed& f = feed;
-    if (f.left <= 0) return;
-    while (f.at >= f.end) {
-      f.at -= static_cast<int>(f.u.end - f.u.begin);
-      next_unit<KEYS>(a, f.u);
-      f.end = static_cast<int>(min(f.u.end, f.hi) - f.u.begin);
-    }
-    const Visit& v = f.u.v;
-    const bool sink = f.at < v.sink_tiles;
-    const int n = min((sink ? min(v.sink_tiles, f.end) : f.end) - f.at, kWarps), j = v.tile_at(f.at) * KEYS, bh = f.u.b * a.c.Hk + f.u.h;
-    f.at += n;
-    f.left -= n;
-    Stage& g = stages[st];
-    g.u = f.u;
-    g.j = j;
-    g.n = n;
-    g.last = f.at == f.end;
-    g.plain_lo = sink || a.window == 0 ? 0 : v.hi_row - a.window;
-    g.plain_hi = v.lo_row - KEYS + 1;
-    if (sink) g.plain_hi = min(g.plain_hi, a.sinks - KEYS);
-    const int64_t sc = (static_cast<int64_t>(bh) * a.c.capacity + j) * GROUPS;
-    unsigned char* codes = smem + st * kWarps * TL::kBytes;
-    unsigned char* scales = codes + 2 * kWarps * TL::kCodes;
-    mbar_expect_tx(&full[st], n * TL::kBytes);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      unsigned char* dst = codes + i * kWarps * TL::kCodes;
-      if (n == kWarps) {
-#pragma unroll
-        for (int x = 0; x < kWarps * KEYS; x += TL::kBox) tma_load_3d(dst + x * ROW, &maps.all[i], &full[st], 0, j + x, bh);
-      } else {
-        for (int x = 0; x < n; ++x) tma_load_3d(dst + x * TL::kCodes, &maps.few[i], &full[st], 0, j + x * KEYS, bh);
-      }
-      bulk_load(scales + i * kWarps * TL::kScales, a.c.scales[i] + sc, n * TL::kScales, &full[st]);
-    }
-  };
   if (threadIdx.x == 0) {
     feed.u = first_unit = u;
     feed.lo = span.lo;
@@ -390,32 +355,78 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
     feed.end = static_cast<int>(min(u.end, span.hi) - u.begin);
   }
   __syncthreads();
+  if (warp == kWarps) {
+    // The loading warp runs ahead of the others, over the units' borders.
+    Feed& f = feed;
+    for (int k = 0; f.left > 0; ++k) {
+      const int st = k % kStages;
+      if (k >= kStages && !mbar_wait_bounded_w(&empty[st], (k / kStages + 1) & 1, a.status, 212)) break;
+      if (lane == 0) {
+        while (f.at >= f.end) {
+          f.at -= static_cast<int>(f.u.end - f.u.begin);
+          next_unit<KEYS>(a, f.u);
+          f.end = static_cast<int>(min(f.u.end, f.hi) - f.u.begin);
+        }
+        const Visit& v = f.u.v;
+        const bool sink = f.at < v.sink_tiles;
+        const int n = min((sink ? min(v.sink_tiles, f.end) : f.end) - f.at, kWarps), j = v.tile_at(f.at) * KEYS, bh = f.u.b * a.c.Hk + f.u.h;
+        f.at += n;
+        f.left -= n;
+        Stage& g = stages[st];
+        g.u = f.u;
+        g.j = j;
+        g.n = n;
+        g.last = f.at == f.end;
+        g.plain_lo = sink || a.window == 0 ? 0 : v.hi_row - a.window;
+        g.plain_hi = v.lo_row - KEYS + 1;
+        if (sink) g.plain_hi = min(g.plain_hi, a.sinks - KEYS);
+        const int64_t sc = (static_cast<int64_t>(bh) * a.c.capacity + j) * GROUPS;
+        unsigned char* codes = smem + st * TL::kStageBytes;
+        unsigned char* scales = codes + 2 * kWarps * TL::kCodes;
+        mbar_expect_tx(&full[st], n * TL::kBytes);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          unsigned char* dst = codes + i * kWarps * TL::kCodes;
+          if (n == kWarps) {
+#pragma unroll
+            for (int x = 0; x < kWarps * KEYS; x += TL::kBox) tma_load_3d(dst + x * ROW, &maps.all[i], &full[st], 0, j + x, bh);
+          } else {
+            for (int x = 0; x < n; ++x) tma_load_3d(dst + x * TL::kCodes, &maps.few[i], &full[st], 0, j + x * KEYS, bh);
+          }
+          bulk_load(scales + i * kWarps * TL::kScales, a.c.scales[i] + sc, n * TL::kScales, &full[st]);
+        }
+      }
+      __syncwarp();
+    }
+    return;
+  }
 
   // A lane's row address for ldmatrix (16 rows, two neighbouring chunks of 16 bytes), swizzled as TMA has written it.
   const uint32_t row16 = static_cast<uint32_t>(lane & 15) * ROW;
   const uint32_t lane_at = row16 + ((static_cast<uint32_t>(lane >> 4) * 16u) ^ ((row16 >> 3) & (ROW - 16u)));
 
+  const auto together = []() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); };   // the computing warps
   int used = 0;
   bool ok = true, first = true;
   for (;;) {                                           // one unit after the other
-    const Unit& unit = first ? first_unit : stages[used % kStages].u;   // (of that stage's time: it is read before the stage is left)
+    if (!first) ok = mbar_wait_bounded_w(&full[used % kStages], (used / kStages) & 1, a.status, 213);   // (the stage names its unit)
+    const Unit& unit = first || !ok ? first_unit : stages[used % kStages].u;
     const int ub = unit.b, uh = unit.h, hi_row = unit.v.hi_row;
     const int64_t pos = unit.pos, count = unit.count;
-    const bool whole = unit.begin >= feed.lo && unit.end <= feed.hi, last_unit = unit.end >= feed.hi, any = feed.lo < feed.hi;
+    const bool whole = unit.begin >= feed.lo && unit.end <= feed.hi, last_unit = unit.end >= feed.hi, any = ok && feed.lo < feed.hi;
     float* part = whole ? nullptr : a.part + (static_cast<int64_t>(blockIdx.x) * 2 + (unit.begin < feed.lo ? 0 : 1)) * Part<D, NT>::kFloats;
     // Q: a thread takes four columns of a row, a power of two brings the row's largest value near 64, and the terms go to
     // shared memory in the order in which lanes need them: word 2 ks + i of lane 4 (row mod 8) + tig is b_i of product step ks.
-    for (int n = 0; n < NT; ++n) {
-      constexpr int kPer = D / 4;                      // threads of a row: 16 or 32
-      const int rr = 8 * n + static_cast<int>(threadIdx.x) / kPer, c4 = static_cast<int>(threadIdx.x) % kPer, r = r0 + rr;
-      if (rr >= 8 * n + 8) break;                      // whole warps
+    constexpr int kPer = D / 4, kAtOnce = kWarps * 32 / kPer;   // threads of a row: 16 or 32
+#pragma unroll 1
+    for (int rr = static_cast<int>(threadIdx.x) / kPer; rr < 8 * NT; rr += kAtOnce) {
+      const int n = rr / 8, c4 = static_cast<int>(threadIdx.x) % kPer, r = r0 + rr;
       float x[4] = {};
       if (rr < rows) {
         const int t = r / a.group;
         load_row<4>(static_cast<const QT*>(a.q) + ub * a.batch_stride + static_cast<int64_t>(t) * a.row_stride +
                         static_cast<int64_t>(uh * a.group + (r - t * a.group)) * D + 4 * c4, x);
       }
-      if (first && n == 0 && threadIdx.x == 0) load(0);   // while the rows are on their way
       float most = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
 #pragma unroll
       for (int o = 1; o < kPer; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -454,11 +465,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
         }
       }
     }
-    __syncthreads();
-    if (first && threadIdx.x == 0)
-#pragma unroll 1
-      for (int i = 1; i < kStages; ++i) load(i);
     first = false;
+    together();
     uint32_t qf[NT][NQ][2 * STEPS];
     float factor[NT][2], init[NT][GROUPS][2];          // of rows 2 tig, 2 tig + 1: score to log2 domain; what takes the codes' bias off
 #pragma unroll
@@ -685,7 +693,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
       }
     };
 
-    int st = used % kStages;
+    int st = used % kStages, all_ok;
     for (bool more = any; more && ok; ++used) {
       st = used % kStages;
       ok = mbar_wait_bounded_w(&full[st], (used / kStages) & 1, a.status, 210);
@@ -693,8 +701,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
       const Stage& f = stages[st];
       more = f.last == 0;
       if (warp < f.n) {
-        const uint32_t kbase = smem_u32(smem) + st * kWarps * TL::kBytes + warp * TL::kCodes;
-        const uint32_t ksc = smem_u32(smem) + st * kWarps * TL::kBytes + 2 * kWarps * TL::kCodes + warp * TL::kScales;
+        const uint32_t kbase = smem_u32(smem) + st * TL::kStageBytes + warp * TL::kCodes;
+        const uint32_t ksc = smem_u32(smem) + st * TL::kStageBytes + 2 * kWarps * TL::kCodes + warp * TL::kScales;
         const int j0 = f.j + warp * KEYS;
         if (j0 >= f.plain_lo && j0 <= f.plain_hi) {
           tile(std::true_type{}, j0, kbase, ksc);
@@ -703,10 +711,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
         }
       }
       __syncwarp();
-      if (lane == 0 && leave(&done[st]) == kWarps - 1) {   // the last warp to leave a stage has it filled again
-        done[st] = 0;
-        if (more) load(st);                            // the unit's last stage is needed below first
-      }
+      if (lane == 0 && more) mbar_arrive(&empty[st]);  // (the unit's last stage is needed below first)
     }
 
     // ---- the warps' results of this unit together
@@ -722,9 +727,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
           row_l[warp][8 * n + 2 * tig + c] = x;
         }
       }
-    // All warps have left the stage st: its room serves for the exchange.
-    __syncthreads();
-    float* exchange = reinterpret_cast<float*>(smem + st * kWarps * TL::kBytes);
+    // All warps have left the stage st: its room serves for the exchange. (They give up together.)
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.pred q, 1, %2, p;\n selp.b32 %0, 1, 0, q;\n}"
+                 : "=r"(all_ok) : "r"(static_cast<int>(ok)), "n"(kWarps * 32) : "memory");
+    ok = all_ok != 0;
+    float* exchange = reinterpret_cast<float*>(smem + st * TL::kStageBytes);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -735,7 +742,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
         e[8] = o[n][i][2];
         e[TL::kPitch + 8] = o[n][i][3];
       }
-      __syncthreads();
+      together();
       for (int i = threadIdx.x; i < 8 * D; i += kWarps * 32) {
         const int r = i / D, e = i % D, rr = 8 * n + r;
         if (rr >= rows) continue;
@@ -765,16 +772,15 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1)
           store_out(static_cast<QT*>(a.out) + ((static_cast<int64_t>(ub) * a.T + t) * a.H + uh * a.group + hg) * D + d, valid ? sum / ll : 0.0f);
         }
       }
-      __syncthreads();
+      together();
     }
-    if (last_unit) break;
-    if (threadIdx.x == 0) {
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // copies may write where the exchange was
-      load(st);
-    }
+    if (last_unit || !ok) break;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // copies may write where the exchange was
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[st]);
   }
-  for (int i = 0; !ok && i < kStages; ++i, ++used)     // copies still on their way
-    mbar_wait_bounded_w(&full[used % kStages], (used / kStages) & 1, a.status, 211);
+  if (!ok)                                             // copies still on their way
+    for (int i = 0; i < kStages; ++i, ++used) mbar_wait_bounded_w(&full[used % kStages], (used / kStages) & 1, a.status, 211);
 }
 
 // Joins the parts of the units that several CTAs worked on, in the order of their positions, and writes zeros for the units that
@@ -814,6 +820,7 @@ __global__ void __launch_bounds__(kJoinThreads) kvq_join_kernel(const TokenArgs 
     }
     return;
   }
+  ctas = sharing(all, ctas);
   const int64_t end = begin + v.tiles;
   const int c0 = static_cast<int>(quotient((begin + 1) * ctas - 1, all)), c1 = static_cast<int>(quotient(end * ctas - 1, all));
   if (c0 == c1) return;
@@ -922,7 +929,7 @@ int launch_token(const TokenArgs& ta, int ctas, cudaStream_t s) {
     if (rc != CTDK_OK) return rc;
   }
   cudaError_t e = raise_dynamic_smem(reinterpret_cast<const void*>(kernel), kSmem);
-  if (e == cudaSuccess) e = launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kWarps * 32), kSmem, s, maps, ta);
+  if (e == cudaSuccess) e = launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), kSmem, s, maps, ta);
   if (e != cudaSuccess) return fail(CTDK_ELAUNCH, "kvq_attn: %s", cudaGetErrorString(e));
   if (const int rc = check_launch("kvq_attn"); rc != CTDK_OK || !ta.split) return rc;
   e = launch_pdl(kvq_join_kernel<QT, D, BITS, NT>, dim3(static_cast<unsigned>(ta.a.c.B * ta.a.c.Hk)), dim3(kJoinThreads), 0, s, ta, ctas);

@@ -195,6 +195,16 @@ def test_long_caches_are_split_over_the_device(K, bits, dtype, H, Hk, D, window,
 
 
 @pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("H,Hk,D", [(9, 3, 64), (16, 8, 128)])
+@pytest.mark.parametrize("lengths", [[1, 1], [31, 32], [33, 130], [0, 450], [0, 0]])
+def test_short_sequences_in_a_large_cache(K, bits, H, Hk, D, lengths):
+    """The host sees the capacity only: far more CTAs than there is work."""
+    cache = filled(K, 2, Hk, 450, D, bits, 25, capacity=8192)
+    for dtype in (F32, BF16):
+        check(K, cache, rnd((2, 1, H, D), 26, 1.0, dtype).cuda(), [n - 1 for n in lengths], n=450)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("H,Hk,D,T", [(4, 4, 64, 5), (16, 8, 128, 3), (8, 2, 64, 5), (15, 5, 64, 16), (4, 2, 128, 40), (3, 1, 64, 129)])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (20, 3), (1, 0)])
