@@ -54,6 +54,11 @@ __device__ __forceinline__ uint32_t add_f16x2(uint32_t x, uint32_t c) {
   return d;
 }
 
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t x, uint32_t s) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(s));
+  return d;
+}
 #endif  // __CUDACC__
 
 // Every conversion below is exact, one operation behind the extraction of the bits.

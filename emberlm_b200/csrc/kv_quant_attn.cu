@@ -963,7 +963,7 @@ int64_t ctdk_kvq_attn_workspace_bytes(const ctdk_kvq_cache* cache, int64_t T, in
   if (const int rc = kvq::check_cache(cache, "kvq_attn"); rc != CTDK_OK) return rc;
   CTDK_REQUIRE(T >= 0 && H > 0 && H % cache->Hk == 0, "kvq_attn: heads must be a multiple of kv heads");
   const int64_t rows = T * (H / cache->Hk);
-  return rows <= 16 ? kvq::part_bytes(cache->D, rows) : 0;
+  return rows <= 16 ? kvq::part_bytes(cache->D, rows) : kvq::attn_tc_bytes(cache->B, cache->Hk, cache->D, rows);
 }
 
 int ctdk_kvq_attn(const ctdk_kvq_cache* cache, const void* q, int dtype, int64_t row_stride, int64_t batch_stride, int64_t T, int H,
@@ -1004,6 +1004,13 @@ int ctdk_kvq_attn(const ctdk_kvq_cache* cache, const void* q, int dtype, int64_t
   a.status = device_status_word();
   if (a.status == nullptr) return fail(CTDK_ELAUNCH, "kvq_attn: no status word");
   const int64_t rows = T * a.group, units = cache->B * cache->Hk;
+  // More rows than two tiles of mma.sync take: the prompt kernel, whose tiles have 128.
+  if (rows > 16) {
+    const int64_t need = kvq::attn_tc_bytes(cache->B, cache->Hk, cache->D, rows);
+    CTDK_REQUIRE(need == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= need),
+                 "kvq_attn: the workspace needs %lld bytes, 16-byte aligned", static_cast<long long>(need));
+    return kvq::attn_tc(a, dtype, cache->bits, cache->D, static_cast<cudaStream_t>(stream));
+  }
   ta.rows = static_cast<int>(rows);
   ta.bits = kvq::patterns();
   const int nt = rows <= 8 ? 1 : 2;

@@ -63,8 +63,8 @@ __device__ __forceinline__ bool sees(int i, int j, int w, int s) { return j <= i
 #endif
 
 int check_cache(const ctdk_kvq_cache* c, const char* what);   // kv_quant.cu
-// kv_quant_attn_tc.cu: prompts.
-bool attn_tc_ok(const AttnArgs& a, int D);
+// kv_quant_attn_tc.cu: prompts, in a workspace (a.part) of attn_tc_bytes for rows = T * group.
+int64_t attn_tc_bytes(int64_t B, int Hk, int D, int64_t rows);
 int attn_tc(const AttnArgs& a, int dtype, int bits, int D, cudaStream_t s);
 
 }  // namespace kvq

@@ -1,0 +1,691 @@
+// Attention of prompts and longer drafts over a key/value cache of 4 or 8 bits, on the tcgen05 tensor cores.
+//
+// An item is 128 query rows of one key/value head (its query heads side by side, row = token * heads + head) and a range of tiles of
+// 128 positions. Persistent CTAs, one per SM, walk the items, longest first. 14 warps:
+//   warp 0      TMA producer: codes and scales of keys and of values, two stages of each.
+//   warp 1      MMA issuer: S(j) = Q K(j)^T into one of two 128-column buffers in tensor memory, Q from tensor memory;
+//               O += P(j) V(j) with P from tensor memory, over S. S(j + 2) is queued right behind P V(j).
+//   warps 2-5   softmax, a row a thread: loads Q and puts it into tensor memory; maxima, exponentials and sums in fp32, in the log2
+//               domain; O is rescaled only when a row's maximum grew by more than 2^8.
+//   warps 6-13  turn codes into fp16 tiles, 128-byte-swizzled rows that serve as the K-major keys and the MN-major values alike.
+// The products take fp16 operands. c * s is not exact in fp16 for every scale s, but c * s * 2^-e is, for the power of two that
+// brings a tile's largest scale near the top of the range, unless a scale is 2^28 times smaller than that one. Keys have an e of
+// their own in every tile (it joins the scores' factor), values one that O is rescaled for when a tile exceeds it. fp32 queries
+// enter as two fp16 terms (22 bits), and so do the probabilities of fp32 outputs; those of bfloat16 outputs as one.
+// With A from tensor memory the products read 64 bytes a clock of shared memory; with both operands there they would wait for it.
+// Every mbarrier wait is bounded.
+#include <climits>
+
+#include "kv_quant_attn.h"
+
+namespace ctdk {
+namespace kvq {
+namespace {
+
+constexpr int TQ = 128, KT = 128;
+constexpr int kChunk = 128 * 128;        // bytes of a {64 columns x 128 rows} tile
+constexpr float kSlack = 8.0f;
+// Probabilities (2^kSlack at most) are held times 2^kLift, sums alike: fp16's smallest step is then 2^-31 of the largest one.
+constexpr float kLift = 7.0f;
+constexpr int kThreads = 14 * 32, kMakers = 256;
+constexpr int kRing = 4;                 // tiles whose exponents and NaN marks are kept
+constexpr int kRoom = 6;                 // powers of two by which values may grow before O is rescaled
+
+template <int D, int BITS>
+struct Cfg {
+  static constexpr int kRow = D * BITS / 8, kGroups = D / kGroup, kChunks = D / 64;
+  static constexpr int kCodes = KT * kRow, kScales = KT * kGroups * 2;
+  static constexpr int kTile = kChunks * kChunk;                     // a converted tile
+  static constexpr int kSmem = 1024 + 4 * kTile + 4 * kCodes + 4 * kScales;
+  static constexpr int kTop = BITS == 4 ? 11 : 7;                    // the largest scale comes to [2^kTop, 2^(kTop + 1))
+};
+
+struct TcArgs {
+  AttnArgs a;
+  int rows, row_tiles, splits, items;    // T * group; of 128; ranges of an item's tiles; in all
+  uint32_t x64;                          // 0x64006400: fp16 1024
+};
+struct Item {
+  int b, h, r0, rows, ks, k0, k1;        // tiles k0 .. k1 - 1 of the visit
+  int64_t pos, count;
+  Visit v;
+};
+__device__ __forceinline__ Item item_at(const TcArgs& ta, int it) {
+  const AttnArgs& a = ta.a;
+  Item w;
+  const int ks = it % ta.splits, i = it / ta.splits, units = a.c.B * a.c.Hk, u = i % units, rt = ta.row_tiles - 1 - i / units;
+  w.ks = ks;
+  w.b = u / a.c.Hk;
+  w.h = u - w.b * a.c.Hk;
+  w.r0 = rt * TQ;
+  w.rows = min(TQ, ta.rows - w.r0);
+  w.pos = a.pos != nullptr ? static_cast<int64_t>(a.pos[w.b]) : a.pos_all;
+  w.count = a.count != nullptr ? min(static_cast<int64_t>(a.count[w.b]), static_cast<int64_t>(a.T)) : a.T;
+  const int t0 = w.r0 / a.group, t1 = (w.r0 + w.rows - 1) / a.group;
+  w.v = visit_of(w.pos, w.count, t0, t1 - t0 + 1, a.c.capacity, a.window, a.sinks, KT);
+  w.k0 = static_cast<int>(static_cast<int64_t>(w.v.tiles) * ks / ta.splits);
+  w.k1 = static_cast<int>(static_cast<int64_t>(w.v.tiles) * (ks + 1) / ta.splits);
+  return w;
+}
+
+__device__ __forceinline__ uint32_t idesc_f16(bool b_mn, int n) {
+  return (1u << 4) | (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(TQ >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ void unpack_f16(uint32_t w, float& lo, float& hi) {
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.f32.f16 %0, a;\n cvt.f32.f16 %1, b;\n}" : "=f"(lo), "=f"(hi) : "r"(w));
+}
+// The lowest n bits (n below 0: none; from 32 on: all).
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(max(-126, min(127, e)) + 127) << 23); }
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+               "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+__device__ __forceinline__ void bulk_in(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+template <typename QT>
+__device__ __forceinline__ void load8(const QT* p, float (&x)[8]);
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+template <>
+__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&x)[8]) {
+  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+__device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) { *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d); }
+__device__ __forceinline__ void store4(__nv_bfloat16* p, float a, float b, float c, float d) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(a, b), pack_bf16(c, d));
+}
+
+template <typename QT, int D, int BITS>
+__global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const TcArgs ta) {
+  using C = Cfg<D, BITS>;
+  constexpr int NT = sizeof(QT) == 4 ? 2 : 1;          // fp16 terms of a query, of a probability
+  constexpr uint32_t kColS = 0, kColO = 2 * KT, kColQ = 2 * KT + 128;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint64_t bars[24];
+  __shared__ uint32_t tmem_slot;
+  __shared__ uint32_t most[2][8];                      // warps' largest scales (bits), by parity of the tile
+  __shared__ int exp_k[kRing], exp_v[kRing], grow_v[kRing];   // exponents of a tile's keys and values; how far the latter has moved
+  __shared__ uint32_t nan_any[kRing];
+  __shared__ uint8_t nan_of[kRing][KT];                // groups of values that are NaN, by position
+  const AttnArgs& a = ta.a;
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  unsigned char* k_s = smem;                           // [2] converted tiles
+  unsigned char* v_s = k_s + 2 * C::kTile;
+  unsigned char* codes_s = v_s + 2 * C::kTile;         // [2][keys, values]
+  unsigned char* scales_s = codes_s + 4 * C::kCodes;   // [2][keys, values]
+  uint64_t* in_full = bars;          // [2][keys, values]: codes and scales are there
+  uint64_t* in_empty = bars + 4;     // [2][keys, values]: converted
+  uint64_t* k_full = bars + 8;       // [2] converted keys
+  uint64_t* k_empty = bars + 10;
+  uint64_t* v_full = bars + 12;
+  uint64_t* v_empty = bars + 14;
+  uint64_t* s_full = bars + 16;      // [2] S(g) is in tensor memory
+  uint64_t* p_ready = bars + 18;     // [2] P(g) has replaced S(g)
+  uint64_t* q_ready = bars + 20;     // Q of the item is in tensor memory, O of the one before has been read
+  uint64_t* pv_full = bars + 21;     // O += P(g) V(g) has finished (one phase per step)
+  uint64_t* o_full = bars + 22;      // the item's last one has
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_launch();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 23; ++i) mbar_init(&bars[i], i >= 4 && i < 8 ? 8 : i >= 8 && i < 10 ? 8 : i >= 12 && i < 14 ? 8 : i >= 18 && i < 21 ? 128 : 1);
+    mbar_fence_init();
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_slot;
+  pdl_wait();
+  // g = running count of tiles over all items of this CTA: stage g & 1, phase (g >> 1) & 1
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t g = 0;
+      bool ok = true;
+      for (int it = blockIdx.x; it < ta.items && ok; it += gridDim.x) {
+        const Item w = item_at(ta, it);
+        const int bh = w.b * a.c.Hk + w.h;
+        for (int k = w.k0; k < w.k1 && ok; ++k, ++g) {
+          const int st = g & 1u, j = w.v.tile_at(k) * KT;
+          const int there = static_cast<int>(min(static_cast<int64_t>(KT), a.c.capacity - j));   // positions that the cache has
+          const int64_t sc = (static_cast<int64_t>(bh) * a.c.capacity + j) * C::kGroups;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            ok = ok && mbar_wait_bounded(&in_empty[2 * st + i], ((g >> 1) & 1u) ^ 1u, a.status, 220 + i);
+            if (!ok) break;
+            uint64_t* bar = &in_full[2 * st + i];
+            mbar_expect_tx(bar, C::kCodes + there * C::kGroups * 2);
+            tma_load_3d(codes_s + (2 * st + i) * C::kCodes, i ? &tm_v : &tm_k, bar, 0, j, bh);
+            bulk_in(scales_s + (2 * st + i) * C::kScales, a.c.scales[i] + sc, there * C::kGroups * 2, bar);
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // The whole warp runs this role converged; one elected lane issues each MMA / commit.
+    const uint32_t idesc_s = idesc_f16(false, KT), idesc_pv = idesc_f16(true, D);
+    const uint32_t k_base = smem_u32(k_s), v_base = smem_u32(v_s);
+    uint32_t g0 = 0, n_it = 0;
+    bool ok = true;
+    for (int it = blockIdx.x; it < ta.items && ok; it += gridDim.x) {
+      const Item w = item_at(ta, it);
+      const int steps = w.k1 - w.k0;
+      if (steps <= 0) continue;
+      auto issue_s = [&](int j) {
+        const uint32_t g = g0 + static_cast<uint32_t>(j), s = g & 1u;
+        if (!mbar_wait_bounded_w(&k_full[s], (g >> 1) & 1u, a.status, 222)) return false;
+        tc_fence_after();
+        const uint64_t kd = make_smem_desc(k_base + s * C::kTile, 16, 1024, kLayoutSw128);
+        const uint32_t ts = tmem_base + kColS + s * KT, tq = tmem_base + kColQ;
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks)
+            umma_bf16_ta_w(ts, tq + static_cast<uint32_t>(x * (D / 2) + ks * 8), kd + (((ks >> 2) * kChunk + (ks & 3) * 32) >> 4), idesc_s, x + ks != 0 ? 1u : 0u);
+        umma_commit_w(&k_empty[s]);
+        umma_commit_w(&s_full[s]);
+        return true;
+      };
+      if (!mbar_wait_bounded_w(q_ready, n_it & 1u, a.status, 223)) break;
+      ++n_it;
+      tc_fence_after();
+      ok = issue_s(0);
+      if (ok && steps > 1) ok = issue_s(1);
+      for (int j = 0; j < steps && ok; ++j) {
+        const uint32_t g = g0 + static_cast<uint32_t>(j), s = g & 1u, ph = (g >> 1) & 1u;
+        ok = mbar_wait_bounded_w(&v_full[s], ph, a.status, 224) && mbar_wait_bounded_w(&p_ready[s], ph, a.status, 225);
+        if (!ok) break;
+        tc_fence_after();
+        // B: 16 key rows (two 8-row swizzle groups, SBO) of every 64-column chunk of V (LBO)
+        const uint64_t vd = make_smem_desc(v_base + s * C::kTile, kChunk, 1024, kLayoutSw128);
+        const uint32_t ts = tmem_base + kColS + s * KT;
+#pragma unroll
+        for (int kb = 0; kb < KT / 16; ++kb)
+#pragma unroll
+          for (int x = 0; x < NT; ++x)
+            umma_bf16_ta_w(tmem_base + kColO, ts + static_cast<uint32_t>((kb >> 2) * 64 + x * 32 + (kb & 3) * 8), vd + ((kb * 2048) >> 4), idesc_pv,
+                           kb + x != 0 ? 1u : (j != 0 ? 1u : 0u));
+        umma_commit_w(&v_empty[s]);
+        umma_commit_w(pv_full);
+        if (j == steps - 1) umma_commit_w(o_full);
+        if (j + 2 < steps) ok = issue_s(j + 2);
+      }
+      g0 += static_cast<uint32_t>(steps);
+    }
+    __syncwarp();
+  } else if (warp < 6) {
+    const int quarter = warp & 3;                      // tensor-memory lanes of this warp
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t to = tmem_base + kColO + lane_off, tq = tmem_base + kColQ + lane_off;
+    uint32_t g0 = 0, n_done = 0;
+    bool ok = true;
+    for (int it = blockIdx.x; it < ta.items && ok; it += gridDim.x) {
+      const Item w = item_at(ta, it);
+      const int steps = w.k1 - w.k0, rr = quarter * 32 + lane, r = w.r0 + rr, t = r / a.group, hg = r - t * a.group;
+      const bool live = rr < w.rows;
+      const int at = live ? row_position(w.pos, w.count, t, a.c.capacity) : -1;
+      float m_ref = -INFINITY, l = 0.0f, o_scale = 0.0f;
+      uint32_t poison = 0;                             // groups of columns that have met a NaN
+      if (steps > 0) {
+        // Q: a power of two brings the row's largest value near 64; terms into tensor memory, in the order of the converted keys
+        const QT* src = static_cast<const QT*>(a.q) + w.b * a.batch_stride + static_cast<int64_t>(t) * a.row_stride + static_cast<int64_t>(w.h * a.group + hg) * D;
+        float big = 0.0f;
+        if (live)
+#pragma unroll 4
+          for (int i = 0; i < D; i += 8) {
+            float x[8];
+            load8(src + i, x);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) big = fmaxf(big, fabsf(x[c]));
+          }
+        const int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;              // 128: not finite
+        const int up = big == 0.0f || e == 128 ? 0 : max(min(6 - e, 126), -100);
+        const float f = a.scale_log2 < 0.0f ? -pow2(up) : pow2(up);
+        const float factor = fabsf(a.scale_log2) * pow2(-up);
+#pragma unroll 1
+        for (int i = 0; i < D; i += 32) {
+          uint32_t q16[NT][16];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float x[8] = {};
+            if (live) load8(src + i + 8 * k, x);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              // 4 bits: a word's codes come as pairs (c, c + 4); 8 bits: in order
+              float u = (BITS == 4 ? x[c] : x[2 * c]) * f, v = (BITS == 4 ? x[c + 4] : x[2 * c + 1]) * f;
+#pragma unroll
+              for (int y = 0; y < NT; ++y) {
+                q16[y][4 * k + c] = pack_f16(u, v);
+                if (y + 1 < NT) {
+                  float a0, a1;
+                  unpack_f16(q16[y][4 * k + c], a0, a1);
+                  u -= a0, v -= a1;
+                }
+              }
+            }
+          }
+#pragma unroll
+          for (int y = 0; y < NT; ++y) tmem_st_32x16(tq + static_cast<uint32_t>(y * (D / 2) + i / 2), q16[y]);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(q_ready);
+        for (int j = 0; j < steps && ok; ++j) {
+          const uint32_t g = g0 + static_cast<uint32_t>(j), s = g & 1u;
+          ok = mbar_wait_bounded_w(&s_full[s], (g >> 1) & 1u, a.status, 230);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t ts = tmem_base + kColS + s * KT + lane_off;
+          const int j0 = w.v.tile_at(w.k0 + j) * KT;
+          const bool plain = j0 + KT - 1 <= w.v.lo_row && (a.window == 0 || w.v.hi_row - 1 - j0 < a.window || j0 + KT <= a.sinks);
+          const float sc = fmaxf(factor * pow2(exp_k[g % kRing]), 0x1p-126f);
+          float x[64], mx = -INFINITY;
+          // which of a half's positions the row sees, as bits: up to its own, from the window's first on or below the sinks
+          auto masked = [&](int hf) {
+            const int base = j0 + 64 * hf, last = at - base, first = a.window == 0 ? 0 : at - a.window + 1 - base, sink = a.sinks - base;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const uint32_t upto = below(last + 1 - 32 * q), from = ~below(first - 32 * q), sk = a.window == 0 ? 0u : below(sink - 32 * q);
+              const uint32_t bits = upto & (from | sk);
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if ((bits >> i & 1u) == 0) x[32 * q + i] = -INFINITY;
+            }
+          };
+#pragma unroll
+          for (int hf = 1; hf >= 0; --hf) {            // the second half first: the first one stays for the exponentials
+            tmem_ld_32x64_nowait(ts + 64 * hf, x);
+            tmem_wait_ld();
+            if (!plain) masked(hf);
+            float m0 = mx, m1 = x[0];
+#pragma unroll
+            for (int i = 1; i + 3 < 64; i += 4) {
+              m0 = fmax3(m0, x[i], x[i + 1]);
+              m1 = fmax3(m1, x[i + 2], x[i + 3]);
+            }
+            mx = fmax3(fmax3(m0, m1, x[61]), x[62], x[63]);
+          }
+          const float mxs = mx * sc;
+          const int dv = grow_v[g % kRing];
+          float c = 1.0f;
+          bool grow = dv != 0;
+          if (mxs > m_ref + kSlack) {
+            c = ex2(m_ref - mxs);
+            m_ref = mxs;
+            grow = true;
+          }
+          if (__any_sync(0xffffffffu, grow)) {
+            if (j != 0) {
+              // P V(g-1) must have landed before the accumulator is touched; P V(g) cannot start before every
+              // row has arrived at p_ready below
+              ok = mbar_wait_bounded_w(pv_full, (g - 1u) & 1u, a.status, 231);
+              if (!ok) break;
+              tc_fence_after();
+              const float co = c * pow2(-dv);
+#pragma unroll 1
+              for (int p = 0; p < D / 32; ++p) {
+                float o[32];
+                tmem_ld_32x32(to + p * 32, o);
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) fmul2(o[i], o[i + 1], o[i], o[i + 1], co, co);
+                tmem_st_32x32(to + p * 32, *reinterpret_cast<uint32_t(*)[32]>(o));
+                tmem_wait_st();
+              }
+            }
+            l *= c;
+          }
+          const float neg_m = (m_ref == -INFINITY ? 0.0f : -m_ref) + kLift;
+          float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            if (hf == 1) {
+              tmem_ld_32x64_nowait(ts + 64, x);
+              tmem_wait_ld();
+              if (!plain) masked(1);
+            }
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t p16[NT][16];
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                float u, v;
+                ffma2(u, v, x[32 * q + i], x[32 * q + i + 1], sc, sc, neg_m, neg_m);
+                u = ex2(u);
+                v = ex2(v);
+                fadd2(s0, s1, s0, s1, u, v);
+#pragma unroll
+                for (int y = 0; y < NT; ++y) {
+                  p16[y][i >> 1] = pack_f16(u, v);
+                  if (y + 1 < NT) {
+                    float a0, a1;
+                    unpack_f16(p16[y][i >> 1], a0, a1);
+                    u -= a0, v -= a1;
+                  }
+                }
+              }
+#pragma unroll
+              for (int y = 0; y < NT; ++y) tmem_st_32x16(ts + 64 * hf + 32 * y + 16 * q, p16[y]);
+            }
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          if (nan_any[g % kRing] != 0)                 // NaN values: zeros in the tile; the rows that see them get NaN
+            for (int i = 0; i < KT; ++i)
+              if (nan_of[g % kRing][i] != 0 && sees(at, j0 + i, a.window, a.sinks)) poison |= nan_of[g % kRing][i];
+          if (j == steps - 1) o_scale = pow2(exp_v[g % kRing]);
+          mbar_arrive(&p_ready[s]);
+          l += s0 + s1;
+        }
+        g0 += static_cast<uint32_t>(steps);
+        // The item's last P V. The next item's first one cannot start before these threads have read O and arrived at q_ready.
+        ok = ok && mbar_wait_bounded_w(o_full, n_done & 1u, a.status, 232);
+        if (!ok) break;
+        ++n_done;
+        tc_fence_after();
+      }
+      float* part = ta.splits > 1 ? a.part + static_cast<int64_t>(it) * TQ * (D + 2) : nullptr;
+      const float f = part != nullptr ? o_scale : (at >= 0 ? o_scale / l : 0.0f);
+      QT* dst = static_cast<QT*>(a.out) + ((static_cast<int64_t>(w.b) * a.T + t) * a.H + w.h * a.group + hg) * D;
+#pragma unroll 1
+      for (int p = 0; p < D / 32; ++p) {
+        float o[32];
+        if (steps > 0) {
+          tmem_ld_32x32(to + p * 32, o);               // warp-collective: rows past the end take part too
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = (poison >> p & 1u) != 0 ? __int_as_float(0x7fc00000) : o[i] * f;
+        if (part == nullptr && at < 0)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          // columns as they came: pairs (c, c + 4) of eight, or in order
+          const float y[8] = {o[i], BITS == 4 ? o[i + 2] : o[i + 1], BITS == 4 ? o[i + 4] : o[i + 2], BITS == 4 ? o[i + 6] : o[i + 3],
+                              BITS == 4 ? o[i + 1] : o[i + 4], BITS == 4 ? o[i + 3] : o[i + 5], BITS == 4 ? o[i + 5] : o[i + 6], o[i + 7]};
+          if (part != nullptr) {
+            store4(part + rr * D + 32 * p + i, y[0], y[1], y[2], y[3]);
+            store4(part + rr * D + 32 * p + i + 4, y[4], y[5], y[6], y[7]);
+          } else if (live) {
+            store4(dst + 32 * p + i, y[0], y[1], y[2], y[3]);
+            store4(dst + 32 * p + i + 4, y[4], y[5], y[6], y[7]);
+          }
+        }
+        __syncwarp();
+      }
+      if (part != nullptr) {
+        part[TQ * D + rr] = m_ref - kLift;
+        part[TQ * D + TQ + rr] = l;
+      }
+      tc_fence_before();
+    }
+  } else {
+    const int mt = static_cast<int>(threadIdx.x) - 6 * 32, mw = mt >> 5;               // of the 256 that convert
+    uint32_t g0 = 0;
+    bool ok = true, go = true;                         // of this warp; of all of them
+    for (int it = blockIdx.x; it < ta.items && go; it += gridDim.x) {
+      const Item w = item_at(ta, it);
+      const int steps = w.k1 - w.k0;
+      int vref = 0;
+      // Exponents of tile j's keys and values, and its NaN values: thread i reads a position's scales of one of them. False: over.
+      auto survey = [&](int j) {
+        const uint32_t g = g0 + static_cast<uint32_t>(j), st = g & 1u, which = static_cast<uint32_t>(mt) >> 7;
+        const int row = mt & 127, at = w.v.tile_at(w.k0 + j) * KT + row;
+        ok = ok && mbar_wait_bounded_w(&in_full[2 * st + which], (g >> 1) & 1u, a.status, 240);
+        // seen by one of the rows: what else lies in the tile must not matter
+        const bool seen = at < w.v.hi_row && (at >= w.v.lo_row || a.window == 0 || w.v.lo_row - at < a.window || at < a.sinks);
+        const unsigned char* p = scales_s + (2 * st + which) * C::kScales + row * C::kGroups * 2;
+        uint32_t sw[C::kGroups / 2], big = 0, nan = 0;
+#pragma unroll
+        for (int i = 0; i < C::kGroups / 2; ++i) sw[i] = *reinterpret_cast<const uint32_t*>(p + 4 * i);
+#pragma unroll
+        for (int i = 0; i < C::kGroups; ++i) {
+          const uint32_t b = (i & 1 ? sw[i / 2] >> 16 : sw[i / 2]) & 0x7fffu;
+          if (is_nan_scale(b)) nan |= 1u << i;
+          else big = max(big, b);
+        }
+        if (!seen) big = nan = 0;
+        big = __reduce_max_sync(0xffffffffu, big);
+        if (which == 1) nan_of[g % kRing][row] = static_cast<uint8_t>(nan);
+        const bool any = __any_sync(0xffffffffu, nan != 0 && which == 1);
+        if (lane == 0) most[g & 1u][mw] = big | (any ? 0x80000000u : 0u);
+        // These warps give up together: a barrier that one of them never reached would hold the others for good.
+        int all_ok;
+        asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.pred q, 1, 256, p;\n selp.b32 %0, 1, 0, q;\n}"
+                     : "=r"(all_ok) : "r"(static_cast<int>(ok)) : "memory");
+        if (all_ok == 0) return false;
+        uint32_t bk = 0, bv = 0, flag = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          bk = max(bk, most[g & 1u][i]);
+          bv = max(bv, most[g & 1u][4 + i] & 0x7fffffffu);
+          flag |= most[g & 1u][4 + i] >> 31;
+        }
+        const int ek = bk == 0 ? 0 : max(static_cast<int>(bk >> 7) - 127 - C::kTop, -120);
+        const int ev = bv == 0 ? -120 : max(static_cast<int>(bv >> 7) - 127 - C::kTop, -120);
+        int moved = 0;
+        if (j == 0) {
+          vref = ev + kRoom;
+        } else if (ev > vref) {
+          moved = ev + kRoom - vref;
+          vref += moved;
+        }
+        if (mt == 0) {
+          exp_k[g % kRing] = ek;
+          exp_v[g % kRing] = vref;
+          grow_v[g % kRing] = moved;
+          nan_any[g % kRing] = flag;
+        }
+        return true;
+      };
+      // Tile j of keys (which 0) or values: a thread takes 16 bytes of codes at a time, neighbouring lanes neighbouring positions.
+      auto convert = [&](int j, int which, int ex) {
+        const uint32_t g = g0 + static_cast<uint32_t>(j), st = g & 1u;
+        const int j0 = w.v.tile_at(w.k0 + j) * KT;
+        const uint32_t src = smem_u32(codes_s) + (2 * st + which) * C::kCodes;
+        const unsigned char* scale = scales_s + (2 * st + which) * C::kScales;
+        const uint32_t dst = smem_u32(which ? v_s : k_s) + st * C::kTile;
+        const float up = pow2(-ex);
+        constexpr int kUnits = C::kRow / 16;           // of a position
+#pragma unroll 2
+        for (int i = mt; i < KT * kUnits; i += kMakers) {
+          const int row = i & 127, unit = i >> 7, at = j0 + row;
+          const uint32_t off = static_cast<uint32_t>(row * C::kRow + unit * 16);
+          uint32_t wd[4];
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(wd[0]), "=r"(wd[1]), "=r"(wd[2]), "=r"(wd[3])
+                       : "r"(src + (off ^ ((off >> 3) & (C::kRow - 16u)))));
+          const uint32_t sb = *reinterpret_cast<const uint16_t*>(scale + (row * C::kGroups + (BITS == 4 ? unit : unit / 2)) * 2);
+          float sf = __uint_as_float(sb << 16) * up;
+          const bool seen = at < w.v.hi_row && (at >= w.v.lo_row || a.window == 0 || w.v.lo_row - at < a.window || at < a.sinks);
+          if (is_nan_scale(sb)) sf = which ? 0.0f : __int_as_float(0x7fc00000);
+          if (!seen) sf = 0.0f;
+          const uint32_t s2 = pack_f16(sf, sf);
+          if constexpr (BITS == 4) {
+            const uint32_t base = dst + static_cast<uint32_t>(unit >> 1) * kChunk + static_cast<uint32_t>(row) * 128u;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {              // a word: eight columns
+              const uint32_t v = wd[k] >> 8;
+              uint32_t y[4];
+              y[0] = add_f16x2((wd[k] & 0x000f000fu) | ta.x64, 0xe408e408u);               // 1024 + u - 1032
+              y[1] = fma_f16x2((wd[k] & 0x00f000f0u) | ta.x64, 0x2c002c00u, 0xd480d480u);  // (1024 + 16 u) / 16 - 72
+              y[2] = add_f16x2((v & 0x000f000fu) | ta.x64, 0xe408e408u);
+              y[3] = fma_f16x2((v & 0x00f000f0u) | ta.x64, 0x2c002c00u, 0xd480d480u);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) y[c] = mul_f16x2(y[c], s2);
+              sts128(base + (static_cast<uint32_t>(((unit & 1) * 4 + k) ^ (row & 7)) << 4), y[0], y[1], y[2], y[3]);
+            }
+          } else {
+            const uint32_t base = dst + static_cast<uint32_t>(unit >> 2) * kChunk + static_cast<uint32_t>(row) * 128u;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {              // two words: eight columns
+              uint32_t y[4];
+              y[0] = add_f16x2(prmt(wd[2 * k], ta.x64, 0x5150), 0xe480e480u);              // 1024 + u - 1152
+              y[1] = add_f16x2(prmt(wd[2 * k], ta.x64, 0x5352), 0xe480e480u);
+              y[2] = add_f16x2(prmt(wd[2 * k + 1], ta.x64, 0x5150), 0xe480e480u);
+              y[3] = add_f16x2(prmt(wd[2 * k + 1], ta.x64, 0x5352), 0xe480e480u);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) y[c] = mul_f16x2(y[c], s2);
+              sts128(base + (static_cast<uint32_t>(((unit & 3) * 2 + k) ^ (row & 7)) << 4), y[0], y[1], y[2], y[3]);
+            }
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(which ? &v_full[st] : &k_full[st]);
+          mbar_arrive(&in_empty[2 * st + which]);
+        }
+      };
+      int ev[2] = {0, 0};                              // exponents of the values of tiles j, j + 1
+      auto keys = [&](int j) {
+        const uint32_t g = g0 + static_cast<uint32_t>(j);
+        ok = ok && mbar_wait_bounded_w(&in_full[2 * (g & 1u)], (g >> 1) & 1u, a.status, 241);
+        if (!survey(j)) return false;
+        ev[j & 1] = vref;
+        ok = mbar_wait_bounded_w(&k_empty[g & 1u], ((g >> 1) & 1u) ^ 1u, a.status, 242);
+        uint32_t bk = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bk = max(bk, most[g & 1u][i]);
+        if (ok) convert(j, 0, bk == 0 ? 0 : max(static_cast<int>(bk >> 7) - 127 - C::kTop, -120));
+        return true;
+      };
+      go = steps <= 0 || keys(0);
+      for (int j = 0; j < steps && go; ++j) {          // keys run one tile ahead of values
+        const uint32_t g = g0 + static_cast<uint32_t>(j);
+        if (j + 1 < steps) go = keys(j + 1);
+        ok = ok && mbar_wait_bounded_w(&in_full[2 * (g & 1u) + 1], (g >> 1) & 1u, a.status, 243) &&
+             mbar_wait_bounded_w(&v_empty[g & 1u], ((g >> 1) & 1u) ^ 1u, a.status, 244);
+        if (ok && go) convert(j, 1, ev[j & 1]);
+      }
+      g0 += static_cast<uint32_t>(steps > 0 ? steps : 0);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// Joins the ranges of the items: a CTA takes 16 rows of one, a thread a column (or two rows' columns).
+template <typename QT, int D>
+__global__ void __launch_bounds__(256) kvq_prompt_join_kernel(const TcArgs ta) {
+  const AttnArgs& a = ta.a;
+  pdl_launch();
+  pdl_wait();
+  const int i = blockIdx.x / (TQ / 16), units = a.c.B * a.c.Hk, u = i % units, rt = ta.row_tiles - 1 - i / units;
+  const int b = u / a.c.Hk, h = u - b * a.c.Hk;
+  const float* part = a.part + static_cast<int64_t>(i) * ta.splits * TQ * (D + 2);
+  const int64_t pos = a.pos != nullptr ? static_cast<int64_t>(a.pos[b]) : a.pos_all;
+  const int64_t count = a.count != nullptr ? min(static_cast<int64_t>(a.count[b]), static_cast<int64_t>(a.T)) : a.T;
+  for (int e = threadIdx.x; e < 16 * D; e += 256) {
+    const int rr = static_cast<int>(blockIdx.x % (TQ / 16)) * 16 + e / D, d = e % D, r = rt * TQ + rr;
+    if (r >= ta.rows) continue;
+    float m = -INFINITY;
+#pragma unroll 8
+    for (int k = 0; k < ta.splits; ++k) m = fmaxf(m, part[static_cast<int64_t>(k) * TQ * (D + 2) + TQ * D + rr]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, s = 0.0f;
+#pragma unroll 8
+    for (int k = 0; k < ta.splits; ++k) {
+      const float* p = part + static_cast<int64_t>(k) * TQ * (D + 2);
+      const float w = ex2(p[TQ * D + rr] - ref);
+      l += w * p[TQ * D + TQ + rr];
+      s += w * p[rr * D + d];
+    }
+    const int t = r / a.group, hg = r - t * a.group;
+    const float x = row_position(pos, count, t, a.c.capacity) >= 0 ? s / l : 0.0f;
+    QT* out = static_cast<QT*>(a.out) + ((static_cast<int64_t>(b) * a.T + t) * a.H + h * a.group + hg) * D + d;
+    if constexpr (sizeof(QT) == 4) *out = x;
+    else *out = __float2bfloat16_rn(x);
+  }
+}
+
+template <typename QT, int D, int BITS>
+int launch(const TcArgs& ta, cudaStream_t s) {
+  using C = Cfg<D, BITS>;
+  CUtensorMap m[2];
+  const Cache& c = ta.a.c;
+  const uint64_t dims[3] = {C::kRow, static_cast<uint64_t>(c.capacity), static_cast<uint64_t>(c.B) * c.Hk};
+  const uint64_t strides[2] = {C::kRow, static_cast<uint64_t>(c.capacity) * C::kRow};
+  const uint32_t box[3] = {C::kRow, KT, 1};
+  for (int i = 0; i < 2; ++i)
+    if (const int rc = encode_tensor_map_u8(&m[i], c.codes[i], 3, dims, strides, box); rc != CTDK_OK) return rc;
+  auto* kernel = kvq_prompt_kernel<QT, D, BITS>;
+  const int ctas = ta.items < sm_count() ? ta.items : sm_count();
+  cudaError_t e = raise_dynamic_smem(reinterpret_cast<const void*>(kernel), C::kSmem);
+  if (e == cudaSuccess) e = launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), C::kSmem, s, m[0], m[1], ta);
+  if (e != cudaSuccess) return fail(CTDK_ELAUNCH, "kvq_attn: %s", cudaGetErrorString(e));
+  if (const int rc = check_launch("kvq_attn"); rc != CTDK_OK || ta.splits == 1) return rc;
+  e = launch_pdl(kvq_prompt_join_kernel<QT, D>, dim3(static_cast<unsigned>(ta.items / ta.splits * (TQ / 16))), dim3(256), 0, s, ta);
+  if (e != cudaSuccess) return fail(CTDK_ELAUNCH, "kvq_attn: %s", cudaGetErrorString(e));
+  return check_launch("kvq_attn");
+}
+
+// Ranges of an item's tiles: as many as fill the SMs, where there are fewer items; a range has four tiles at least.
+int splits_of(int64_t items, int64_t tiles) {
+  const int64_t want = sm_count() / items, most = tiles / 4;
+  const int64_t n = want < most ? want : most;
+  return n < 1 ? 1 : static_cast<int>(n);
+}
+int64_t row_items(int64_t B, int Hk, int64_t rows) { return B * Hk * ((rows + TQ - 1) / TQ); }
+
+}  // namespace
+
+int64_t attn_tc_bytes(int64_t B, int Hk, int D, int64_t rows) {
+  const int64_t items = row_items(B, Hk, rows), splits = splits_of(items, INT32_MAX);
+  return splits > 1 ? items * splits * TQ * (D + 2) * 4 : 0;
+}
+
+int attn_tc(const AttnArgs& a, int dtype, int bits, int D, cudaStream_t s) {
+  TcArgs ta;
+  ta.a = a;
+  const int64_t rows = static_cast<int64_t>(a.T) * a.group, items = row_items(a.c.B, a.c.Hk, rows);
+  int64_t tiles = (a.c.capacity + KT - 1) / KT;        // the most that an item can have
+  if (a.pos == nullptr) tiles = (a.pos_all + a.T + KT - 1) / KT;
+  if (a.window > 0) tiles = min(tiles, (static_cast<int64_t>(a.window) + a.T + a.sinks) / KT + 3);
+  ta.rows = static_cast<int>(rows);
+  ta.row_tiles = static_cast<int>((rows + TQ - 1) / TQ);
+  ta.splits = splits_of(items, tiles);
+  CTDK_REQUIRE(rows <= INT32_MAX / 2 && items * ta.splits <= INT32_MAX / 16, "kvq_attn: too many rows");
+  ta.items = static_cast<int>(items * ta.splits);
+  ta.x64 = 0x64006400u;
+  const bool f32 = dtype == CTDK_DTYPE_F32;
+  if (bits == 4) {
+    if (D == 64) return f32 ? launch<float, 64, 4>(ta, s) : launch<__nv_bfloat16, 64, 4>(ta, s);
+    return f32 ? launch<float, 128, 4>(ta, s) : launch<__nv_bfloat16, 128, 4>(ta, s);
+  }
+  if (D == 64) return f32 ? launch<float, 64, 8>(ta, s) : launch<__nv_bfloat16, 64, 8>(ta, s);
+  return f32 ? launch<float, 128, 8>(ta, s) : launch<__nv_bfloat16, 128, 8>(ta, s);
+}
+
+}  // namespace kvq
+}  // namespace ctdk

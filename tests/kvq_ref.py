@@ -49,7 +49,8 @@ def attention(q, k, v, pos, count, window=0, sinks=0, scale=None, split_q=True, 
     the sum) and by 8u of its size in the log2 domain's arithmetic; twice that moves the weights (numerator and
     denominator); a probability is off by 2^-16 (two terms, half a step of 2^-8 each) or 2^-8 (one), its exponential by 2^-21; sums over n positions go
     in steps of 16, off by 2u each, and through at most 64 joins; what is below 2^-126
-    (before it meets a value) may be zero; the result is rounded to its type."""
+    (before it meets a value) may be zero, and fp16 probabilities, held times 2^7 relative to a maximum that is at most the
+    row's (so that the sum is 1 or more), are off by half of fp16's smallest step: 2^-25 / 2^7; the result is rounded to its type."""
     T, H, D = q.shape
     Hk, n, _ = k.shape
     u = 2.0 ** -24
@@ -70,5 +71,5 @@ def attention(q, k, v, pos, count, window=0, sinks=0, scale=None, split_q=True, 
             m = len(z)
             off = (size * ((2.0 ** -16 if split_q else 0.0) + 2 * D * u) + 8 * u * (np.abs(z) + np.abs(z).max())).max()
             rel = np.expm1(2 * off) + (2.0 ** -16 if split_q else 2.0 ** -8) + 2.0 ** -21 + 2 * u * (m / 16 + 64)
-            tol[t, h] = (1 + 2.0 ** -out_bits) * rel * (w @ np.abs(vv)) + 2.0 ** -out_bits * np.abs(out[t, h]) + 2.0 ** -126 * np.abs(vv).sum(0)
+            tol[t, h] = (1 + 2.0 ** -out_bits) * rel * (w @ np.abs(vv)) + 2.0 ** -out_bits * np.abs(out[t, h]) + (2.0 ** -126 + 2.0 ** -32) * np.abs(vv).sum(0)
     return out, tol
