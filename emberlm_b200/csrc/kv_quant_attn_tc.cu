@@ -27,7 +27,7 @@ constexpr int kChunk = 128 * 128;        // bytes of a {64 columns x 128 rows} t
 constexpr float kSlack = 8.0f;
 // Probabilities (2^kSlack at most) are held times 2^kLift, sums alike: fp16's smallest step is then 2^-31 of the largest one.
 constexpr float kLift = 7.0f;
-constexpr int kThreads = 14 * 32, kMakers = 256;
+constexpr int kThreads = 14 * 32;
 constexpr int kRing = 4;                 // tiles whose exponents and NaN marks are kept
 constexpr int kRoom = 6;                 // powers of two by which values may grow before O is rescaled
 
@@ -304,31 +304,42 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
           const int j0 = w.v.tile_at(w.k0 + j) * KT;
           const bool plain = j0 + KT - 1 <= w.v.lo_row && (a.window == 0 || w.v.hi_row - 1 - j0 < a.window || j0 + KT <= a.sinks);
           const float sc = fmaxf(factor * pow2(exp_k[g % kRing]), 0x1p-126f);
-          float x[64], mx = -INFINITY;
-          // which of a half's positions the row sees, as bits: up to its own, from the window's first on or below the sinks
-          auto masked = [&](int hf) {
-            const int base = j0 + 64 * hf, last = at - base, first = a.window == 0 ? 0 : at - a.window + 1 - base, sink = a.sinks - base;
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const uint32_t upto = below(last + 1 - 32 * q), from = ~below(first - 32 * q), sk = a.window == 0 ? 0u : below(sink - 32 * q);
-              const uint32_t bits = upto & (from | sk);
+          if (!plain) {
+            // Scores that the row does not see become minus infinity where they lie, so that the code below, which has to
+            // stay in the instruction cache beside the other roles', has one form. Which of 32 positions it sees, as bits: up
+            // to its own, from the window's first on or below the sinks.
+#pragma unroll 1
+            for (int q = 0; q < KT / 32; ++q) {
+              const int base = j0 + 32 * q;
+              const uint32_t from = a.window == 0 ? 0xffffffffu : ~below(at - a.window + 1 - base) | below(a.sinks - base);
+              const uint32_t bits = below(at + 1 - base) & from;
+              if (__all_sync(0xffffffffu, bits == 0xffffffffu)) continue;
+              float x[32];
+              tmem_ld_32x32(ts + 32 * q, x);
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if ((bits >> i & 1u) == 0) x[32 * q + i] = -INFINITY;
+                if ((bits >> i & 1u) == 0) x[i] = -INFINITY;
+              tmem_st_32x32(ts + 32 * q, *reinterpret_cast<uint32_t(*)[32]>(x));
             }
-          };
-#pragma unroll
-          for (int hf = 1; hf >= 0; --hf) {            // the second half first: the first one stays for the exponentials
+            tmem_wait_st();
+          }
+          float mx = -INFINITY;
+#pragma unroll 1
+          for (int hf = 0; hf < 2; ++hf) {
+            float x[64];
             tmem_ld_32x64_nowait(ts + 64 * hf, x);
             tmem_wait_ld();
-            if (!plain) masked(hf);
-            float m0 = mx, m1 = x[0];
+            float m0 = mx, m1 = x[0], m2 = x[1], m3 = x[2];
 #pragma unroll
-            for (int i = 1; i + 3 < 64; i += 4) {
+            for (int i = 3; i + 7 < 64; i += 8) {
               m0 = fmax3(m0, x[i], x[i + 1]);
               m1 = fmax3(m1, x[i + 2], x[i + 3]);
+              m2 = fmax3(m2, x[i + 4], x[i + 5]);
+              m3 = fmax3(m3, x[i + 6], x[i + 7]);
             }
-            mx = fmax3(fmax3(m0, m1, x[61]), x[62], x[63]);
+            m0 = fmax3(m0, x[59], x[60]);
+            m1 = fmax3(m1, x[61], x[62]);
+            mx = fmaxf(fmax3(m0, m1, m2), fmaxf(m3, x[63]));
           }
           const float mxs = mx * sc;
           const int dv = grow_v[g % kRing];
@@ -361,13 +372,11 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
           }
           const float neg_m = (m_ref == -INFINITY ? 0.0f : -m_ref) + kLift;
           float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll
+#pragma unroll 1
           for (int hf = 0; hf < 2; ++hf) {
-            if (hf == 1) {
-              tmem_ld_32x64_nowait(ts + 64, x);
-              tmem_wait_ld();
-              if (!plain) masked(1);
-            }
+            float x[64];
+            tmem_ld_32x64_nowait(ts + 64 * hf, x);
+            tmem_wait_ld();
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
               uint32_t p16[NT][16];
@@ -395,6 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
           tmem_wait_st();
           tc_fence_before();
           if (nan_any[g % kRing] != 0)                 // NaN values: zeros in the tile; the rows that see them get NaN
+#pragma unroll 1
             for (int i = 0; i < KT; ++i)
               if (nan_of[g % kRing][i] != 0 && sees(at, j0 + i, a.window, a.sinks)) poison |= nan_of[g % kRing][i];
           if (j == steps - 1) o_scale = pow2(exp_v[g % kRing]);
@@ -448,6 +458,13 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
     }
   } else {
     const int mt = static_cast<int>(threadIdx.x) - 6 * 32, mw = mt >> 5;               // of the 256 that convert
+    // A thread's position in every tile; where its first 16 bytes of codes lie, as TMA has swizzled them; where its columns go.
+    const int row = mt & 127, half = mt >> 7;
+    const uint32_t row_at = static_cast<uint32_t>(row * C::kRow);
+    const uint32_t src_row = row_at + ((16u * half) ^ ((row_at >> 3) & (C::kRow - 16u)));
+    uint32_t dst_at[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) dst_at[k] = static_cast<uint32_t>(row) * 128u + ((static_cast<uint32_t>(half * (BITS == 4 ? 4 : 2) + k) ^ (row & 7u)) << 4);
     uint32_t g0 = 0;
     bool ok = true, go = true;                         // of this warp; of all of them
     for (int it = blockIdx.x; it < ta.items && go; it += gridDim.x) {
@@ -455,9 +472,9 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
       const int steps = w.k1 - w.k0;
       int vref = 0;
       // Exponents of tile j's keys and values, and its NaN values: thread i reads a position's scales of one of them. False: over.
-      auto survey = [&](int j) {
-        const uint32_t g = g0 + static_cast<uint32_t>(j), st = g & 1u, which = static_cast<uint32_t>(mt) >> 7;
-        const int row = mt & 127, at = w.v.tile_at(w.k0 + j) * KT + row;
+      auto survey = [&](int j, int& ek) {
+        const uint32_t g = g0 + static_cast<uint32_t>(j), st = g & 1u, which = static_cast<uint32_t>(half);
+        const int at = w.v.tile_at(w.k0 + j) * KT + row;
         ok = ok && mbar_wait_bounded_w(&in_full[2 * st + which], (g >> 1) & 1u, a.status, 240);
         // seen by one of the rows: what else lies in the tile must not matter
         const bool seen = at < w.v.hi_row && (at >= w.v.lo_row || a.window == 0 || w.v.lo_row - at < a.window || at < a.sinks);
@@ -488,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
           bv = max(bv, most[g & 1u][4 + i] & 0x7fffffffu);
           flag |= most[g & 1u][4 + i] >> 31;
         }
-        const int ek = bk == 0 ? 0 : max(static_cast<int>(bk >> 7) - 127 - C::kTop, -120);
+        ek = bk == 0 ? 0 : max(static_cast<int>(bk >> 7) - 127 - C::kTop, -120);
         const int ev = bv == 0 ? -120 : max(static_cast<int>(bv >> 7) - 127 - C::kTop, -120);
         int moved = 0;
         if (j == 0) {
@@ -505,30 +522,32 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
         }
         return true;
       };
-      // Tile j of keys (which 0) or values: a thread takes 16 bytes of codes at a time, neighbouring lanes neighbouring positions.
+      // Tile j of keys (which 0) or values. A thread has one position and every second 16 bytes of its codes: neighbouring lanes
+      // neighbouring positions, whose swizzles keep the reads and the writes off each other's banks.
       auto convert = [&](int j, int which, int ex) {
         const uint32_t g = g0 + static_cast<uint32_t>(j), st = g & 1u;
-        const int j0 = w.v.tile_at(w.k0 + j) * KT;
-        const uint32_t src = smem_u32(codes_s) + (2 * st + which) * C::kCodes;
-        const unsigned char* scale = scales_s + (2 * st + which) * C::kScales;
+        const int at = w.v.tile_at(w.k0 + j) * KT + row;
+        const uint32_t src = smem_u32(codes_s) + (2 * st + which) * C::kCodes + src_row;
         const uint32_t dst = smem_u32(which ? v_s : k_s) + st * C::kTile;
-        const float up = pow2(-ex);
-        constexpr int kUnits = C::kRow / 16;           // of a position
-#pragma unroll 2
-        for (int i = mt; i < KT * kUnits; i += kMakers) {
-          const int row = i & 127, unit = i >> 7, at = j0 + row;
-          const uint32_t off = static_cast<uint32_t>(row * C::kRow + unit * 16);
+        const uint32_t scale = smem_u32(scales_s) + (2 * st + which) * C::kScales + static_cast<uint32_t>(row * C::kGroups * 2);
+        const bool seen = at < w.v.hi_row && (at >= w.v.lo_row || a.window == 0 || w.v.lo_row - at < a.window || at < a.sinks);
+        const float up = seen ? pow2(-ex) : 0.0f;
+        uint32_t sw[C::kGroups / 2];
+        if constexpr (C::kGroups == 4) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(sw[0]), "=r"(sw[1]) : "r"(scale));
+        else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sw[0]) : "r"(scale));
+#pragma unroll
+        for (int kk = 0; kk < C::kRow / 32; ++kk) {
           uint32_t wd[4];
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(wd[0]), "=r"(wd[1]), "=r"(wd[2]), "=r"(wd[3])
-                       : "r"(src + (off ^ ((off >> 3) & (C::kRow - 16u)))));
-          const uint32_t sb = *reinterpret_cast<const uint16_t*>(scale + (row * C::kGroups + (BITS == 4 ? unit : unit / 2)) * 2);
-          float sf = __uint_as_float(sb << 16) * up;
-          const bool seen = at < w.v.hi_row && (at >= w.v.lo_row || a.window == 0 || w.v.lo_row - at < a.window || at < a.sinks);
-          if (is_nan_scale(sb)) sf = which ? 0.0f : __int_as_float(0x7fc00000);
-          if (!seen) sf = 0.0f;
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(wd[0]), "=r"(wd[1]), "=r"(wd[2]), "=r"(wd[3]) : "r"(src ^ (32u * kk)));
+          // 4 bits: 16 bytes are a group; 8 bits: half of one
+          uint32_t sb = sw[BITS == 4 ? kk : kk / 2];
+          if constexpr (BITS == 4) sb = half ? sb >> 16 : sb & 0xffffu;
+          else sb = kk & 1 ? sb >> 16 : sb & 0xffffu;
+          float sf = __uint_as_float(sb << 16);
+          if (is_nan_scale(sb)) sf = which || !seen ? 0.0f : __int_as_float(0x7fc00000);
+          sf *= up;
           const uint32_t s2 = pack_f16(sf, sf);
           if constexpr (BITS == 4) {
-            const uint32_t base = dst + static_cast<uint32_t>(unit >> 1) * kChunk + static_cast<uint32_t>(row) * 128u;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {              // a word: eight columns
               const uint32_t v = wd[k] >> 8;
@@ -539,10 +558,9 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
               y[3] = fma_f16x2((v & 0x00f000f0u) | ta.x64, 0x2c002c00u, 0xd480d480u);
 #pragma unroll
               for (int c = 0; c < 4; ++c) y[c] = mul_f16x2(y[c], s2);
-              sts128(base + (static_cast<uint32_t>(((unit & 1) * 4 + k) ^ (row & 7)) << 4), y[0], y[1], y[2], y[3]);
+              sts128(dst + kk * kChunk + dst_at[k], y[0], y[1], y[2], y[3]);
             }
           } else {
-            const uint32_t base = dst + static_cast<uint32_t>(unit >> 2) * kChunk + static_cast<uint32_t>(row) * 128u;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {              // two words: eight columns
               uint32_t y[4];
@@ -552,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
               y[3] = add_f16x2(prmt(wd[2 * k + 1], ta.x64, 0x5352), 0xe480e480u);
 #pragma unroll
               for (int c = 0; c < 4; ++c) y[c] = mul_f16x2(y[c], s2);
-              sts128(base + (static_cast<uint32_t>(((unit & 3) * 2 + k) ^ (row & 7)) << 4), y[0], y[1], y[2], y[3]);
+              sts128(dst + (kk >> 1) * kChunk + (dst_at[k] ^ (64u * (kk & 1))), y[0], y[1], y[2], y[3]);
             }
           }
         }
@@ -563,26 +581,23 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
           mbar_arrive(&in_empty[2 * st + which]);
         }
       };
-      int ev[2] = {0, 0};                              // exponents of the values of tiles j, j + 1
-      auto keys = [&](int j) {
-        const uint32_t g = g0 + static_cast<uint32_t>(j);
-        ok = ok && mbar_wait_bounded_w(&in_full[2 * (g & 1u)], (g >> 1) & 1u, a.status, 241);
-        if (!survey(j)) return false;
-        ev[j & 1] = vref;
-        ok = mbar_wait_bounded_w(&k_empty[g & 1u], ((g >> 1) & 1u) ^ 1u, a.status, 242);
-        uint32_t bk = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) bk = max(bk, most[g & 1u][i]);
-        if (ok) convert(j, 0, bk == 0 ? 0 : max(static_cast<int>(bk >> 7) - 127 - C::kTop, -120));
-        return true;
-      };
-      go = steps <= 0 || keys(0);
-      for (int j = 0; j < steps && go; ++j) {          // keys run one tile ahead of values
-        const uint32_t g = g0 + static_cast<uint32_t>(j);
-        if (j + 1 < steps) go = keys(j + 1);
-        ok = ok && mbar_wait_bounded_w(&in_full[2 * (g & 1u) + 1], (g >> 1) & 1u, a.status, 243) &&
-             mbar_wait_bounded_w(&v_empty[g & 1u], ((g >> 1) & 1u) ^ 1u, a.status, 244);
-        if (ok && go) convert(j, 1, ev[j & 1]);
+      // Keys run one tile ahead of values: K0, K1, V0, K2, V1, ...
+      int ev[2] = {0, 0};                              // exponents of the values of an even, an odd tile
+#pragma unroll 1
+      for (int n = 0; n < 2 * steps + 1 && go; ++n) {
+        const int which = n > 0 && (n & 1) == 0 ? 1 : 0, j = which ? n / 2 - 1 : (n + 1) / 2;
+        if (j >= steps) continue;
+        const uint32_t g = g0 + static_cast<uint32_t>(j), st = g & 1u, ph = (g >> 1) & 1u;
+        ok = ok && mbar_wait_bounded_w(&in_full[2 * st + which], ph, a.status, 241);
+        int ex = ev[j & 1];
+        if (which == 0) {
+          go = survey(j, ex);
+          if (!go) break;
+          if (j & 1) ev[1] = vref;
+          else ev[0] = vref;
+        }
+        ok = ok && mbar_wait_bounded_w(which ? &v_empty[st] : &k_empty[st], ph ^ 1u, a.status, 242);
+        if (ok) convert(j, which, ex);
       }
       g0 += static_cast<uint32_t>(steps > 0 ? steps : 0);
     }
