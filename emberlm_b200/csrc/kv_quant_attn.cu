@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
     Feed& f = feed;
     for (int k = 0; f.left > 0; ++k) {
       const int st = k % kStages;
-      if (k >= kStages && !mbar_wait_bounded_w(&empty[st], (k / kStages + 1) & 1, a.status, 212)) break;
+      if (k >= kStages && !wait_w(&empty[st], (k / kStages + 1) & 1, a.status, 212)) break;
       if (lane == 0) {
         while (f.at >= f.end) {
           f.at -= static_cast<int>(f.u.end - f.u.begin);
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
   int used = 0;
   bool ok = true, first = true;
   for (;;) {                                           // one unit after the other
-    if (!first) ok = mbar_wait_bounded_w(&full[used % kStages], (used / kStages) & 1, a.status, 213);   // (the stage names its unit)
+    if (!first) ok = wait_w(&full[used % kStages], (used / kStages) & 1, a.status, 213);   // (the stage names its unit)
     const Unit& unit = first || !ok ? first_unit : stages[used % kStages].u;
     const int ub = unit.b, uh = unit.h, hi_row = unit.v.hi_row;
     const int64_t pos = unit.pos, count = unit.count;
@@ -696,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
     int st = used % kStages, all_ok;
     for (bool more = any; more && ok; ++used) {
       st = used % kStages;
-      ok = mbar_wait_bounded_w(&full[st], (used / kStages) & 1, a.status, 210);
+      ok = wait_w(&full[st], (used / kStages) & 1, a.status, 210);
       if (!ok) break;
       const Stage& f = stages[st];
       more = f.last == 0;
@@ -780,7 +780,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
     if (lane == 0) mbar_arrive(&empty[st]);
   }
   if (!ok)                                             // copies still on their way
-    for (int i = 0; i < kStages; ++i, ++used) mbar_wait_bounded_w(&full[used % kStages], (used / kStages) & 1, a.status, 211);
+    for (int i = 0; i < kStages; ++i, ++used) wait_w(&full[used % kStages], (used / kStages) & 1, a.status, 211);
 }
 
 // Joins the parts of the units that several CTAs worked on, in the order of their positions, and writes zeros for the units that

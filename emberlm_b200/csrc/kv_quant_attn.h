@@ -53,6 +53,29 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// As mbar_wait_bounded_w of common.cuh, with a time for which the hardware may put the warp to sleep: where many warps wait for one
+// another, those that poll take issue slots (a third of them in the prompt kernel) from those that work.
+__device__ __forceinline__ bool wait_w(uint64_t* bar, uint32_t parity, int* status, int where) {
+  uint32_t ok = 0;
+  uint64_t since = 0;
+  for (int tries = 0;; ++tries) {
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.b32 %0, 1, 0, p;\n}"
+                 : "=r"(ok)
+                 : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+                 : "memory");
+    if (ok != 0) break;
+    if (tries == 0) since = globaltimer_ns();
+    if ((tries & 15) == 15 && globaltimer_ns() - since > kWaitBudgetNs) {
+      if (status != nullptr && atomicCAS(status, 0, CTDK_ETIMEOUT) == 0) {
+        status[1] = where;
+        status[2] = static_cast<int>(blockIdx.x);
+        status[3] = static_cast<int>(parity);
+      }
+      break;
+    }
+  }
+  return __all_sync(0xffffffffu, ok != 0);
+}
 // Position of row t of a sequence, or -1 if it is not valid.
 __device__ __forceinline__ int row_position(int64_t pos, int64_t count, int64_t t, int64_t capacity) {
   const int64_t i = pos + t;

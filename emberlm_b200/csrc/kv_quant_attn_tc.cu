@@ -1,13 +1,16 @@
 // Attention of prompts and longer drafts over a key/value cache of 4 or 8 bits, on the tcgen05 tensor cores.
 //
 // An item is 128 query rows of one key/value head (its query heads side by side, row = token * heads + head) and a range of tiles of
-// 128 positions. Persistent CTAs, one per SM, walk the items, longest first. 14 warps:
-//   warp 0      TMA producer: codes and scales of keys and of values, two stages of each.
-//   warp 1      MMA issuer: S(j) = Q K(j)^T into one of two 128-column buffers in tensor memory, Q from tensor memory;
-//               O += P(j) V(j) with P from tensor memory, over S. S(j + 2) is queued right behind P V(j).
-//   warps 2-5   softmax, a row a thread: loads Q and puts it into tensor memory; maxima, exponentials and sums in fp32, in the log2
-//               domain; O is rescaled only when a row's maximum grew by more than 2^8.
-//   warps 6-13  turn codes into fp16 tiles, 128-byte-swizzled rows that serve as the K-major keys and the MN-major values alike.
+// 128 positions. Persistent CTAs, one per SM, walk the items, longest first. 19 warps:
+//   warp 0       TMA producer: codes and scales of keys and of values, two stages of each.
+//   warp 1       MMA issuer: S(j) = Q K(j)^T into one of two 128-column buffers in tensor memory, Q from tensor memory;
+//                O += P(j) V(j) with P from tensor memory, over S. S(j + 2) is queued right behind P V(j).
+//   warps 2-9    softmax, two threads a row, half of the columns each (one thread a row took twice as long as the products): load Q
+//                and put it into tensor memory; maxima, exponentials and sums in fp32, in the log2 domain; O is rescaled only when a
+//                row's maximum grew by more than 2^8.
+//   warps 10-17  turn codes into fp16 tiles, 128-byte-swizzled rows that serve as the K-major keys (four of them) and the MN-major
+//                values (the others) alike.
+//   warp 18      looks a tile's scales over, a tile ahead of those: exponents, NaN.
 // The products take fp16 operands. c * s is not exact in fp16 for every scale s, but c * s * 2^-e is, for the power of two that
 // brings a tile's largest scale near the top of the range, unless a scale is 2^28 times smaller than that one. Keys have an e of
 // their own in every tile (it joins the scores' factor), values one that O is rescaled for when a tile exceeds it. fp32 queries
@@ -27,7 +30,11 @@ constexpr int kChunk = 128 * 128;        // bytes of a {64 columns x 128 rows} t
 constexpr float kSlack = 8.0f;
 // Probabilities (2^kSlack at most) are held times 2^kLift, sums alike: fp16's smallest step is then 2^-31 of the largest one.
 constexpr float kLift = 7.0f;
-constexpr int kThreads = 14 * 32;
+constexpr int kSoft = 4, kMake = 12;     // first warps of the roles: whole warpgroups, which share out the registers anew
+constexpr int kThreads = 20 * 32;
+// Registers a thread: 96 at launch, shared out as 64 + 2 * 128 + 2 * 80 = 5 * 96.
+constexpr int kRegsLead = 64, kRegsSoft = 128, kRegsMake = 80;
+static_assert(kRegsLead + 2 * kRegsSoft + 2 * kRegsMake == 5 * 96, "an increase waits for what the others give back");
 constexpr int kRing = 4;                 // tiles whose exponents and NaN marks are kept
 constexpr int kRoom = 6;                 // powers of two by which values may grow before O is rescaled
 
@@ -121,9 +128,9 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
   constexpr int NT = sizeof(QT) == 4 ? 2 : 1;          // fp16 terms of a query, of a probability
   constexpr uint32_t kColS = 0, kColO = 2 * KT, kColQ = 2 * KT + 128;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t bars[24];
+  __shared__ uint64_t bars[27 + kRing];
   __shared__ uint32_t tmem_slot;
-  __shared__ uint32_t most[2][8];                      // warps' largest scales (bits), by parity of the tile
+  __shared__ float row_x[2][2][TQ];                    // what the two threads of a row tell each other, by parity of the exchange
   __shared__ int exp_k[kRing], exp_v[kRing], grow_v[kRing];   // exponents of a tile's keys and values; how far the latter has moved
   __shared__ uint32_t nan_any[kRing];
   __shared__ uint8_t nan_of[kRing][KT];                // groups of values that are NaN, by position
@@ -144,10 +151,12 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
   uint64_t* q_ready = bars + 20;     // Q of the item is in tensor memory, O of the one before has been read
   uint64_t* pv_full = bars + 21;     // O += P(g) V(g) has finished (one phase per step)
   uint64_t* o_full = bars + 22;      // the item's last one has
+  uint64_t* looked = bars + 23;      // [2][keys, values]: the scales have been looked over, for the warps that convert
+  uint64_t* told = bars + 27;        // [kRing] the same of values, for the softmax (which may lag by more than two tiles)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 23; ++i) mbar_init(&bars[i], i >= 4 && i < 8 ? 8 : i >= 8 && i < 10 ? 8 : i >= 12 && i < 14 ? 8 : i >= 18 && i < 21 ? 128 : 1);
+    for (int i = 0; i < 27 + kRing; ++i) mbar_init(&bars[i], (i >= 4 && i < 10) || i == 12 || i == 13 ? 4 : i >= 18 && i < 21 ? 256 : 1);
     mbar_fence_init();
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
@@ -162,30 +171,31 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
   const uint32_t tmem_base = tmem_slot;
   pdl_wait();
   // g = running count of tiles over all items of this CTA: stage g & 1, phase (g >> 1) & 1
+  if (warp < kSoft) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLead));
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t g = 0;
-      bool ok = true;
-      for (int it = blockIdx.x; it < ta.items && ok; it += gridDim.x) {
-        const Item w = item_at(ta, it);
-        const int bh = w.b * a.c.Hk + w.h;
-        for (int k = w.k0; k < w.k1 && ok; ++k, ++g) {
-          const int st = g & 1u, j = w.v.tile_at(k) * KT;
-          const int there = static_cast<int>(min(static_cast<int64_t>(KT), a.c.capacity - j));   // positions that the cache has
-          const int64_t sc = (static_cast<int64_t>(bh) * a.c.capacity + j) * C::kGroups;
+    uint32_t g = 0;
+    bool ok = true;
+    for (int it = blockIdx.x; it < ta.items && ok; it += gridDim.x) {
+      const Item w = item_at(ta, it);
+      const int bh = w.b * a.c.Hk + w.h;
+      for (int k = w.k0; k < w.k1 && ok; ++k, ++g) {
+        const int st = g & 1u, j = w.v.tile_at(k) * KT;
+        const int there = static_cast<int>(min(static_cast<int64_t>(KT), a.c.capacity - j));   // positions that the cache has
+        const int64_t sc = (static_cast<int64_t>(bh) * a.c.capacity + j) * C::kGroups;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            ok = ok && mbar_wait_bounded(&in_empty[2 * st + i], ((g >> 1) & 1u) ^ 1u, a.status, 220 + i);
-            if (!ok) break;
+        for (int i = 0; i < 2; ++i) {
+          ok = ok && wait_w(&in_empty[2 * st + i], ((g >> 1) & 1u) ^ 1u, a.status, 220 + i);
+          if (ok && lane == 0) {
             uint64_t* bar = &in_full[2 * st + i];
             mbar_expect_tx(bar, C::kCodes + there * C::kGroups * 2);
             tma_load_3d(codes_s + (2 * st + i) * C::kCodes, i ? &tm_v : &tm_k, bar, 0, j, bh);
             bulk_in(scales_s + (2 * st + i) * C::kScales, a.c.scales[i] + sc, there * C::kGroups * 2, bar);
           }
+          __syncwarp();
         }
       }
     }
-    __syncwarp();
   } else if (warp == 1) {
     // The whole warp runs this role converged; one elected lane issues each MMA / commit.
     const uint32_t idesc_s = idesc_f16(false, KT), idesc_pv = idesc_f16(true, D);
@@ -198,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
       if (steps <= 0) continue;
       auto issue_s = [&](int j) {
         const uint32_t g = g0 + static_cast<uint32_t>(j), s = g & 1u;
-        if (!mbar_wait_bounded_w(&k_full[s], (g >> 1) & 1u, a.status, 222)) return false;
+        if (!wait_w(&k_full[s], (g >> 1) & 1u, a.status, 222)) return false;
         tc_fence_after();
         const uint64_t kd = make_smem_desc(k_base + s * C::kTile, 16, 1024, kLayoutSw128);
         const uint32_t ts = tmem_base + kColS + s * KT, tq = tmem_base + kColQ;
@@ -211,14 +221,14 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
         umma_commit_w(&s_full[s]);
         return true;
       };
-      if (!mbar_wait_bounded_w(q_ready, n_it & 1u, a.status, 223)) break;
+      if (!wait_w(q_ready, n_it & 1u, a.status, 223)) break;
       ++n_it;
       tc_fence_after();
       ok = issue_s(0);
       if (ok && steps > 1) ok = issue_s(1);
       for (int j = 0; j < steps && ok; ++j) {
         const uint32_t g = g0 + static_cast<uint32_t>(j), s = g & 1u, ph = (g >> 1) & 1u;
-        ok = mbar_wait_bounded_w(&v_full[s], ph, a.status, 224) && mbar_wait_bounded_w(&p_ready[s], ph, a.status, 225);
+        ok = wait_w(&v_full[s], ph, a.status, 224) && wait_w(&p_ready[s], ph, a.status, 225);
         if (!ok) break;
         tc_fence_after();
         // B: 16 key rows (two 8-row swizzle groups, SBO) of every 64-column chunk of V (LBO)
@@ -228,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
         for (int kb = 0; kb < KT / 16; ++kb)
 #pragma unroll
           for (int x = 0; x < NT; ++x)
-            umma_bf16_ta_w(tmem_base + kColO, ts + static_cast<uint32_t>((kb >> 2) * 64 + x * 32 + (kb & 3) * 8), vd + ((kb * 2048) >> 4), idesc_pv,
+            umma_bf16_ta_w(tmem_base + kColO, ts + static_cast<uint32_t>((kb >> 1) * 32 + x * 16 + (kb & 1) * 8), vd + ((kb * 2048) >> 4), idesc_pv,
                            kb + x != 0 ? 1u : (j != 0 ? 1u : 0u));
         umma_commit_w(&v_empty[s]);
         umma_commit_w(pv_full);
@@ -238,37 +248,116 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
       g0 += static_cast<uint32_t>(steps);
     }
     __syncwarp();
-  } else if (warp < 6) {
-    const int quarter = warp & 3;                      // tensor-memory lanes of this warp
-    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t to = tmem_base + kColO + lane_off, tq = tmem_base + kColQ + lane_off;
-    uint32_t g0 = 0, n_done = 0;
+  } else if (warp == 2) {
+    // Exponents of a tile's keys and values, and which groups of its values are NaN. What none of the rows sees must not matter.
+    uint32_t g = 0;
     bool ok = true;
     for (int it = blockIdx.x; it < ta.items && ok; it += gridDim.x) {
       const Item w = item_at(ta, it);
-      const int steps = w.k1 - w.k0, rr = quarter * 32 + lane, r = w.r0 + rr, t = r / a.group, hg = r - t * a.group;
+      int vref = 0;
+      for (int k = w.k0; k < w.k1 && ok; ++k, ++g) {
+        const uint32_t st = g & 1u, ph = (g >> 1) & 1u;
+        const int j0 = w.v.tile_at(k) * KT;
+#pragma unroll 1
+        for (int which = 0; which < 2 && ok; ++which) {
+          ok = wait_w(&in_full[2 * st + which], ph, a.status, 243);
+          if (!ok) break;
+          const unsigned char* p = scales_s + (2 * st + which) * C::kScales;
+          uint32_t big = 0, any = 0;
+#pragma unroll
+          for (int i = 0; i < KT / 32; ++i) {
+            const int row = 32 * i + lane, at = j0 + row;
+            const bool seen = at < w.v.hi_row && (at >= w.v.lo_row || a.window == 0 || w.v.lo_row - at < a.window || at < a.sinks);
+            uint32_t sw[C::kGroups / 2], nan = 0, most = 0;
+            if constexpr (C::kGroups == 4) {
+              const uint2 x = *reinterpret_cast<const uint2*>(p + row * 8);
+              sw[0] = x.x, sw[C::kGroups / 2 - 1] = x.y;
+            } else {
+              sw[0] = *reinterpret_cast<const uint32_t*>(p + row * 4);
+            }
+#pragma unroll
+            for (int y = 0; y < C::kGroups; ++y) {
+              const uint32_t b = (y & 1 ? sw[y / 2] >> 16 : sw[y / 2]) & 0x7fffu;
+              if (is_nan_scale(b)) nan |= 1u << y;
+              else most = max(most, b);
+            }
+            if (!seen) most = nan = 0;
+            big = max(big, most);
+            any |= nan;
+            if (which == 1) nan_of[g % kRing][row] = static_cast<uint8_t>(nan);
+          }
+          big = __reduce_max_sync(0xffffffffu, big);
+          any = __any_sync(0xffffffffu, any != 0) ? 1u : 0u;
+          const int e = big == 0 ? (which ? -120 : 0) : max(static_cast<int>(big >> 7) - 127 - C::kTop, -120);
+          if (which == 0) {
+            exp_k[g % kRing] = e;                      // (all lanes: the same)
+          } else {
+            int moved = 0;
+            if (k == w.k0) {
+              vref = e + kRoom;
+            } else if (e > vref) {
+              moved = e + kRoom - vref;
+              vref += moved;
+            }
+            exp_v[g % kRing] = vref;
+            grow_v[g % kRing] = moved;
+            nan_any[g % kRing] = any;
+          }
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&looked[2 * st + which]);
+            if (which == 1) mbar_arrive(&told[g % kRing]);
+          }
+        }
+      }
+    }
+  }
+  } else if (warp < kMake) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
+    const int quarter = warp & 3, half = (warp - kSoft) >> 2;   // tensor-memory lanes of this warp; of the columns, 64 half ..
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t to = tmem_base + kColO + lane_off + half * (D / 2), tq = tmem_base + kColQ + lane_off;
+    const int rr = quarter * 32 + lane;
+    uint32_t g0 = 0, n_done = 0, n_ex = 0;
+    bool ok = true;
+    // The other thread's value of the row. The two warps also agree on `ok`: they give up together.
+    auto other = [&](float mine) {
+      float* x = &row_x[n_ex & 1u][0][0];
+      ++n_ex;
+      x[half * TQ + rr] = mine;
+      int all_ok;
+      asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.pred q, %2, 64, p;\n selp.b32 %0, 1, 0, q;\n}"
+                   : "=r"(all_ok) : "r"(static_cast<int>(ok)), "r"(1 + quarter) : "memory");
+      ok = all_ok != 0;
+      return x[(half ^ 1) * TQ + rr];
+    };
+    for (int it = blockIdx.x; it < ta.items && ok; it += gridDim.x) {
+      const Item w = item_at(ta, it);
+      const int steps = w.k1 - w.k0, r = w.r0 + rr, t = r / a.group, hg = r - t * a.group;
       const bool live = rr < w.rows;
       const int at = live ? row_position(w.pos, w.count, t, a.c.capacity) : -1;
       float m_ref = -INFINITY, l = 0.0f, o_scale = 0.0f;
       uint32_t poison = 0;                             // groups of columns that have met a NaN
       if (steps > 0) {
         // Q: a power of two brings the row's largest value near 64; terms into tensor memory, in the order of the converted keys
-        const QT* src = static_cast<const QT*>(a.q) + w.b * a.batch_stride + static_cast<int64_t>(t) * a.row_stride + static_cast<int64_t>(w.h * a.group + hg) * D;
+        const QT* src = static_cast<const QT*>(a.q) + w.b * a.batch_stride + static_cast<int64_t>(t) * a.row_stride +
+                        static_cast<int64_t>(w.h * a.group + hg) * D + half * (D / 2);
         float big = 0.0f;
         if (live)
 #pragma unroll 4
-          for (int i = 0; i < D; i += 8) {
+          for (int i = 0; i < D / 2; i += 8) {
             float x[8];
             load8(src + i, x);
 #pragma unroll
             for (int c = 0; c < 8; ++c) big = fmaxf(big, fabsf(x[c]));
           }
+        big = fmaxf(big, other(big));
         const int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;              // 128: not finite
         const int up = big == 0.0f || e == 128 ? 0 : max(min(6 - e, 126), -100);
         const float f = a.scale_log2 < 0.0f ? -pow2(up) : pow2(up);
         const float factor = fabsf(a.scale_log2) * pow2(-up);
 #pragma unroll 1
-        for (int i = 0; i < D; i += 32) {
+        for (int i = 0; i < D / 2; i += 32) {
           uint32_t q16[NT][16];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -290,76 +379,72 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
             }
           }
 #pragma unroll
-          for (int y = 0; y < NT; ++y) tmem_st_32x16(tq + static_cast<uint32_t>(y * (D / 2) + i / 2), q16[y]);
+          for (int y = 0; y < NT; ++y) tmem_st_32x16(tq + static_cast<uint32_t>(y * (D / 2) + half * (D / 4) + i / 2), q16[y]);
         }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(q_ready);
-        for (int j = 0; j < steps && ok; ++j) {
+        for (int j = 0; j < steps; ++j) {
           const uint32_t g = g0 + static_cast<uint32_t>(j), s = g & 1u;
-          ok = mbar_wait_bounded_w(&s_full[s], (g >> 1) & 1u, a.status, 230);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t ts = tmem_base + kColS + s * KT + lane_off;
-          const int j0 = w.v.tile_at(w.k0 + j) * KT;
-          const bool plain = j0 + KT - 1 <= w.v.lo_row && (a.window == 0 || w.v.hi_row - 1 - j0 < a.window || j0 + KT <= a.sinks);
+          ok = ok && wait_w(&told[g % kRing], (g / kRing) & 1u, a.status, 233);
+          const int j0 = w.v.tile_at(w.k0 + j) * KT + 64 * half;
+          const bool plain = j0 + 63 <= w.v.lo_row && (a.window == 0 || w.v.hi_row - 1 - j0 < a.window || j0 + 64 <= a.sinks);
           const float sc = fmaxf(factor * pow2(exp_k[g % kRing]), 0x1p-126f);
+          const int dv = grow_v[g % kRing];
+          const uint32_t ts = tmem_base + kColS + s * KT + lane_off + 64 * half;
+          ok = ok && wait_w(&s_full[s], (g >> 1) & 1u, a.status, 230);
+          tc_fence_after();
+          if (quarter * 32 >= w.rows) {                // none of the warp's rows is there: whatever lies in theirs may stay
+            mbar_arrive(&p_ready[s]);
+            continue;
+          }
+          float x[64];
+          tmem_ld_32x64_nowait(ts, x);
+          tmem_wait_ld();
           if (!plain) {
-            // Scores that the row does not see become minus infinity where they lie, so that the code below, which has to
-            // stay in the instruction cache beside the other roles', has one form. Which of 32 positions it sees, as bits: up
-            // to its own, from the window's first on or below the sinks.
-#pragma unroll 1
-            for (int q = 0; q < KT / 32; ++q) {
+            // which of 32 positions the row sees, as bits: up to its own, from the window's first on or below the sinks
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
               const int base = j0 + 32 * q;
               const uint32_t from = a.window == 0 ? 0xffffffffu : ~below(at - a.window + 1 - base) | below(a.sinks - base);
               const uint32_t bits = below(at + 1 - base) & from;
-              if (__all_sync(0xffffffffu, bits == 0xffffffffu)) continue;
-              float x[32];
-              tmem_ld_32x32(ts + 32 * q, x);
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if ((bits >> i & 1u) == 0) x[i] = -INFINITY;
-              tmem_st_32x32(ts + 32 * q, *reinterpret_cast<uint32_t(*)[32]>(x));
+                if ((bits >> i & 1u) == 0) x[32 * q + i] = -INFINITY;
             }
-            tmem_wait_st();
           }
-          float mx = -INFINITY;
-#pragma unroll 1
-          for (int hf = 0; hf < 2; ++hf) {
-            float x[64];
-            tmem_ld_32x64_nowait(ts + 64 * hf, x);
-            tmem_wait_ld();
-            float m0 = mx, m1 = x[0], m2 = x[1], m3 = x[2];
+          float mx;
+          {
+            float m0 = x[0], m1 = x[1], m2 = x[2], m3 = x[3];
 #pragma unroll
-            for (int i = 3; i + 7 < 64; i += 8) {
+            for (int i = 4; i + 7 < 64; i += 8) {
               m0 = fmax3(m0, x[i], x[i + 1]);
               m1 = fmax3(m1, x[i + 2], x[i + 3]);
               m2 = fmax3(m2, x[i + 4], x[i + 5]);
               m3 = fmax3(m3, x[i + 6], x[i + 7]);
             }
-            m0 = fmax3(m0, x[59], x[60]);
-            m1 = fmax3(m1, x[61], x[62]);
-            mx = fmaxf(fmax3(m0, m1, m2), fmaxf(m3, x[63]));
+            mx = fmax3(fmax3(m0, x[60], x[61]), fmax3(m1, x[62], x[63]), fmaxf(m2, m3));
           }
-          const float mxs = mx * sc;
-          const int dv = grow_v[g % kRing];
-          float c = 1.0f;
-          bool grow = dv != 0;
-          if (mxs > m_ref + kSlack) {
-            c = ex2(m_ref - mxs);
-            m_ref = mxs;
-            grow = true;
-          }
-          if (__any_sync(0xffffffffu, grow)) {
+          // Most tiles move no reference point: one barrier tells the two warps of these rows so.
+          int move;
+          asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, 64, p;\n selp.b32 %0, 1, 0, q;\n}"
+                       : "=r"(move) : "r"(static_cast<int>(mx * sc > m_ref + kSlack || dv != 0 || !ok)), "r"(1 + quarter) : "memory");
+          if (move != 0) {
+            const float mxs = fmaxf(mx, other(mx)) * sc;
+            if (!ok) break;
+            float c = 1.0f;
+            if (mxs > m_ref + kSlack) {
+              c = ex2(m_ref - mxs);
+              m_ref = mxs;
+            }
             if (j != 0) {
               // P V(g-1) must have landed before the accumulator is touched; P V(g) cannot start before every
-              // row has arrived at p_ready below
-              ok = mbar_wait_bounded_w(pv_full, (g - 1u) & 1u, a.status, 231);
-              if (!ok) break;
+              // row has arrived at p_ready below. Each thread of a row rescales half of the columns.
+              ok = wait_w(pv_full, (g - 1u) & 1u, a.status, 231);
               tc_fence_after();
               const float co = c * pow2(-dv);
 #pragma unroll 1
-              for (int p = 0; p < D / 32; ++p) {
+              for (int p = 0; p < D / 64; ++p) {
                 float o[32];
                 tmem_ld_32x32(to + p * 32, o);
 #pragma unroll
@@ -372,57 +457,50 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
           }
           const float neg_m = (m_ref == -INFINITY ? 0.0f : -m_ref) + kLift;
           float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll 1
-          for (int hf = 0; hf < 2; ++hf) {
-            float x[64];
-            tmem_ld_32x64_nowait(ts + 64 * hf, x);
-            tmem_wait_ld();
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t p16[NT][16];
+          for (int q = 0; q < 2; ++q) {                // 32 columns of scores make room for 16 of each term
+            uint32_t p16[NT][16];
 #pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                float u, v;
-                ffma2(u, v, x[32 * q + i], x[32 * q + i + 1], sc, sc, neg_m, neg_m);
-                u = ex2(u);
-                v = ex2(v);
-                fadd2(s0, s1, s0, s1, u, v);
-#pragma unroll
-                for (int y = 0; y < NT; ++y) {
-                  p16[y][i >> 1] = pack_f16(u, v);
-                  if (y + 1 < NT) {
-                    float a0, a1;
-                    unpack_f16(p16[y][i >> 1], a0, a1);
-                    u -= a0, v -= a1;
-                  }
-                }
+            for (int i = 0; i < 32; i += 2) {
+              // (packed pairs of fp32 measured slower here: 20 cycles an element of two terms against 17)
+              const float u = ex2(fmaf(x[32 * q + i], sc, neg_m)), v = ex2(fmaf(x[32 * q + i + 1], sc, neg_m));
+              s0 += u;
+              s1 += v;
+              if constexpr (NT == 2) {                 // the upper eleven bits, and the rest
+                const float u1 = __uint_as_float(__float_as_uint(u) & 0xffffe000u), v1 = __uint_as_float(__float_as_uint(v) & 0xffffe000u);
+                p16[0][i >> 1] = pack_f16(u1, v1);
+                p16[NT - 1][i >> 1] = pack_f16(u - u1, v - v1);
+              } else {
+                p16[0][i >> 1] = pack_f16(u, v);
               }
-#pragma unroll
-              for (int y = 0; y < NT; ++y) tmem_st_32x16(ts + 64 * hf + 32 * y + 16 * q, p16[y]);
             }
+#pragma unroll
+            for (int y = 0; y < NT; ++y) tmem_st_32x16(ts + 32 * q + 16 * y, p16[y]);
           }
           tmem_wait_st();
           tc_fence_before();
           if (nan_any[g % kRing] != 0)                 // NaN values: zeros in the tile; the rows that see them get NaN
 #pragma unroll 1
-            for (int i = 0; i < KT; ++i)
-              if (nan_of[g % kRing][i] != 0 && sees(at, j0 + i, a.window, a.sinks)) poison |= nan_of[g % kRing][i];
+            for (int i = 0; i < 64; ++i)
+              if (nan_of[g % kRing][64 * half + i] != 0 && sees(at, j0 + i, a.window, a.sinks)) poison |= nan_of[g % kRing][64 * half + i];
           if (j == steps - 1) o_scale = pow2(exp_v[g % kRing]);
           mbar_arrive(&p_ready[s]);
           l += s0 + s1;
         }
         g0 += static_cast<uint32_t>(steps);
         // The item's last P V. The next item's first one cannot start before these threads have read O and arrived at q_ready.
-        ok = ok && mbar_wait_bounded_w(o_full, n_done & 1u, a.status, 232);
-        if (!ok) break;
+        ok = ok && wait_w(o_full, n_done & 1u, a.status, 232);
         ++n_done;
         tc_fence_after();
+        l += other(l);
+        poison |= __float_as_uint(other(__uint_as_float(poison)));
+        if (!ok) break;
       }
       float* part = ta.splits > 1 ? a.part + static_cast<int64_t>(it) * TQ * (D + 2) : nullptr;
       const float f = part != nullptr ? o_scale : (at >= 0 ? o_scale / l : 0.0f);
-      QT* dst = static_cast<QT*>(a.out) + ((static_cast<int64_t>(w.b) * a.T + t) * a.H + w.h * a.group + hg) * D;
+      QT* dst = static_cast<QT*>(a.out) + ((static_cast<int64_t>(w.b) * a.T + t) * a.H + w.h * a.group + hg) * D + half * (D / 2);
 #pragma unroll 1
-      for (int p = 0; p < D / 32; ++p) {
+      for (int p = 0; p < D / 64; ++p) {
         float o[32];
         if (steps > 0) {
           tmem_ld_32x32(to + p * 32, o);               // warp-collective: rows past the end take part too
@@ -430,19 +508,18 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0.0f;
         }
+        const bool nan = (poison >> (half * (D / 64) + p) & 1u) != 0, none = part == nullptr && at < 0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = (poison >> p & 1u) != 0 ? __int_as_float(0x7fc00000) : o[i] * f;
-        if (part == nullptr && at < 0)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+        for (int i = 0; i < 32; ++i) o[i] = none ? 0.0f : nan ? __int_as_float(0x7fc00000) : o[i] * f;
 #pragma unroll
         for (int i = 0; i < 32; i += 8) {
           // columns as they came: pairs (c, c + 4) of eight, or in order
           const float y[8] = {o[i], BITS == 4 ? o[i + 2] : o[i + 1], BITS == 4 ? o[i + 4] : o[i + 2], BITS == 4 ? o[i + 6] : o[i + 3],
                               BITS == 4 ? o[i + 1] : o[i + 4], BITS == 4 ? o[i + 3] : o[i + 5], BITS == 4 ? o[i + 5] : o[i + 6], o[i + 7]};
           if (part != nullptr) {
-            store4(part + rr * D + 32 * p + i, y[0], y[1], y[2], y[3]);
-            store4(part + rr * D + 32 * p + i + 4, y[4], y[5], y[6], y[7]);
+            float* x = part + rr * D + half * (D / 2) + 32 * p + i;
+            store4(x, y[0], y[1], y[2], y[3]);
+            store4(x + 4, y[4], y[5], y[6], y[7]);
           } else if (live) {
             store4(dst + 32 * p + i, y[0], y[1], y[2], y[3]);
             store4(dst + 32 * p + i + 4, y[4], y[5], y[6], y[7]);
@@ -450,156 +527,84 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
         }
         __syncwarp();
       }
-      if (part != nullptr) {
+      if (part != nullptr && half == 0) {
         part[TQ * D + rr] = m_ref - kLift;
         part[TQ * D + TQ + rr] = l;
       }
       tc_fence_before();
     }
   } else {
-    const int mt = static_cast<int>(threadIdx.x) - 6 * 32, mw = mt >> 5;               // of the 256 that convert
-    // A thread's position in every tile; where its first 16 bytes of codes lie, as TMA has swizzled them; where its columns go.
-    const int row = mt & 127, half = mt >> 7;
-    const uint32_t row_at = static_cast<uint32_t>(row * C::kRow);
-    const uint32_t src_row = row_at + ((16u * half) ^ ((row_at >> 3) & (C::kRow - 16u)));
-    uint32_t dst_at[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) dst_at[k] = static_cast<uint32_t>(row) * 128u + ((static_cast<uint32_t>(half * (BITS == 4 ? 4 : 2) + k) ^ (row & 7u)) << 4);
-    uint32_t g0 = 0;
-    bool ok = true, go = true;                         // of this warp; of all of them
-    for (int it = blockIdx.x; it < ta.items && go; it += gridDim.x) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMake));
+    // Four warps convert keys, four values, each at its own pace. A thread has one position of a tile: its swizzles keep the reads
+    // and the writes of neighbouring lanes off each other's banks.
+    const int which = (warp - kMake) >> 2, row = ((warp - kMake) & 3) * 32 + lane;
+    const uint32_t row_at = static_cast<uint32_t>(row * C::kRow), row_swz = (row_at >> 3) & (C::kRow - 16u);   // as TMA has written it
+    const uint32_t dst_row = static_cast<uint32_t>(row) * 128u, dst_swz = static_cast<uint32_t>(row & 7) << 4;
+    uint64_t *full = which ? v_full : k_full, *empty = which ? v_empty : k_empty;
+    uint32_t g = 0;
+    bool ok = true;
+    for (int it = blockIdx.x; it < ta.items && ok; it += gridDim.x) {
       const Item w = item_at(ta, it);
-      const int steps = w.k1 - w.k0;
-      int vref = 0;
-      // Exponents of tile j's keys and values, and its NaN values: thread i reads a position's scales of one of them. False: over.
-      auto survey = [&](int j, int& ek) {
-        const uint32_t g = g0 + static_cast<uint32_t>(j), st = g & 1u, which = static_cast<uint32_t>(half);
-        const int at = w.v.tile_at(w.k0 + j) * KT + row;
-        ok = ok && mbar_wait_bounded_w(&in_full[2 * st + which], (g >> 1) & 1u, a.status, 240);
-        // seen by one of the rows: what else lies in the tile must not matter
-        const bool seen = at < w.v.hi_row && (at >= w.v.lo_row || a.window == 0 || w.v.lo_row - at < a.window || at < a.sinks);
-        const unsigned char* p = scales_s + (2 * st + which) * C::kScales + row * C::kGroups * 2;
-        uint32_t sw[C::kGroups / 2], big = 0, nan = 0;
-#pragma unroll
-        for (int i = 0; i < C::kGroups / 2; ++i) sw[i] = *reinterpret_cast<const uint32_t*>(p + 4 * i);
-#pragma unroll
-        for (int i = 0; i < C::kGroups; ++i) {
-          const uint32_t b = (i & 1 ? sw[i / 2] >> 16 : sw[i / 2]) & 0x7fffu;
-          if (is_nan_scale(b)) nan |= 1u << i;
-          else big = max(big, b);
-        }
-        if (!seen) big = nan = 0;
-        big = __reduce_max_sync(0xffffffffu, big);
-        if (which == 1) nan_of[g % kRing][row] = static_cast<uint8_t>(nan);
-        const bool any = __any_sync(0xffffffffu, nan != 0 && which == 1);
-        if (lane == 0) most[g & 1u][mw] = big | (any ? 0x80000000u : 0u);
-        // These warps give up together: a barrier that one of them never reached would hold the others for good.
-        int all_ok;
-        asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.pred q, 1, 256, p;\n selp.b32 %0, 1, 0, q;\n}"
-                     : "=r"(all_ok) : "r"(static_cast<int>(ok)) : "memory");
-        if (all_ok == 0) return false;
-        uint32_t bk = 0, bv = 0, flag = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          bk = max(bk, most[g & 1u][i]);
-          bv = max(bv, most[g & 1u][4 + i] & 0x7fffffffu);
-          flag |= most[g & 1u][4 + i] >> 31;
-        }
-        ek = bk == 0 ? 0 : max(static_cast<int>(bk >> 7) - 127 - C::kTop, -120);
-        const int ev = bv == 0 ? -120 : max(static_cast<int>(bv >> 7) - 127 - C::kTop, -120);
-        int moved = 0;
-        if (j == 0) {
-          vref = ev + kRoom;
-        } else if (ev > vref) {
-          moved = ev + kRoom - vref;
-          vref += moved;
-        }
-        if (mt == 0) {
-          exp_k[g % kRing] = ek;
-          exp_v[g % kRing] = vref;
-          grow_v[g % kRing] = moved;
-          nan_any[g % kRing] = flag;
-        }
-        return true;
-      };
-      // Tile j of keys (which 0) or values. A thread has one position and every second 16 bytes of its codes: neighbouring lanes
-      // neighbouring positions, whose swizzles keep the reads and the writes off each other's banks.
-      auto convert = [&](int j, int which, int ex) {
-        const uint32_t g = g0 + static_cast<uint32_t>(j), st = g & 1u;
-        const int at = w.v.tile_at(w.k0 + j) * KT + row;
-        const uint32_t src = smem_u32(codes_s) + (2 * st + which) * C::kCodes + src_row;
-        const uint32_t dst = smem_u32(which ? v_s : k_s) + st * C::kTile;
+#pragma unroll 1
+      for (int k = w.k0; k < w.k1; ++k, ++g) {
+        const uint32_t st = g & 1u, ph = (g >> 1) & 1u;
+        const int at = w.v.tile_at(k) * KT + row;
+        // (that the scales have been looked over says that the codes are there too)
+        ok = wait_w(&looked[2 * st + which], ph, a.status, 240) && wait_w(&empty[st], ph ^ 1u, a.status, 242);
+        if (!ok) break;
+        const int ex = which ? exp_v[g % kRing] : exp_k[g % kRing];
+        const uint32_t src = smem_u32(codes_s) + (2 * st + which) * C::kCodes + row_at;
+        const uint32_t dst = smem_u32(which ? v_s : k_s) + st * C::kTile + dst_row;
         const uint32_t scale = smem_u32(scales_s) + (2 * st + which) * C::kScales + static_cast<uint32_t>(row * C::kGroups * 2);
         const bool seen = at < w.v.hi_row && (at >= w.v.lo_row || a.window == 0 || w.v.lo_row - at < a.window || at < a.sinks);
         const float up = seen ? pow2(-ex) : 0.0f;
-        uint32_t sw[C::kGroups / 2];
-        if constexpr (C::kGroups == 4) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(sw[0]), "=r"(sw[1]) : "r"(scale));
-        else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(sw[0]) : "r"(scale));
-#pragma unroll
-        for (int kk = 0; kk < C::kRow / 32; ++kk) {
-          uint32_t wd[4];
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(wd[0]), "=r"(wd[1]), "=r"(wd[2]), "=r"(wd[3]) : "r"(src ^ (32u * kk)));
-          // 4 bits: 16 bytes are a group; 8 bits: half of one
-          uint32_t sb = sw[BITS == 4 ? kk : kk / 2];
-          if constexpr (BITS == 4) sb = half ? sb >> 16 : sb & 0xffffu;
-          else sb = kk & 1 ? sb >> 16 : sb & 0xffffu;
+#pragma unroll 1
+        for (int u = 0; u < C::kRow / 16; ++u) {       // 16 bytes: a group of 4-bit codes, half of one of 8-bit codes
+          uint32_t wd[4], sb;
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(wd[0]), "=r"(wd[1]), "=r"(wd[2]), "=r"(wd[3]) : "r"(src + ((16u * u) ^ row_swz)));
+          {
+            unsigned short x;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(scale + 2u * (BITS == 4 ? u : u / 2)));
+            sb = x;
+          }
           float sf = __uint_as_float(sb << 16);
           if (is_nan_scale(sb)) sf = which || !seen ? 0.0f : __int_as_float(0x7fc00000);
           sf *= up;
-          const uint32_t s2 = pack_f16(sf, sf);
+          const uint32_t su = pack_f16(sf, sf);        // the group's scale under the tile's power of two, twice
           if constexpr (BITS == 4) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {              // a word: eight columns
-              const uint32_t v = wd[k] >> 8;
+            for (int k4 = 0; k4 < 4; ++k4) {           // a word: eight columns
+              const uint32_t v = wd[k4] >> 8;
               uint32_t y[4];
-              y[0] = add_f16x2((wd[k] & 0x000f000fu) | ta.x64, 0xe408e408u);               // 1024 + u - 1032
-              y[1] = fma_f16x2((wd[k] & 0x00f000f0u) | ta.x64, 0x2c002c00u, 0xd480d480u);  // (1024 + 16 u) / 16 - 72
+              y[0] = add_f16x2((wd[k4] & 0x000f000fu) | ta.x64, 0xe408e408u);               // 1024 + u - 1032
+              y[1] = fma_f16x2((wd[k4] & 0x00f000f0u) | ta.x64, 0x2c002c00u, 0xd480d480u);  // (1024 + 16 u) / 16 - 72
               y[2] = add_f16x2((v & 0x000f000fu) | ta.x64, 0xe408e408u);
               y[3] = fma_f16x2((v & 0x00f000f0u) | ta.x64, 0x2c002c00u, 0xd480d480u);
 #pragma unroll
-              for (int c = 0; c < 4; ++c) y[c] = mul_f16x2(y[c], s2);
-              sts128(dst + kk * kChunk + dst_at[k], y[0], y[1], y[2], y[3]);
+              for (int c = 0; c < 4; ++c) y[c] = mul_f16x2(y[c], su);
+              sts128(dst + (u >> 1) * kChunk + (dst_swz ^ (16u * ((u & 1) * 4 + k4))), y[0], y[1], y[2], y[3]);
             }
           } else {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {              // two words: eight columns
+            for (int k2 = 0; k2 < 2; ++k2) {           // two words: eight columns
               uint32_t y[4];
-              y[0] = add_f16x2(prmt(wd[2 * k], ta.x64, 0x5150), 0xe480e480u);              // 1024 + u - 1152
-              y[1] = add_f16x2(prmt(wd[2 * k], ta.x64, 0x5352), 0xe480e480u);
-              y[2] = add_f16x2(prmt(wd[2 * k + 1], ta.x64, 0x5150), 0xe480e480u);
-              y[3] = add_f16x2(prmt(wd[2 * k + 1], ta.x64, 0x5352), 0xe480e480u);
+              y[0] = add_f16x2(prmt(wd[2 * k2], ta.x64, 0x5150), 0xe480e480u);              // 1024 + u - 1152
+              y[1] = add_f16x2(prmt(wd[2 * k2], ta.x64, 0x5352), 0xe480e480u);
+              y[2] = add_f16x2(prmt(wd[2 * k2 + 1], ta.x64, 0x5150), 0xe480e480u);
+              y[3] = add_f16x2(prmt(wd[2 * k2 + 1], ta.x64, 0x5352), 0xe480e480u);
 #pragma unroll
-              for (int c = 0; c < 4; ++c) y[c] = mul_f16x2(y[c], s2);
-              sts128(dst + (kk >> 1) * kChunk + (dst_at[k] ^ (64u * (kk & 1))), y[0], y[1], y[2], y[3]);
+              for (int c = 0; c < 4; ++c) y[c] = mul_f16x2(y[c], su);
+              sts128(dst + (u >> 2) * kChunk + (dst_swz ^ (16u * ((u & 3) * 2 + k2))), y[0], y[1], y[2], y[3]);
             }
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(which ? &v_full[st] : &k_full[st]);
+          mbar_arrive(&full[st]);
           mbar_arrive(&in_empty[2 * st + which]);
         }
-      };
-      // Keys run one tile ahead of values: K0, K1, V0, K2, V1, ...
-      int ev[2] = {0, 0};                              // exponents of the values of an even, an odd tile
-#pragma unroll 1
-      for (int n = 0; n < 2 * steps + 1 && go; ++n) {
-        const int which = n > 0 && (n & 1) == 0 ? 1 : 0, j = which ? n / 2 - 1 : (n + 1) / 2;
-        if (j >= steps) continue;
-        const uint32_t g = g0 + static_cast<uint32_t>(j), st = g & 1u, ph = (g >> 1) & 1u;
-        ok = ok && mbar_wait_bounded_w(&in_full[2 * st + which], ph, a.status, 241);
-        int ex = ev[j & 1];
-        if (which == 0) {
-          go = survey(j, ex);
-          if (!go) break;
-          if (j & 1) ev[1] = vref;
-          else ev[0] = vref;
-        }
-        ok = ok && mbar_wait_bounded_w(which ? &v_empty[st] : &k_empty[st], ph ^ 1u, a.status, 242);
-        if (ok) convert(j, which, ex);
       }
-      g0 += static_cast<uint32_t>(steps > 0 ? steps : 0);
     }
   }
   tc_fence_before();
