@@ -65,9 +65,9 @@ __global__ void __launch_bounds__(kThreads) kvq_write_kernel(const RowArgs a) {
   float x[8] = {};
   int64_t at = 0;
   if (live) {
-    const int64_t bh = r / a.T;
+    const int64_t bh = quotient(r, a.T);
     const int t = static_cast<int>(r - bh * a.T);
-    const int64_t b = bh / a.Hk;
+    const int64_t b = quotient(bh, a.Hk);
     const int h = static_cast<int>(bh - b * a.Hk);
     const int64_t p = (a.pos != nullptr ? static_cast<int64_t>(a.pos[b]) : a.pos_all) + t;
     live = p >= 0 && p < a.capacity && (a.count == nullptr || t < a.count[b]);
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kThreads) kvq_read_kernel(const ReadArgs a) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, r = i / kPerRow;
   const int lane8 = static_cast<int>(i % kPerRow), which = blockIdx.y;
   if (r >= a.rows) return;
-  const int64_t bh = r / a.length, t = r - bh * a.length, at = bh * a.c.capacity + a.start + t;
+  const int64_t bh = quotient(r, a.length), t = r - bh * a.length, at = bh * a.c.capacity + a.start + t;
   const float s = __bfloat162float((which ? a.c.scales[1] : a.c.scales[0])[at * (D / kGroup) + lane8 / 4]);
   const uint8_t* src = (which ? a.c.codes[1] : a.c.codes[0]) + at * kRowBytes + lane8 * BITS;
   float x[8];

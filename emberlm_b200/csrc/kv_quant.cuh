@@ -30,6 +30,11 @@ struct Cache {
 // Bits of a scale that stands for NaN: larger than any that is written (below 2^98), in either sign.
 __device__ __forceinline__ bool is_nan_scale(uint32_t bits) { return (bits & 0x7fffu) >= 0x7080u; }
 
+// x / n for x >= 0, n > 0: 64-bit divisions are a hundred instructions, and the numbers are small as a rule.
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t n) {
+  if (((x | n) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(n);
+  return x / n;
+}
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {

@@ -199,11 +199,6 @@ __device__ __forceinline__ void next_unit(const AttnArgs& a, Unit& u) {
   u.end += u.v.tiles;
 }
 
-// x / n for x >= 0, n > 0: 64-bit divisions are a hundred instructions, and the numbers are small as a rule.
-__device__ __forceinline__ int64_t quotient(int64_t x, int64_t n) {
-  if (((x | n) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(n);
-  return x / n;
-}
 __device__ __forceinline__ int64_t span_start(int64_t all, int i, int n) { return quotient(all * i, n); }
 
 // Sum over the CTA of one value a thread (all threads get it), and of the values of the threads before (exclusive).

@@ -53,18 +53,20 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// As mbar_wait_bounded_w of common.cuh, with a time for which the hardware may put the warp to sleep: where many warps wait for one
-// another, those that poll take issue slots (a third of them in the prompt kernel) from those that work.
-__device__ __forceinline__ bool wait_w(uint64_t* bar, uint32_t parity, int* status, int where) {
-  uint32_t ok = 0;
-  uint64_t since = 0;
-  for (int tries = 0;; ++tries) {
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.b32 %0, 1, 0, p;\n}"
-                 : "=r"(ok)
-                 : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
-                 : "memory");
-    if (ok != 0) break;
-    if (tries == 0) since = globaltimer_ns();
+// As mbar_wait_bounded_w of common.cuh, with a time for which the hardware may put the warp to sleep, and with what follows a first
+// try that fails off the common path: the kernels' roles together are larger than an instruction cache, and most waits are over at once.
+__device__ __forceinline__ uint32_t try_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.b32 %0, 1, 0, p;\n}"
+               : "=r"(ok)
+               : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+               : "memory");
+  return ok;
+}
+__device__ __forceinline__ bool wait_longer(uint64_t* bar, uint32_t parity, int* status, int where) {
+  const uint64_t since = globaltimer_ns();
+  uint32_t ok;
+  for (int tries = 0; (ok = try_wait(bar, parity)) == 0; ++tries)
     if ((tries & 15) == 15 && globaltimer_ns() - since > kWaitBudgetNs) {
       if (status != nullptr && atomicCAS(status, 0, CTDK_ETIMEOUT) == 0) {
         status[1] = where;
@@ -73,8 +75,12 @@ __device__ __forceinline__ bool wait_w(uint64_t* bar, uint32_t parity, int* stat
       }
       break;
     }
-  }
   return __all_sync(0xffffffffu, ok != 0);
+}
+__device__ __forceinline__ bool wait_w(uint64_t* bar, uint32_t parity, int* status, int where) {
+  bool ok = __all_sync(0xffffffffu, try_wait(bar, parity) != 0);
+  if (__builtin_expect(!ok, 0)) ok = wait_longer(bar, parity, status, where);
+  return ok;
 }
 // Position of row t of a sequence, or -1 if it is not valid.
 __device__ __forceinline__ int row_position(int64_t pos, int64_t count, int64_t t, int64_t capacity) {

@@ -131,7 +131,8 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
   __shared__ uint64_t bars[27 + kRing];
   __shared__ uint32_t tmem_slot;
   __shared__ float row_x[2][2][TQ];                    // what the two threads of a row tell each other, by parity of the exchange
-  __shared__ int exp_k[kRing], exp_v[kRing], grow_v[kRing];   // exponents of a tile's keys and values; how far the latter has moved
+  __shared__ int exp_k[kRing], exp_v[kRing];           // exponents of a tile's keys and values
+  __shared__ float scale_k[kRing], shrink_o[kRing];    // 2^exp_k; what O has to be multiplied by, as exp_v has moved
   __shared__ uint32_t nan_any[kRing];
   __shared__ uint8_t nan_of[kRing][KT];                // groups of values that are NaN, by position
   const AttnArgs& a = ta.a;
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
   uint64_t* pv_full = bars + 21;     // O += P(g) V(g) has finished (one phase per step)
   uint64_t* o_full = bars + 22;      // the item's last one has
   uint64_t* looked = bars + 23;      // [2][keys, values]: the scales have been looked over, for the warps that convert
-  uint64_t* told = bars + 27;        // [kRing] the same of values, for the softmax (which may lag by more than two tiles)
+  uint64_t* told = bars + 27;        // [kRing] the same of values, for the MMA issuer and the softmax behind it (by up to three tiles)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch();
   if (threadIdx.x == 0) {
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
       if (steps <= 0) continue;
       auto issue_s = [&](int j) {
         const uint32_t g = g0 + static_cast<uint32_t>(j), s = g & 1u;
-        if (!wait_w(&k_full[s], (g >> 1) & 1u, a.status, 222)) return false;
+        if (!wait_w(&k_full[s], (g >> 1) & 1u, a.status, 222) || !wait_w(&told[g % kRing], (g / kRing) & 1u, a.status, 233)) return false;
         tc_fence_after();
         const uint64_t kd = make_smem_desc(k_base + s * C::kTile, 16, 1024, kLayoutSw128);
         const uint32_t ts = tmem_base + kColS + s * KT, tq = tmem_base + kColQ;
@@ -291,6 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
           const int e = big == 0 ? (which ? -120 : 0) : max(static_cast<int>(big >> 7) - 127 - C::kTop, -120);
           if (which == 0) {
             exp_k[g % kRing] = e;                      // (all lanes: the same)
+            scale_k[g % kRing] = pow2(e);
           } else {
             int moved = 0;
             if (k == w.k0) {
@@ -300,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
               vref += moved;
             }
             exp_v[g % kRing] = vref;
-            grow_v[g % kRing] = moved;
+            shrink_o[g % kRing] = pow2(-moved);
             nan_any[g % kRing] = any;
           }
           __syncwarp();
@@ -384,13 +386,13 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(q_ready);
+        // 64 positions from j0 on are seen by every row: j0 from plain_lo to plain_hi, or up to plain_sink
+        const int plain_lo = a.window == 0 ? 0 : w.v.hi_row - a.window, plain_hi = w.v.lo_row - 63;
+        const int plain_sink = a.window == 0 ? -1 : min(a.sinks - 64, plain_hi);
         for (int j = 0; j < steps; ++j) {
           const uint32_t g = g0 + static_cast<uint32_t>(j), s = g & 1u;
-          ok = ok && wait_w(&told[g % kRing], (g / kRing) & 1u, a.status, 233);
           const int j0 = w.v.tile_at(w.k0 + j) * KT + 64 * half;
-          const bool plain = j0 + 63 <= w.v.lo_row && (a.window == 0 || w.v.hi_row - 1 - j0 < a.window || j0 + 64 <= a.sinks);
-          const float sc = fmaxf(factor * pow2(exp_k[g % kRing]), 0x1p-126f);
-          const int dv = grow_v[g % kRing];
+          const bool plain = (j0 >= plain_lo && j0 <= plain_hi) || j0 <= plain_sink;
           const uint32_t ts = tmem_base + kColS + s * KT + lane_off + 64 * half;
           ok = ok && wait_w(&s_full[s], (g >> 1) & 1u, a.status, 230);
           tc_fence_after();
@@ -400,6 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
           }
           float x[64];
           tmem_ld_32x64_nowait(ts, x);
+          const float sc = fmaxf(factor * scale_k[g % kRing], 0x1p-126f), shrink = shrink_o[g % kRing];
           tmem_wait_ld();
           if (!plain) {
             // which of 32 positions the row sees, as bits: up to its own, from the window's first on or below the sinks
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
           // Most tiles move no reference point: one barrier tells the two warps of these rows so.
           int move;
           asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, 64, p;\n selp.b32 %0, 1, 0, q;\n}"
-                       : "=r"(move) : "r"(static_cast<int>(mx * sc > m_ref + kSlack || dv != 0 || !ok)), "r"(1 + quarter) : "memory");
+                       : "=r"(move) : "r"(static_cast<int>(mx * sc > m_ref + kSlack || shrink != 1.0f || !ok)), "r"(1 + quarter) : "memory");
           if (move != 0) {
             const float mxs = fmaxf(mx, other(mx)) * sc;
             if (!ok) break;
@@ -442,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
               // row has arrived at p_ready below. Each thread of a row rescales half of the columns.
               ok = wait_w(pv_full, (g - 1u) & 1u, a.status, 231);
               tc_fence_after();
-              const float co = c * pow2(-dv);
+              const float co = c * shrink;
 #pragma unroll 1
               for (int p = 0; p < D / 64; ++p) {
                 float o[32];
