@@ -71,8 +71,9 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t x, uint32_t s) {
 // operation it spends a second one on it.
 struct Patterns {
   uint32_t x43, x3f;                     // bfloat16 128, 1 / 2
+  uint32_t up0, up4, less;               // fp16 2^15, 2^11; minus the codes' bias, times 2^-9
 };
-inline Patterns patterns() { return {0x43004300u, 0x3f003f00u}; }
+inline Patterns patterns(int bits) { return {0x43004300u, 0x3f003f00u, 0x78007800u, 0x68006800u, bits == 4 ? 0xa400a400u : 0xb400b400u}; }
 
 #ifdef __CUDACC__
 // Stored codes u as fp16 numbers: the bits alone are the subnormal numbers u * 2^-24, or u * 2^-20 where they lie four places higher.
@@ -88,6 +89,15 @@ __device__ __forceinline__ void codes4_f16(uint32_t w, uint32_t (&out)[4]) {
 __device__ __forceinline__ void codes8_f16(uint32_t w, uint32_t (&out)[2]) {
   out[0] = prmt(w, 0, 0x4140);
   out[1] = prmt(w, 0, 0x4342);
+}
+// The same numbers without the bias, times 2^-9: (u - 8) * 2^-9, (u - 128) * 2^-9.
+__device__ __forceinline__ void unbias4_f16(uint32_t (&x)[4], const Patterns& c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = fma_f16x2(x[i], i & 1 ? c.up4 : c.up0, c.less);
+}
+__device__ __forceinline__ void unbias8_f16(uint32_t (&x)[2], const Patterns& c) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) x[i] = fma_f16x2(x[i], c.up0, c.less);
 }
 // Codes times their scales as bfloat16 numbers: the bits go under the exponent of a power of two.
 // 4 bits: nibble i of both halves of w, the halves' scales in s2.

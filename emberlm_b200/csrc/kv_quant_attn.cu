@@ -434,12 +434,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if ((c4 & 7) == 0) q_init[rr][c4 / 8] = sum * (BITS == 4 ? -8.0f * 0x1p-24f : -128.0f * 0x1p-24f);
-      if (c4 == 0) q_factor[rr] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + 24 - up) << 23);   // up is from -100 to 126
-      if constexpr (BITS == 4) {                       // columns 8 tig + c of a group: pairs (c, c + 4); odd c times 2^-4
+      if (c4 == 0) q_factor[rr] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + (NQ == 1 ? 24 : 9) - up) << 23);   // up is from -100 to 126
+      if constexpr (BITS == 4) {                       // columns 8 tig + c of a group: pairs (c, c + 4); odd c times 2^-4 beside raw codes
         const int row_lane = (rr & 7) * 4 + ((c4 >> 1) & 3), half = c4 & 1, word = 4 * (c4 >> 3);
         uint32_t t01[NQ], t23[NQ];
-        terms_f16<NQ>(x[0], x[1] * 0.0625f, t01);
-        terms_f16<NQ>(x[2], x[3] * 0.0625f, t23);
+        constexpr float odd = NQ == 1 ? 0.0625f : 1.0f;
+        terms_f16<NQ>(x[0], x[1] * odd, t01);
+        terms_f16<NQ>(x[2], x[3] * odd, t23);
 #pragma unroll
         for (int z = 0; z < NQ; ++z) {
           uint16_t* w = reinterpret_cast<uint16_t*>(&q_terms[n][z][row_lane][word]) + half;
@@ -511,14 +512,23 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
         for (int x = 0; x < ROW / 32; ++x) {           // two chunks of 16 bytes: two groups of 4-bit codes, one of 8-bit codes
           uint32_t w[4];                               // chunk 2 x of positions g, g + 8; chunk 2 x + 1 of both
           ldsm4(w, kbase + k * 16 * ROW + (lane_at ^ (32u * x)));
-          auto step = [&](int ks, const uint32_t (&f)[4]) {   // a group is two steps
+          // A group is two steps. The tensor cores cut sums off rather than round them, at the size of the sum so far. For bfloat16
+          // queries that does not matter: raw codes, on top of what takes their bias off. fp32 queries meet codes without
+          // bias, whose sums are smaller, and their small terms go first.
+          auto group = [&](int gr, const uint32_t (&f0)[4], const uint32_t (&f1)[4]) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int y = 0; y < NQ; ++y) {
-                if ((ks & 1) == 0 && y == 0) mma_f16_from(acc[n], f, qf[n][y][2 * ks], qf[n][y][2 * ks + 1], init[n][ks / 2]);
-                else mma_f16(acc[n], f, qf[n][y][2 * ks], qf[n][y][2 * ks + 1]);
+            for (int n = 0; n < NT; ++n) {
+              if constexpr (NQ == 1) {
+                mma_f16_from(acc[n], f0, qf[n][0][4 * gr], qf[n][0][4 * gr + 1], init[n][gr]);
+                mma_f16(acc[n], f1, qf[n][0][4 * gr + 2], qf[n][0][4 * gr + 3]);
+              } else {
+                const float zero[2] = {0.0f, 0.0f};
+                mma_f16_from(acc[n], f0, qf[n][NQ - 1][4 * gr], qf[n][NQ - 1][4 * gr + 1], zero);
+                mma_f16(acc[n], f1, qf[n][NQ - 1][4 * gr + 2], qf[n][NQ - 1][4 * gr + 3]);
+                mma_f16(acc[n], f0, qf[n][0][4 * gr], qf[n][0][4 * gr + 1]);
+                mma_f16(acc[n], f1, qf[n][0][4 * gr + 2], qf[n][0][4 * gr + 3]);
               }
+            }
           };
           auto scaled = [&](int gr) {
             const float s0 = __uint_as_float(gr & 1 ? sc[0][gr / 2] & 0xffff0000u : sc[0][gr / 2] << 16);
@@ -535,20 +545,28 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
               uint32_t p[4], q[4];
               codes4_f16(w[2 * y], p);
               codes4_f16(w[2 * y + 1], q);
+              if constexpr (NQ == 2) {
+                unbias4_f16(p, ta.bits);
+                unbias4_f16(q, ta.bits);
+              }
               const uint32_t f0[4] = {p[0], q[0], p[1], q[1]}, f1[4] = {p[2], q[2], p[3], q[3]};
-              step(4 * x + 2 * y, f0);
-              step(4 * x + 2 * y + 1, f1);
+              group(2 * x + y, f0, f1);
               scaled(2 * x + y);
             }
           } else {
+            uint32_t f[2][4];
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               uint32_t p[2], q[2];
               codes8_f16(w[2 * y], p);
               codes8_f16(w[2 * y + 1], q);
-              const uint32_t f[4] = {p[0], q[0], p[1], q[1]};
-              step(2 * x + y, f);
+              if constexpr (NQ == 2) {
+                unbias8_f16(p, ta.bits);
+                unbias8_f16(q, ta.bits);
+              }
+              f[y][0] = p[0], f[y][1] = q[0], f[y][2] = p[1], f[y][3] = q[1];
             }
+            group(x, f[0], f[1]);
             scaled(x);
           }
         }
@@ -634,11 +652,21 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
 #pragma unroll
           for (int gr = 0; gr < GROUPS; ++gr) s2[hf][gr] = prmt(sc[gr / 2], sc[SW + gr / 2], gr & 1 ? 0x7632 : 0x5410);
         }
+        // (for fp32 outputs the block's sums are formed apart, smallest terms first, and added in fp32: hundreds of sums that are
+        // cut off, one on top of the other, cost 1e-5)
         auto product = [&](int i, const uint32_t (&f)[4]) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n) {
+            if constexpr (NP == 1) {
+              mma_bf16(o[n][i], f, pf[n][0][0], pf[n][0][1]);
+            } else {
+              float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int y = 0; y < NP; ++y) mma_bf16(o[n][i], f, pf[n][y][0], pf[n][y][1]);
+              for (int y = NP - 1; y >= 0; --y) mma_bf16(t, f, pf[n][y][0], pf[n][y][1]);
+              fadd2(o[n][i][0], o[n][i][1], o[n][i][0], o[n][i][1], t[0], t[1]);
+              fadd2(o[n][i][2], o[n][i][3], o[n][i][2], o[n][i][3], t[2], t[3]);
+            }
+          }
         };
 #pragma unroll
         for (int x = 0; x < ROW / 32; ++x) {
@@ -1007,7 +1035,7 @@ int ctdk_kvq_attn(const ctdk_kvq_cache* cache, const void* q, int dtype, int64_t
     return kvq::attn_tc(a, dtype, cache->bits, cache->D, static_cast<cudaStream_t>(stream));
   }
   ta.rows = static_cast<int>(rows);
-  ta.bits = kvq::patterns();
+  ta.bits = kvq::patterns(cache->bits);
   const int nt = rows <= 8 ? 1 : 2;
   const int64_t tiles = kvq::most_tiles(a, cache->D, cache->bits);
   ta.split = kvq::split_wanted(rows, tiles) ? 1 : 0;

@@ -35,6 +35,9 @@ constexpr int kThreads = 20 * 32;
 // Registers a thread: 96 at launch, shared out as 64 + 2 * 128 + 2 * 80 = 5 * 96.
 constexpr int kRegsLead = 64, kRegsSoft = 128, kRegsMake = 80;
 static_assert(kRegsLead + 2 * kRegsSoft + 2 * kRegsMake == 5 * 96, "an increase waits for what the others give back");
+// fp32 outputs: the tensor cores cut sums off rather than round them, which over a long row cost 1e-5. O is summed there over this
+// many tiles, and the sums of those are added in fp32, in memory that stays in L2 (registers and tensor memory are full).
+constexpr int kTogether = 4;
 constexpr int kRing = 4;                 // tiles whose exponents and NaN marks are kept
 constexpr int kRoom = 6;                 // powers of two by which values may grow before O is rescaled
 
@@ -51,6 +54,7 @@ struct TcArgs {
   AttnArgs a;
   int rows, row_tiles, splits, items;    // T * group; of 128; ranges of an item's tiles; in all
   uint32_t x64;                          // 0x64006400: fp16 1024
+  float* total;                          // fp32: gathered sums, [CTA][TQ * D]
 };
 struct Item {
   int b, h, r0, rows, ks, k0, k1;        // tiles k0 .. k1 - 1 of the visit
@@ -214,10 +218,11 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
         const uint64_t kd = make_smem_desc(k_base + s * C::kTile, 16, 1024, kLayoutSw128);
         const uint32_t ts = tmem_base + kColS + s * KT, tq = tmem_base + kColQ;
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
+        for (int x = NT - 1; x >= 0; --x)              // the small terms first: sums are cut off at their own size
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks)
-            umma_bf16_ta_w(ts, tq + static_cast<uint32_t>(x * (D / 2) + ks * 8), kd + (((ks >> 2) * kChunk + (ks & 3) * 32) >> 4), idesc_s, x + ks != 0 ? 1u : 0u);
+            umma_bf16_ta_w(ts, tq + static_cast<uint32_t>(x * (D / 2) + ks * 8), kd + (((ks >> 2) * kChunk + (ks & 3) * 32) >> 4), idesc_s,
+                           x != NT - 1 || ks != 0 ? 1u : 0u);
         umma_commit_w(&k_empty[s]);
         umma_commit_w(&s_full[s]);
         return true;
@@ -236,11 +241,11 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
         const uint64_t vd = make_smem_desc(v_base + s * C::kTile, kChunk, 1024, kLayoutSw128);
         const uint32_t ts = tmem_base + kColS + s * KT;
 #pragma unroll
-        for (int kb = 0; kb < KT / 16; ++kb)
+        for (int x = NT - 1; x >= 0; --x)
 #pragma unroll
-          for (int x = 0; x < NT; ++x)
+          for (int kb = 0; kb < KT / 16; ++kb)
             umma_bf16_ta_w(tmem_base + kColO, ts + static_cast<uint32_t>((kb >> 1) * 32 + x * 16 + (kb & 1) * 8), vd + ((kb * 2048) >> 4), idesc_pv,
-                           kb + x != 0 ? 1u : (j != 0 ? 1u : 0u));
+                           x != NT - 1 || kb != 0 || (NT == 2 ? j % kTogether != 0 : j != 0) ? 1u : 0u);
         umma_commit_w(&v_empty[s]);
         umma_commit_w(pv_full);
         if (j == steps - 1) umma_commit_w(o_full);
@@ -322,6 +327,22 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
     const int rr = quarter * 32 + lane;
     uint32_t g0 = 0, n_done = 0, n_ex = 0;
     bool ok = true;
+    // Adds the thread's part of O, times `now`, to what it has gathered, times `then` (nothing yet: any is false).
+    float4* total = reinterpret_cast<float4*>(ta.total) + static_cast<int64_t>(blockIdx.x) * (TQ * D / 4) + (threadIdx.x - kSoft * 32);
+    auto gather = [&](bool any, float now, float then) {
+#pragma unroll 1
+      for (int p = 0; p < D / 64; ++p) {
+        float4 t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = any ? total[(8 * p + i) * 256] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float o[32];
+        tmem_ld_32x32(to + p * 32, o);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          total[(8 * p + i) * 256] = make_float4(fmaf(t[i].x, then, o[4 * i] * now), fmaf(t[i].y, then, o[4 * i + 1] * now),
+                                                 fmaf(t[i].z, then, o[4 * i + 2] * now), fmaf(t[i].w, then, o[4 * i + 3] * now));
+      }
+    };
     // The other thread's value of the row. The two warps also agree on `ok`: they give up together.
     auto other = [&](float mine) {
       float* x = &row_x[n_ex & 1u][0][0];
@@ -339,6 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
       const bool live = rr < w.rows;
       const int at = live ? row_position(w.pos, w.count, t, a.c.capacity) : -1;
       float m_ref = -INFINITY, l = 0.0f, o_scale = 0.0f;
+      float pending = 1.0f, before = 1.0f;             // what the gathered sums, O itself, have to be multiplied by
       uint32_t poison = 0;                             // groups of columns that have met a NaN
       if (steps > 0) {
         // Q: a power of two brings the row's largest value near 64; terms into tensor memory, in the order of the converted keys
@@ -440,7 +462,8 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
               c = ex2(m_ref - mxs);
               m_ref = mxs;
             }
-            if (j != 0) {
+            pending *= c * shrink;
+            if (j != 0 && (NT == 1 || j % kTogether != 0)) {
               // P V(g-1) must have landed before the accumulator is touched; P V(g) cannot start before every
               // row has arrived at p_ready below. Each thread of a row rescales half of the columns.
               ok = wait_w(pv_full, (g - 1u) & 1u, a.status, 231);
@@ -457,6 +480,16 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
               }
             }
             l *= c;
+            before = c * shrink;
+          }
+          if constexpr (NT == 2) {
+            if (j != 0 && j % kTogether == 0) {        // the sums of the tiles before join the rest
+              ok = ok && wait_w(pv_full, (g - 1u) & 1u, a.status, 234);
+              tc_fence_after();
+              gather(j != kTogether, before, pending);
+              pending = 1.0f;
+            }
+            before = 1.0f;
           }
           const float neg_m = (m_ref == -INFINITY ? 0.0f : -m_ref) + kLift;
           float s0 = 0.0f, s1 = 0.0f;
@@ -510,6 +543,16 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+        }
+        if (NT == 2 && steps > kTogether) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 t = total[(8 * p + i) * 256];
+            o[4 * i] = fmaf(t.x, pending, o[4 * i]);
+            o[4 * i + 1] = fmaf(t.y, pending, o[4 * i + 1]);
+            o[4 * i + 2] = fmaf(t.z, pending, o[4 * i + 2]);
+            o[4 * i + 3] = fmaf(t.w, pending, o[4 * i + 3]);
+          }
         }
         const bool nan = (poison >> (half * (D / 64) + p) & 1u) != 0, none = part == nullptr && at < 0;
 #pragma unroll
@@ -685,7 +728,7 @@ int64_t row_items(int64_t B, int Hk, int64_t rows) { return B * Hk * ((rows + TQ
 
 int64_t attn_tc_bytes(int64_t B, int Hk, int D, int64_t rows) {
   const int64_t items = row_items(B, Hk, rows), splits = splits_of(items, INT32_MAX);
-  return splits > 1 ? items * splits * TQ * (D + 2) * 4 : 0;
+  return static_cast<int64_t>(sm_count()) * TQ * D * 4 + (splits > 1 ? items * splits * TQ * (D + 2) * 4 : 0);
 }
 
 int attn_tc(const AttnArgs& a, int dtype, int bits, int D, cudaStream_t s) {
@@ -701,6 +744,8 @@ int attn_tc(const AttnArgs& a, int dtype, int bits, int D, cudaStream_t s) {
   CTDK_REQUIRE(rows <= INT32_MAX / 2 && items * ta.splits <= INT32_MAX / 16, "kvq_attn: too many rows");
   ta.items = static_cast<int>(items * ta.splits);
   ta.x64 = 0x64006400u;
+  ta.total = a.part;                                   // (used by fp32 calls)
+  ta.a.part = a.part + static_cast<int64_t>(sm_count()) * TQ * D;
   const bool f32 = dtype == CTDK_DTYPE_F32;
   if (bits == 4) {
     if (D == 64) return f32 ? launch<float, 64, 4>(ta, s) : launch<__nv_bfloat16, 64, 4>(ta, s);
