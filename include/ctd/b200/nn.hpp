@@ -120,6 +120,7 @@ struct MLP {
 struct KVLayer {
   Tensor k;   // [B, H_kv, max_seq_len, D]
   Tensor v;
+  ops::QuantizedKV quantized{};   // where it is defined, it holds the layer's keys and values, and k and v are empty
 };
 
 struct KVCache {
@@ -135,6 +136,19 @@ struct KVCache {
     for (int i = 0; i < num_layers; ++i)
       c.layers.push_back({Tensor::zeros({batch, num_kv_heads, max_seq, head_dim}, DType::kFloat32, device),
                           Tensor::zeros({batch, num_kv_heads, max_seq, head_dim}, DType::kFloat32, device)});
+    return c;
+  }
+  // The same in 4 or 8 bits a value; with a window, queries see that many positions back (themselves among them), and the
+  // first `sinks` positions.
+  static KVCache allocate_quantized(int num_layers, int num_kv_heads, int head_dim, int64_t batch, int64_t max_seq, int bits, Device device,
+                                    int64_t window = 0, int64_t sinks = 0) {
+    KVCache c;
+    c.batch = batch;
+    c.max_seq_len = max_seq;
+    for (int i = 0; i < num_layers; ++i) {
+      c.layers.emplace_back();
+      c.layers.back().quantized = ops::QuantizedKV::allocate(num_kv_heads, head_dim, batch, max_seq, bits, device, window, sinks);
+    }
     return c;
   }
   void reset() { current_len = 0; }
@@ -159,7 +173,7 @@ struct Attention {
   int hidden_size() const { return num_heads * head_dim; }
 
   // Inference. With a cache: K / V of the T new positions are written at position_start and the
-  // queries attend over cache[0 : position_start + T].
+  // queries attend over cache[0 : position_start + T]; a quantised cache is attended over as it is, with its window and sinks.
   Tensor forward(const Tensor& x, KVLayer* kv = nullptr, int position_start = 0) const {
     const int64_t B = x.shape()[0], T = x.shape()[1];
     const int H = num_heads, Hk = num_kv_heads, D = head_dim;
@@ -172,6 +186,10 @@ struct Attention {
     }
     ops::apply_rope_inplace(q, position_start, rope_theta, rope_scaling);
     ops::apply_rope_inplace(k, position_start, rope_theta, rope_scaling);
+    if (kv != nullptr && kv->quantized.defined()) {
+      ops::write_kv_quantized(kv->quantized, k, v, position_start);
+      return o_proj.forward(ops::attention_quantized(q, kv->quantized, position_start).reshape({B, T, static_cast<int64_t>(H) * D}));
+    }
     int64_t L = T;
     Tensor keys, values;   // [B, H, L, D]
     if (kv != nullptr) {

@@ -398,6 +398,110 @@ inline Tensor read_kv_expanded(const Tensor& cache, int valid_len, int group) {
   return out;
 }
 
+// A cache held in 4 or 8 bits (the format of ctdk_kvq_write) in place of the fp32 one: written as it is filled, attended over
+// as it is. The reference has no counterpart. Inference only, like the fp32 cache: nothing is recorded on the tape.
+struct QuantizedKV {
+  Tensor k_codes, v_codes;     // int32 [B, H_kv, capacity, D * bits / 32], 32 / bits codes each
+  Tensor k_scales, v_scales;   // bf16 [B, H_kv, capacity, D / 32]
+  int bits = 0;                // 4 or 8; 0: there is no cache
+  int64_t window = 0;          // how far back a query sees (0: to the start), and the first positions, which all queries see
+  int64_t sinks = 0;
+
+  bool defined() const { return bits != 0; }
+  int64_t batch() const { return k_codes.shape()[0]; }
+  int num_kv_heads() const { return static_cast<int>(k_codes.shape()[1]); }
+  int64_t capacity() const { return k_codes.shape()[2]; }
+  int head_dim() const { return static_cast<int>(k_scales.shape()[3]) * 32; }
+
+  // Room for max_seq positions, rounded up to a multiple of 64.
+  static QuantizedKV allocate(int num_kv_heads, int head_dim, int64_t batch, int64_t max_seq, int bits, Device device, int64_t window = 0,
+                              int64_t sinks = 0) {
+    if (!device.is_cuda()) throw std::runtime_error("QuantizedKV: CUDA only");
+    if (bits != 4 && bits != 8) throw std::runtime_error("QuantizedKV: bits must be 4 or 8");
+    if (head_dim != 64 && head_dim != 128) throw std::runtime_error("QuantizedKV: head_dim must be 64 or 128");
+    if (num_kv_heads <= 0 || batch < 0 || max_seq <= 0) throw std::runtime_error("QuantizedKV: num_kv_heads and max_seq must be > 0, batch >= 0");
+    if (window < 0 || sinks < 0) throw std::runtime_error("QuantizedKV: window and sinks must be >= 0");
+    const int64_t cap = (max_seq + 63) / 64 * 64;
+    QuantizedKV c;
+    c.k_codes = Tensor::zeros({batch, num_kv_heads, cap, head_dim * bits / 32}, DType::kInt32, device);
+    c.v_codes = Tensor::zeros({batch, num_kv_heads, cap, head_dim * bits / 32}, DType::kInt32, device);
+    c.k_scales = Tensor::zeros({batch, num_kv_heads, cap, head_dim / 32}, DType::kBFloat16, device);
+    c.v_scales = Tensor::zeros({batch, num_kv_heads, cap, head_dim / 32}, DType::kBFloat16, device);
+    c.bits = bits;
+    c.window = window;
+    c.sinks = sinks;
+    return c;
+  }
+  ctdk_kvq_cache desc() const {
+    ctdk_kvq_cache d;
+    d.k_codes = const_cast<void*>(k_codes.data_ptr());
+    d.k_scales = const_cast<void*>(k_scales.data_ptr());
+    d.v_codes = const_cast<void*>(v_codes.data_ptr());
+    d.v_scales = const_cast<void*>(v_scales.data_ptr());
+    d.B = batch();
+    d.capacity = capacity();
+    d.Hk = num_kv_heads();
+    d.D = head_dim();
+    d.bits = bits;
+    return d;
+  }
+};
+
+namespace detail {
+inline int kvq_type(DType dt, const char* op) {
+  if (dt != DType::kFloat32 && dt != DType::kBFloat16) throw std::runtime_error(std::string(op) + ": fp32 or bf16 only");
+  return dt == DType::kFloat32 ? CTDK_DTYPE_F32 : CTDK_DTYPE_BF16;
+}
+inline void kvq_rows(const QuantizedKV& cache, const Tensor& x, int64_t pos, const char* op) {
+  if (!cache.defined()) throw std::runtime_error(std::string(op) + ": the cache is not allocated");
+  kvq_type(x.dtype(), op);
+  if (!x.device().is_cuda() || !x.is_contiguous()) throw std::runtime_error(std::string(op) + ": CUDA / contiguous only");
+  if (x.dim() != 4) throw std::runtime_error(std::string(op) + ": expected [B, T, H, D]");
+  if (x.shape()[0] != cache.batch() || x.shape()[3] != cache.head_dim()) throw std::runtime_error(std::string(op) + ": cache / input dim mismatch");
+  if (pos < 0 || pos + x.shape()[1] > cache.capacity()) throw std::runtime_error(std::string(op) + ": positions outside the cache");
+}
+}  // namespace detail
+
+// k, v [B, T, H_kv, D] become positions pos .. pos + T - 1.
+inline void write_kv_quantized(QuantizedKV& cache, const Tensor& k, const Tensor& v, int64_t pos) {
+  detail::kvq_rows(cache, k, pos, "write_kv_quantized");
+  detail::kvq_rows(cache, v, pos, "write_kv_quantized");
+  if (k.dtype() != v.dtype() || k.shape() != v.shape()) throw std::runtime_error("write_kv_quantized: k / v mismatch");
+  if (k.shape()[2] != cache.num_kv_heads()) throw std::runtime_error("write_kv_quantized: cache / src dim mismatch");
+  const ctdk_kvq_cache d = cache.desc();
+  const int64_t T = k.shape()[1], row = k.shape()[2] * k.shape()[3];
+  detail::ctdk_ok(ctdk_kvq_write(&d, k.data_ptr(), v.data_ptr(), detail::kvq_type(k.dtype(), "write_kv_quantized"), row, T * row, T, nullptr, pos,
+                                 nullptr, nullptr));
+}
+// The first valid_len positions, each KV head `group` times: k, v [B, H_kv * group, valid_len, D].
+inline std::pair<Tensor, Tensor> read_kv_quantized(const QuantizedKV& cache, int64_t valid_len, int group, DType dtype = DType::kFloat32) {
+  if (!cache.defined()) throw std::runtime_error("read_kv_quantized: the cache is not allocated");
+  const int type = detail::kvq_type(dtype, "read_kv_quantized");
+  if (valid_len < 0 || valid_len > cache.capacity()) throw std::runtime_error("read_kv_quantized: valid_len out of range");
+  if (group <= 0) throw std::runtime_error("read_kv_quantized: group must be > 0");
+  const std::vector<int64_t> shape = {cache.batch(), static_cast<int64_t>(cache.num_kv_heads()) * group, valid_len, cache.head_dim()};
+  std::pair<Tensor, Tensor> out = {Tensor::empty(shape, dtype, cache.k_codes.device()), Tensor::empty(shape, dtype, cache.k_codes.device())};
+  const ctdk_kvq_cache d = cache.desc();
+  detail::ctdk_ok(ctdk_kvq_read(&d, 0, valid_len, group, type, out.first.data_ptr(), out.second.data_ptr(), nullptr));
+  return out;
+}
+// q [B, T, H, D] at positions pos .. pos + T - 1 -> [B, T, H, D]: softmax(scale q k^T) v over the positions that the causal
+// mask and the cache's window and sinks let each query see. scale 0: 1 / sqrt(D).
+inline Tensor attention_quantized(const Tensor& q, const QuantizedKV& cache, int64_t pos, float scale = 0.0f) {
+  detail::kvq_rows(cache, q, pos, "attention_quantized");
+  const int64_t T = q.shape()[1], H = q.shape()[2], D = q.shape()[3];
+  if (H == 0 || H % cache.num_kv_heads() != 0) throw std::runtime_error("attention_quantized: heads must be a multiple of kv heads");
+  const ctdk_kvq_cache d = cache.desc();
+  const int64_t bytes = ctdk_kvq_attn_workspace_bytes(&d, T, static_cast<int>(H));
+  if (bytes < 0) throw std::runtime_error(std::string("attention_quantized: ") + ctdk_last_error());
+  Tensor out = Tensor::empty(q.shape(), q.dtype(), q.device());
+  Tensor work = Tensor::empty({(bytes + 3) / 4}, DType::kInt32, q.device());
+  detail::ctdk_ok(ctdk_kvq_attn(&d, q.data_ptr(), detail::kvq_type(q.dtype(), "attention_quantized"), H * D, T * H * D, T, static_cast<int>(H), nullptr,
+                                pos, nullptr, cache.window, cache.sinks, scale != 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(D)),
+                                out.data_ptr(), bytes != 0 ? work.data_ptr() : nullptr, bytes, nullptr));
+  return out;
+}
+
 // ---- loss.h ---------------------------------------------------------------------------------
 inline Tensor mse_loss_impl(const Tensor& pred, const Tensor& target) {
   detail::need_f32_cuda(pred, "mse_loss");
