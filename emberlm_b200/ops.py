@@ -319,6 +319,7 @@ class KvqCache:
             raise RuntimeError("KvqCache: capacity must be a multiple of 64")
         self.tensors = (k_codes, k_scales, v_codes, v_scales)
         self.device, self.B, self.Hk, self.capacity, self.D, self.bits = k_codes.device, B, Hk, capacity, D, row * 8 // D
+        self.index = self.device.index if self.device.index is not None else -1
         self.desc = lib.KvqCacheDesc(*(t.data_ptr() for t in self.tensors), B, capacity, Hk, D, self.bits)
         self.ref = C.addressof(self.desc)
 
@@ -346,10 +347,11 @@ def _kvq_rows(x, name, cache, heads):
         raise RuntimeError(f"{name}: expected a tensor on {cache.device}")
     if x.dim() != 4 or x.shape[0] != cache.B or x.shape[3] != cache.D or (heads and x.shape[2] != heads):
         raise RuntimeError(f"{name}: expected [B, T, heads, D] that fits the cache")
+    B, T, H, D = x.shape
     sb, st, sh, sd = x.stride()
-    if x.numel() and ((sd != 1) or (sh != cache.D and x.shape[2] > 1)):
+    if (sd != 1 or (sh != D and H > 1)) and x.numel():
         raise RuntimeError(f"{name}: a token's heads must be contiguous")
-    return (st if x.shape[1] > 1 else 0), (sb if x.shape[0] > 1 else 0)
+    return (st if T > 1 else 0), (sb if B > 1 else 0)
 
 
 def _kvq_places(pos, count, cache, name):
@@ -367,8 +369,25 @@ def _kvq_places(pos, count, cache, name):
     return at
 
 
+class _Same:
+    """Stands in for torch.cuda.device where the cache is on the current device already (which costs a token's call less)."""
+
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *error):
+        return False
+
+
+_SAME = _Same()
+
+
+def _kvq_device(cache):
+    return _SAME if torch.cuda.current_device() == cache.index else torch.cuda.device(cache.device)
+
+
 def _kvq_stream(cache):
-    return torch.cuda.current_stream(cache.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(cache.index)
 
 
 def kvq_write(cache, k, v, pos, count=None):
@@ -378,7 +397,7 @@ def kvq_write(cache, k, v, pos, count=None):
     if v.shape != k.shape or v.dtype != k.dtype or _kvq_rows(v, "kvq_write", cache, cache.Hk) != strides:
         raise RuntimeError("kvq_write: k and v must have the same shape, type and strides")
     p, at, n = _kvq_places(pos, count, cache, "kvq_write")
-    with torch.cuda.device(cache.device):
+    with _kvq_device(cache):
         lib.call("ctdk_kvq_write", cache.ref, k.data_ptr(), v.data_ptr(), _KVQ_DTYPES[k.dtype], *strides, k.shape[1], p, at, n, _kvq_stream(cache))
 
 
@@ -390,7 +409,7 @@ def kvq_read(cache, start, length, group=1, dtype=torch.float32):
         raise RuntimeError("kvq_read: positions out of range, or a group below 1")
     out = torch.empty(2, cache.B, cache.Hk * group, length, cache.D, device=cache.device, dtype=dtype)
     k, v = out[0], out[1]
-    with torch.cuda.device(cache.device):
+    with _kvq_device(cache):
         lib.call("ctdk_kvq_read", cache.ref, start, length, group, _KVQ_DTYPES[dtype], k.data_ptr(), v.data_ptr(), _kvq_stream(cache))
     return k, v
 
@@ -404,7 +423,7 @@ def kvq_attention(q, cache, pos, count=None, window=0, sinks=0, scale=None):
     if H == 0 or H % cache.Hk:
         raise RuntimeError("kvq_attention: heads must be a multiple of kv heads")
     p, at, n = _kvq_places(pos, count, cache, "kvq_attention")
-    with torch.cuda.device(cache.device):
+    with _kvq_device(cache):
         out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         need = lib.raw().ctdk_kvq_attn_workspace_bytes(cache.ref, T, H)
         work = torch.empty(need, device=q.device, dtype=torch.uint8) if need > 0 else None
