@@ -4,6 +4,9 @@
 // A thread takes sixteen neighbouring values, two threads a group; a row's threads are neighbours and consecutive rows
 // are consecutive positions of one head, so that the cache side is contiguous and the other side comes in whole head
 // rows of 128 to 512 bytes. (With eight values a thread the index arithmetic, not memory, was the limit.)
+// Measured (B200, copy bandwidth 6.45 TB/s): 4 x 4096 rows of 8 x 128, keys and values: bfloat16 to 4 bits 29 us (86 MB each way,
+// 3.0 TB/s), back 18 us (4.7 TB/s); fp32 to 8 bits 28 us (6.1 TB/s), back 33 us (5.1 TB/s). Writing 4 bits is bound by
+// the exact rounding (a quotient with its remainder a value), the others by memory.
 #include "kv_quant.cuh"
 
 namespace ctdk {

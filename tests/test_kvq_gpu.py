@@ -382,3 +382,51 @@ def test_refusals(K):
     for f in bad:
         with pytest.raises(RuntimeError):
             f()
+
+
+# ---- what long sums cost, and prompts as they are replayed ----------------------------------------
+@pytest.mark.parametrize("bits,D", [(4, 128), (8, 64)])
+@pytest.mark.parametrize("T,H", [(1, 4), (2, 8), (3, 48)])
+def test_fp32_sums_over_long_rows(K, bits, D, T, H):
+    """Values of one sign, so that what the tensor cores cut off an accumulator (2^-23 of it at most, every sum) adds up. An
+    accumulator takes 64 sums at most (four tiles of 128 positions, 16 a product, in two terms) before fp32 addition takes over;
+    probabilities and scores in two terms leave 2^-20. Sums kept in one accumulator would be off by up to 2048 * 2^-23."""
+    n, Hk = 16384, 1
+    cache = K.kvq_cache(1, Hk, n, D, bits)
+    v = 1 + 0.05 * rnd((1, n, Hk, D), 131)
+    K.kvq_write(cache, rnd((1, n, Hk, D), 132, 0.05).cuda(), v.cuda(), 0)
+    q = rnd((1, T, H, D), 133)
+    got = K.kvq_attention(q.cuda(), cache, n - T).double().cpu().numpy()
+    kk, vv = host_values(cache, n)
+    want, _ = R.attention(q[0].double().numpy(), kk[0], vv[0], n - T, T)
+    assert np.linalg.norm(got[0] - want) <= (64 * 2.0 ** -23 + 2.0 ** -20) * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_prompts_replayed_and_on_two_streams(K, dtype):
+    """A captured prompt follows positions and counts on the device; two graphs' prompts run at once with a workspace each."""
+    B, T, H, Hk, D = 2, 70, 6, 2, 64
+    caches = [filled(K, B, Hk, 1200, D, bits, 141, capacity=1280) for bits in (4, 8)]
+    q = rnd((B, T, H, D), 142, dtype=dtype).cuda()
+    pos = torch.tensor([0, 900], dtype=torch.int32, device="cuda")
+    count = torch.tensor([70, 9], dtype=torch.int32, device="cuda")
+    streams, graphs, outs = [torch.cuda.Stream() for _ in caches], [], []
+    for c in caches:
+        K.kvq_attention(q, c, pos, count=count)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(K.kvq_attention(q, c, pos, count=count))
+        graphs.append(g)
+    for i in range(3):
+        pos.copy_(torch.tensor([60 * i, 900 + i], dtype=torch.int32))
+        count.copy_(torch.tensor([70 - 30 * i, 9 + 20 * i], dtype=torch.int32))
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for s, g in zip(streams, graphs):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for c, out in zip(caches, outs):
+            want = check(K, c, q, pos.tolist(), count.tolist())
+            assert np.array_equal(out.double().cpu().numpy(), want)
