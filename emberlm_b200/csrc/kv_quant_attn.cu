@@ -939,8 +939,11 @@ int64_t most_tiles(const AttnArgs& a, int D, int bits) {
   if (a.window > 0) n = min(n, static_cast<int64_t>(a.window) + a.T + a.sinks + 3 * keys);
   return (n + keys - 1) / keys;
 }
-// Whether the work is split over all SMs: not where a unit's tiles are few, for which the second launch costs more than it saves.
-bool split_wanted(int64_t rows, int64_t tiles) { return rows <= 16 && tiles > 2 * kWarps; }
+// Whether the work is split over all SMs: not where a unit has few tiles, for which the shares' beginnings and the second launch cost more
+// than they save. Split and unsplit, us, 8 bits, 8 x 128, two fp32 rows a head: one sequence of 15, 35, 49, 98 tiles 12.4 / 7.2,
+// 9.9 / 9.8, 10.5 / 12.2, 12.6 / 20.6; 32 sequences 18.3 / 9.7, 23.1 / 14.2, 25.8 / 17.7, 38.0 / 32.1 (which sequences there
+// are is not known on the host, and one long one among them has to be split: a unit's tiles decide, not their number in all).
+bool split_wanted(int64_t rows, int64_t tiles) { return rows <= 16 && tiles > 5 * kWarps; }
 
 template <typename QT, int D, int BITS, int NT>
 int launch_token(const TokenArgs& ta, int ctas, cudaStream_t s) {
@@ -1033,7 +1036,8 @@ int ctdk_kvq_attn(const ctdk_kvq_cache* cache, const void* q, int dtype, int64_t
   a.status = device_status_word();
   if (a.status == nullptr) return fail(CTDK_ELAUNCH, "kvq_attn: no status word");
   const int64_t rows = T * a.group, units = cache->B * cache->Hk;
-  // More rows than two tiles of mma.sync take: the prompt kernel, whose tiles have 128.
+  // More rows than two tiles of mma.sync take (a third one's sums leave no registers): the prompt kernel, whose tiles have 128. 16 rows here,
+  // 20 there, us, 8 heads of 64: one sequence of 2048 positions in 4 bits 25 / 19, eight of 16384 46 / 97.
   if (rows > 16) {
     const int64_t need = kvq::attn_tc_bytes(cache->B, cache->Hk, cache->D, rows);
     CTDK_REQUIRE(need == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= need),
