@@ -994,6 +994,7 @@ extern "C" {
 int64_t ctdk_kvq_attn_workspace_bytes(const ctdk_kvq_cache* cache, int64_t T, int H) {
   if (const int rc = kvq::check_cache(cache, "kvq_attn"); rc != CTDK_OK) return rc;
   CTDK_REQUIRE(T >= 0 && H > 0 && H % cache->Hk == 0, "kvq_attn: heads must be a multiple of kv heads");
+  if (T == 0 || cache->B == 0) return 0;
   const int64_t rows = T * (H / cache->Hk);
   return rows <= 16 ? kvq::part_bytes(cache->D, rows) : kvq::attn_tc_bytes(cache->B, cache->Hk, cache->D, rows);
 }

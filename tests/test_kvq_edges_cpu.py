@@ -1,0 +1,33 @@
+"""The quantised cache at the edges of what its calls take, as far as that needs no GPU."""
+import ctypes as C
+import subprocess
+import sys
+
+import pytest
+
+from emberlm_b200 import lib
+
+
+def desc(**k):
+    a = dict(k_codes=4096, k_scales=4096, v_codes=4096, v_scales=4096, B=2, capacity=128, Hk=2, D=64, bits=4)
+    a.update(k)
+    return lib.KvqCacheDesc(**a)
+
+
+@pytest.mark.parametrize("T,H", [(1, 4), (8, 4), (9, 4), (64, 4), (1, 64), (0, 4)])
+def test_an_empty_batch_needs_nothing(T, H):
+    """In a process of its own: a division by the number of rows would end it."""
+    code = (f"import ctypes as C; from emberlm_b200 import lib; L = lib.raw()\n"
+            f"d = lib.KvqCacheDesc(B=0, capacity=128, Hk=2, D=64, bits=4); p = C.addressof(d)\n"
+            f"assert L.ctdk_kvq_attn_workspace_bytes(p, {T}, {H}) == 0\n"
+            f"assert L.ctdk_kvq_attn(p, None, 0, 0, 0, {T}, {H}, None, 0, None, 0, 0, 0.125, None, None, 0, None) == 0\n"
+            f"assert L.ctdk_kvq_write(p, None, None, 0, 0, 0, {T}, None, 0, None, None) == 0\n"
+            f"assert L.ctdk_kvq_read(p, 0, 8, 1, 0, None, None, None) == 0\n")
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0, (res.returncode, res.stderr[-2000:])
+
+
+def test_no_rows_need_no_workspace():
+    d = desc()
+    assert lib.raw().ctdk_kvq_attn_workspace_bytes(C.addressof(d), 0, 4) == 0
+    assert lib.raw().ctdk_kvq_attn_workspace_bytes(C.addressof(d), 0, 64) == 0
