@@ -42,7 +42,9 @@ static_assert(kRegsLead + 2 * kRegsSoft + 2 * kRegsMake == 5 * 96, "an increase 
 // fp32 outputs: the tensor cores cut sums off rather than round them, which over a long row cost 1e-5. O is summed there over this
 // many tiles, and the sums of those are added in fp32, in memory that stays in L2 (registers and tensor memory are full).
 constexpr int kTogether = 4;
-constexpr int kRing = 4;                 // tiles whose exponents and NaN marks are kept
+// Tiles whose exponents and NaN marks are kept. Five at least: warp 2 looks keys over up to four tiles ahead of the softmax that reads
+// their factor (the keys' stages go by S alone), values up to three (theirs go by P V, which waits for the softmax).
+constexpr int kRing = 8;
 constexpr int kRoom = 6;                 // powers of two by which values may grow before O is rescaled
 
 template <int D, int BITS>
@@ -161,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
   uint64_t* pv_full = bars + 21;     // O += P(g) V(g) has finished (one phase per step)
   uint64_t* o_full = bars + 22;      // the item's last one has
   uint64_t* looked = bars + 23;      // [2][keys, values]: the scales have been looked over, for the warps that convert
-  uint64_t* told = bars + 27;        // [kRing] the same of values, for the MMA issuer and the softmax behind it (by up to three tiles)
+  uint64_t* told = bars + 27;        // [kRing] the same of values, for the MMA issuer and the softmax behind it
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch();
   if (threadIdx.x == 0) {
