@@ -12,8 +12,10 @@
 //                values (the others) alike.
 //   warp 2       looks a tile's scales over, a tile ahead of those: exponents, NaN. (Warp 3 only fills a warpgroup.)
 // The products take fp16 operands. c * s is not exact in fp16 for every scale s, but c * s * 2^-e is, for the power of two that
-// brings a tile's largest scale near the top of the range, unless a scale is 2^28 times smaller than that one. Keys have an e of
-// their own in every tile (it joins the scores' factor), values one that O is rescaled for when a tile exceeds it. fp32 queries
+// brings a tile's largest scale near the top of the range, unless a scale is far smaller than that one (kSpanK, kSpanV below). Keys have
+// an e of their own in every tile (it joins the scores' factor), values one that O is rescaled for when a tile exceeds it. That one is
+// shared by the item's rows, whichever of them see the largest values; where an item's scales lie too far apart for it, warp 2 marks the
+// item, and its rows are formed once more from the cache in fp32 (exact_rows). fp32 queries
 // enter as two fp16 terms (22 bits), and so do the probabilities of fp32 outputs; those of bfloat16 outputs as one.
 // With A from tensor memory the products read 64 bytes a clock of shared memory; with both operands there they would wait for it.
 // Every mbarrier wait is bounded.
@@ -54,6 +56,9 @@ struct Cfg {
   static constexpr int kTile = kChunks * kChunk;                     // a converted tile
   static constexpr int kSmem = 1024 + 4 * kTile + 4 * kCodes + 4 * kScales;
   static constexpr int kTop = BITS == 4 ? 11 : 7;                    // the largest scale comes to [2^kTop, 2^(kTop + 1))
+  // Powers of two between a tile's scales of keys, an item's of values, up to which all products of codes and scales are exact: fp16 has
+  // multiples of 2^-24, a scale four significant bits (4 bits) or one, and values may start kRoom lower.
+  static constexpr int kSpanK = kTop + (BITS == 4 ? 21 : 24), kSpanV = kSpanK - kRoom;
 };
 
 struct TcArgs {
@@ -61,16 +66,17 @@ struct TcArgs {
   int rows, row_tiles, splits, items;    // T * group; of 128; ranges of an item's tiles; in all
   uint32_t x64;                          // 0x64006400: fp16 1024
   float* total;                          // fp32: gathered sums, [CTA][TQ * D]
+  int* wide;                             // [items] whether an item's scales lie too far apart
 };
 struct Item {
   int b, h, r0, rows, ks, k0, k1;        // tiles k0 .. k1 - 1 of the visit
   int64_t pos, count;
   Visit v;
 };
-__device__ __forceinline__ Item item_at(const TcArgs& ta, int it) {
+__device__ __forceinline__ Item item_at(const TcArgs& ta, int it, int splits) {
   const AttnArgs& a = ta.a;
   Item w;
-  const int ks = it % ta.splits, i = it / ta.splits, units = a.c.B * a.c.Hk, u = i % units, rt = ta.row_tiles - 1 - i / units;
+  const int ks = it % splits, i = it / splits, units = a.c.B * a.c.Hk, u = i % units, rt = ta.row_tiles - 1 - i / units;
   w.ks = ks;
   w.b = u / a.c.Hk;
   w.h = u - w.b * a.c.Hk;
@@ -80,10 +86,11 @@ __device__ __forceinline__ Item item_at(const TcArgs& ta, int it) {
   w.count = a.count != nullptr ? min(static_cast<int64_t>(a.count[w.b]), static_cast<int64_t>(a.T)) : a.T;
   const int t0 = w.r0 / a.group, t1 = (w.r0 + w.rows - 1) / a.group;
   w.v = visit_of(w.pos, w.count, t0, t1 - t0 + 1, a.c.capacity, a.window, a.sinks, KT);
-  w.k0 = static_cast<int>(static_cast<int64_t>(w.v.tiles) * ks / ta.splits);
-  w.k1 = static_cast<int>(static_cast<int64_t>(w.v.tiles) * (ks + 1) / ta.splits);
+  w.k0 = static_cast<int>(static_cast<int64_t>(w.v.tiles) * ks / splits);
+  w.k1 = static_cast<int>(static_cast<int64_t>(w.v.tiles) * (ks + 1) / splits);
   return w;
 }
+__device__ __forceinline__ Item item_at(const TcArgs& ta, int it) { return item_at(ta, it, ta.splits); }
 
 __device__ __forceinline__ uint32_t idesc_f16(bool b_mn, int n) {
   return (1u << 4) | (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(TQ >> 4) << 24);
@@ -132,8 +139,168 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, float a, float b, float
   *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(a, b), pack_bf16(c, d));
 }
 
+__device__ __forceinline__ void store1(float* p, float x) { *p = x; }
+__device__ __forceinline__ void store1(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+
+// Rows r0 .. end - 1 of an item, by one warp, N at a time, from the codes and scales in the cache, in fp32 throughout: a lane a position
+// for the scores, a lane D / 32 columns for the output. For items whose scales no single power of two brings into fp16's range: right
+// for every scale, and slow (2048 fp32 rows of 16 heads of 128 after 6144 positions, all of them: 29 ms).
+template <typename QT, int D, int BITS, int N>
+__device__ __forceinline__ void exact_rows(const TcArgs& ta, const Item& w, int r0, int end, int lane) {
+  using C = Cfg<D, BITS>;
+  constexpr int kOwn = D / 32, kBias = 1 << (BITS - 1), kMask = (1 << BITS) - 1, kWords = kGroup * BITS / 32, kAtOnce = 8;
+  const AttnArgs& a = ta.a;
+  const int64_t base = (static_cast<int64_t>(w.b) * a.c.Hk + w.h) * a.c.capacity;
+  const int col = lane * kOwn;
+  auto scale_of = [](uint32_t bits) { return is_nan_scale(bits) ? __int_as_float(0x7fc00000) : __uint_as_float(bits << 16); };
+  const unsigned short* k_scales = reinterpret_cast<const unsigned short*>(a.c.scales[0]);
+  const unsigned short* v_scales = reinterpret_cast<const unsigned short*>(a.c.scales[1]);
+#pragma unroll 1
+  for (; r0 < end; r0 += N) {
+    const QT* q[N];
+    int at[N], last = -1;
+    float m[N], l[N], o[N][kOwn];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int r = w.r0 + min(r0 + n, end - 1), t = r / a.group, hg = r - t * a.group;   // (rows past the end: the last one again)
+      at[n] = row_position(w.pos, w.count, t, a.c.capacity);
+      last = max(last, at[n]);
+      q[n] = static_cast<const QT*>(a.q) + w.b * a.batch_stride + static_cast<int64_t>(t) * a.row_stride + static_cast<int64_t>(w.h * a.group + hg) * D;
+      m[n] = -INFINITY;
+      l[n] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < kOwn; ++c) o[n][c] = 0.0f;
+    }
+#pragma unroll 1
+    for (int k = 4 * w.k0; k < 4 * w.k1; ++k) {
+      const int j0 = w.v.tile_at(k >> 2) * KT + 32 * (k & 3), j = j0 + lane;
+      if (j0 > last) continue;
+      bool mine = false;
+#pragma unroll
+      for (int n = 0; n < N; ++n) mine |= sees(at[n], j, a.window, a.sinks);   // (what a row sees lies in the cache)
+      const uint32_t seen = __ballot_sync(0xffffffffu, mine);
+      if (seen == 0) continue;
+      float x[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) x[n] = 0.0f;
+      if (mine) {
+        const uint4* codes = reinterpret_cast<const uint4*>(a.c.codes[0] + (base + j) * C::kRow);
+#pragma unroll 1
+        for (int g = 0; g < C::kGroups; ++g) {
+          const float s = scale_of(k_scales[(base + j) * C::kGroups + g]);
+          uint32_t word[kWords];
+#pragma unroll
+          for (int i = 0; i < kWords / 4; ++i) {
+            const uint4 c = codes[g * (kWords / 4) + i];
+            word[4 * i] = c.x, word[4 * i + 1] = c.y, word[4 * i + 2] = c.z, word[4 * i + 3] = c.w;
+          }
+          float sum[N];
+#pragma unroll
+          for (int n = 0; n < N; ++n) sum[n] = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kGroup; i += 8) {
+            float v[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              v[c] = static_cast<float>(static_cast<int>(word[(i + c) * BITS / 32] >> ((i + c) * BITS % 32) & kMask) - kBias) * s;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+              float y[8];
+              load8(q[n] + g * kGroup + i, y);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) sum[n] = fmaf(y[c], v[c], sum[n]);
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < N; ++n) x[n] += sum[n];
+        }
+      }
+      float p[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const bool sees_it = mine && sees(at[n], j, a.window, a.sinks);
+        const float z = sees_it ? x[n] * a.scale_log2 : -INFINITY, most = warp_max(z);
+        if (most > m[n]) {
+          const float f = ex2(m[n] - most);
+          m[n] = most;
+          l[n] *= f;
+#pragma unroll
+          for (int c = 0; c < kOwn; ++c) o[n][c] *= f;
+        }
+        p[n] = sees_it ? ex2(z - (m[n] == -INFINITY ? 0.0f : m[n])) : 0.0f;
+        l[n] += warp_sum(p[n]);
+      }
+      float sum[N][kOwn];
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c) sum[n][c] = 0.0f;
+#pragma unroll 1
+      for (int i0 = 0; i0 < 32; i0 += kAtOnce) {
+        float v[kAtOnce][kOwn];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+          const bool there = (seen >> (i0 + i) & 1u) != 0;
+          const int64_t row = base + j0 + (there ? i0 + i : __ffs(seen) - 1);
+          const float s = scale_of(v_scales[row * C::kGroups + col / kGroup]);
+#pragma unroll
+          for (int c = 0; c < kOwn; ++c)
+            v[i][c] = static_cast<float>(static_cast<int>(a.c.codes[1][row * C::kRow + (col + c) * BITS / 8] >> ((col + c) * BITS % 8) & kMask) - kBias) * s;
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+          for (int n = 0; n < N; ++n) {
+            // (a value that the row does not see may be NaN: it is no part of the sum)
+            const float pi = __shfl_sync(0xffffffffu, p[n], i0 + i);
+            const bool sees_it = sees(at[n], j0 + i0 + i, a.window, a.sinks);
+#pragma unroll
+            for (int c = 0; c < kOwn; ++c) sum[n][c] = sees_it ? fmaf(pi, v[i][c], sum[n][c]) : sum[n][c];
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c) o[n][c] += sum[n][c];
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (r0 + n < end) {
+        const int r = w.r0 + r0 + n, t = r / a.group, hg = r - t * a.group;
+        QT* dst = static_cast<QT*>(a.out) + ((static_cast<int64_t>(w.b) * a.T + t) * a.H + w.h * a.group + hg) * D + col;
+#pragma unroll
+        for (int c = 0; c < kOwn; ++c) store1(dst + c, at[n] >= 0 ? o[n][c] / l[n] : 0.0f);
+      }
+  }
+}
+
+// The marked items of a call without ranges (the join sees to those of a call with ranges): the CTA's own, behind its loop over them, by
+// its softmax warps. A call, not in line, and for fp32 queries over 128 columns a launch of its own: registers that the softmax loses to it
+// cost more there (2048 rows after 6144 positions 330 us, in line 380; a launch 3 us on top of 315. The others: the call 0 to 1 us, a launch 3).
+template <typename QT, int D>
+constexpr bool kOwnLaunch = sizeof(QT) == 4 && D == 128;
+template <typename QT, int D, int BITS, int N>
+__device__ __forceinline__ void exact_items(const TcArgs& ta, int warp) {
+  for (int it = blockIdx.x; it < ta.items; it += gridDim.x)
+    if (ta.wide[it] != 0) {
+      const Item w = item_at(ta, it);
+      exact_rows<QT, D, BITS, N>(ta, w, warp * 16, min(warp * 16 + 16, w.rows), threadIdx.x & 31);
+    }
+}
 template <typename QT, int D, int BITS>
-__global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const TcArgs ta) {
+__device__ __noinline__ void exact_call(const TcArgs* ta) {
+  exact_items<QT, D, BITS, 2>(*ta, static_cast<int>(threadIdx.x >> 5) - kSoft);
+}
+template <typename QT, int D, int BITS>
+__global__ void __launch_bounds__(256) kvq_prompt_exact_kernel(const TcArgs ta) {
+  pdl_launch();
+  pdl_wait();
+  exact_items<QT, D, BITS, 4>(ta, threadIdx.x >> 5);
+}
+
+template <typename QT, int D, int BITS>
+__global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                                                                   const __grid_constant__ TcArgs ta) {
   using C = Cfg<D, BITS>;
   constexpr int NT = sizeof(QT) == 4 ? 2 : 1;          // fp16 terms of a query, of a probability
   constexpr uint32_t kColS = 0, kColO = 2 * KT, kColQ = 2 * KT + 128;
@@ -144,6 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
   __shared__ int exp_k[kRing], exp_v[kRing];           // exponents of a tile's keys and values
   __shared__ float scale_k[kRing], shrink_o[kRing];    // 2^exp_k; what O has to be multiplied by, as exp_v has moved
   __shared__ uint32_t nan_any[kRing];
+  __shared__ int any_wide;                             // of this CTA's items
   __shared__ uint8_t nan_of[kRing][KT];                // groups of values that are NaN, by position
   const AttnArgs& a = ta.a;
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -263,10 +431,11 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
   } else if (warp == 2) {
     // Exponents of a tile's keys and values, and which groups of its values are NaN. What none of the rows sees must not matter.
     uint32_t g = 0;
-    bool ok = true;
+    bool ok = true, marked = false;
     for (int it = blockIdx.x; it < ta.items && ok; it += gridDim.x) {
       const Item w = item_at(ta, it);
-      int vref = 0;
+      int vref = 0, vtop = -1, vlow = 0x7fff;          // (exponents of scales as their bits have them)
+      bool wide = false;
       for (int k = w.k0; k < w.k1 && ok; ++k, ++g) {
         const uint32_t st = g & 1u, ph = (g >> 1) & 1u;
         const int j0 = w.v.tile_at(k) * KT;
@@ -275,31 +444,48 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
           ok = wait_w(&in_full[2 * st + which], ph, a.status, 243);
           if (!ok) break;
           const unsigned char* p = scales_s + (2 * st + which) * C::kScales;
-          uint32_t big = 0, any = 0;
-#pragma unroll
-          for (int i = 0; i < KT / 32; ++i) {
-            const int row = 32 * i + lane, at = j0 + row;
-            const bool seen = at < w.v.hi_row && (at >= w.v.lo_row || a.window == 0 || w.v.lo_row - at < a.window || at < a.sinks);
-            uint32_t sw[C::kGroups / 2], nan = 0, most = 0;
+          // The largest scale and the smallest one that is not zero (less one, so that zero becomes the largest), two a word.
+          auto words = [&](int row, uint32_t (&sw)[C::kGroups / 2]) {
             if constexpr (C::kGroups == 4) {
               const uint2 x = *reinterpret_cast<const uint2*>(p + row * 8);
               sw[0] = x.x, sw[C::kGroups / 2 - 1] = x.y;
             } else {
               sw[0] = *reinterpret_cast<const uint32_t*>(p + row * 4);
             }
+            const int at = j0 + row;
+            return at < w.v.hi_row && (at >= w.v.lo_row || a.window == 0 || w.v.lo_row - at < a.window || at < a.sinks);
+          };
+          uint32_t most = 0, least = 0xffffffffu, any = 0;
 #pragma unroll
-            for (int y = 0; y < C::kGroups; ++y) {
-              const uint32_t b = (y & 1 ? sw[y / 2] >> 16 : sw[y / 2]) & 0x7fffu;
-              if (is_nan_scale(b)) nan |= 1u << y;
-              else most = max(most, b);
+          for (int i = 0; i < KT / 32; ++i) {
+            uint32_t sw[C::kGroups / 2];
+            const bool seen = words(32 * i + lane, sw);
+#pragma unroll
+            for (int y = 0; y < C::kGroups / 2; ++y) {
+              most = __vmaxu2(most, seen ? sw[y] & 0x7fff7fffu : 0u);
+              least = __vminu2(least, seen ? ((sw[y] | 0x80008000u) - 0x00010001u) ^ 0x80008000u : 0xffffffffu);
             }
-            if (!seen) most = nan = 0;
-            big = max(big, most);
-            any |= nan;
-            if (which == 1) nan_of[g % kRing][row] = static_cast<uint8_t>(nan);
           }
-          big = __reduce_max_sync(0xffffffffu, big);
-          any = __any_sync(0xffffffffu, any != 0) ? 1u : 0u;
+          uint32_t big = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
+          if (is_nan_scale(big)) {                     // the largest of the others, and where the NaN are
+            big = 0;
+#pragma unroll 1
+            for (int i = 0; i < KT / 32; ++i) {
+              uint32_t sw[C::kGroups / 2], nan = 0;
+              const bool seen = words(32 * i + lane, sw);
+#pragma unroll
+              for (int y = 0; y < C::kGroups; ++y) {
+                const uint32_t b = (y & 1 ? sw[y / 2] >> 16 : sw[y / 2]) & 0x7fffu;
+                if (is_nan_scale(b)) nan |= 1u << y;
+                else if (seen) big = max(big, b);
+              }
+              if (!seen) nan = 0;
+              any |= nan;
+              if (which == 1) nan_of[g % kRing][32 * i + lane] = static_cast<uint8_t>(nan);
+            }
+            big = __reduce_max_sync(0xffffffffu, big);
+            any = __any_sync(0xffffffffu, any != 0) ? 1u : 0u;
+          }
           const int e = big == 0 ? (which ? -120 : 0) : max(static_cast<int>(big >> 7) - 127 - C::kTop, -120);
           if (which == 0) {
             exp_k[g % kRing] = e;                      // (all lanes: the same)
@@ -321,8 +507,21 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
             mbar_arrive(&looked[2 * st + which]);
             if (which == 1) mbar_arrive(&told[g % kRing]);
           }
+          if (big != 0) {                              // (behind what others wait for)
+            const int top = static_cast<int>(big >> 7), bottom = static_cast<int>((__reduce_min_sync(0xffffffffu, min(least & 0xffffu, least >> 16)) + 1u) >> 7);
+            if (which == 0) wide |= top - bottom > C::kSpanK;
+            else vtop = max(vtop, top), vlow = min(vlow, bottom);
+          }
         }
       }
+      wide |= vtop - vlow > C::kSpanV;
+      marked |= wide;
+      if (lane == 0) ta.wide[it] = wide ? 1 : 0;
+    }
+    if constexpr (!kOwnLaunch<QT, D>) {
+      if (lane == 0) any_wide = ok && marked && ta.splits == 1 ? 1 : 0;
+      __syncwarp();
+      asm volatile("barrier.cta.arrive 5, 288;" ::: "memory");   // with the softmax warps
     }
   }
   } else if (warp < kMake) {
@@ -585,6 +784,10 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
       }
       tc_fence_before();
     }
+    if constexpr (!kOwnLaunch<QT, D>) {
+      asm volatile("barrier.cta.sync 5, 288;" ::: "memory");
+      if (any_wide != 0) exact_call<QT, D, BITS>(&ta);
+    }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMake));
     // Four warps convert keys, four values, each at its own pace. A thread has one position of a tile: its swizzles keep the reads
@@ -667,14 +870,22 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
   }
 }
 
-// Joins the ranges of the items: a CTA takes 16 rows of one, a thread a column (or two rows' columns).
-template <typename QT, int D>
+// Joins the ranges of the items: a CTA takes 16 rows of one, a thread a column (or two rows' columns). A marked one is formed anew.
+template <typename QT, int D, int BITS>
 __global__ void __launch_bounds__(256) kvq_prompt_join_kernel(const TcArgs ta) {
   const AttnArgs& a = ta.a;
   pdl_launch();
   pdl_wait();
   const int i = blockIdx.x / (TQ / 16), units = a.c.B * a.c.Hk, u = i % units, rt = ta.row_tiles - 1 - i / units;
   const int b = u / a.c.Hk, h = u - b * a.c.Hk;
+  bool wide = false;
+  for (int k = 0; k < ta.splits; ++k) wide |= ta.wide[i * ta.splits + k] != 0;
+  if (wide) {
+    const Item w = item_at(ta, i, 1);
+    const int rr = static_cast<int>(blockIdx.x % (TQ / 16)) * 16 + static_cast<int>(threadIdx.x >> 5) * 2;
+    exact_rows<QT, D, BITS, 2>(ta, w, rr, min(rr + 2, w.rows), threadIdx.x & 31);
+    return;
+  }
   const float* part = a.part + static_cast<int64_t>(i) * ta.splits * TQ * (D + 2);
   const int64_t pos = a.pos != nullptr ? static_cast<int64_t>(a.pos[b]) : a.pos_all;
   const int64_t count = a.count != nullptr ? min(static_cast<int64_t>(a.count[b]), static_cast<int64_t>(a.T)) : a.T;
@@ -716,8 +927,15 @@ int launch(const TcArgs& ta, cudaStream_t s) {
   cudaError_t e = raise_dynamic_smem(reinterpret_cast<const void*>(kernel), C::kSmem);
   if (e == cudaSuccess) e = launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), C::kSmem, s, m[0], m[1], ta);
   if (e != cudaSuccess) return fail(CTDK_ELAUNCH, "kvq_attn: %s", cudaGetErrorString(e));
-  if (const int rc = check_launch("kvq_attn"); rc != CTDK_OK || ta.splits == 1) return rc;
-  e = launch_pdl(kvq_prompt_join_kernel<QT, D>, dim3(static_cast<unsigned>(ta.items / ta.splits * (TQ / 16))), dim3(256), 0, s, ta);
+  if (const int rc = check_launch("kvq_attn"); rc != CTDK_OK || (ta.splits == 1 && !kOwnLaunch<QT, D>)) return rc;
+  if constexpr (kOwnLaunch<QT, D>) {
+    if (ta.splits == 1) {
+      e = launch_pdl(kvq_prompt_exact_kernel<QT, D, BITS>, dim3(static_cast<unsigned>(ctas)), dim3(256), 0, s, ta);
+      if (e != cudaSuccess) return fail(CTDK_ELAUNCH, "kvq_attn: %s", cudaGetErrorString(e));
+      return check_launch("kvq_attn");
+    }
+  }
+  e = launch_pdl(kvq_prompt_join_kernel<QT, D, BITS>, dim3(static_cast<unsigned>(ta.items / ta.splits * (TQ / 16))), dim3(256), 0, s, ta);
   if (e != cudaSuccess) return fail(CTDK_ELAUNCH, "kvq_attn: %s", cudaGetErrorString(e));
   return check_launch("kvq_attn");
 }
@@ -728,13 +946,14 @@ int splits_of(int64_t items, int64_t tiles) {
   const int64_t n = want < most ? want : most;
   return n < 1 ? 1 : static_cast<int>(n);
 }
+int64_t wide_ints(int64_t items) { return (items + 3) / 4 * 4; }
 int64_t row_items(int64_t B, int Hk, int64_t rows) { return B * Hk * ((rows + TQ - 1) / TQ); }
 
 }  // namespace
 
 int64_t attn_tc_bytes(int64_t B, int Hk, int D, int64_t rows) {
   const int64_t items = row_items(B, Hk, rows), splits = splits_of(items, INT32_MAX);
-  return static_cast<int64_t>(sm_count()) * TQ * D * 4 + (splits > 1 ? items * splits * TQ * (D + 2) * 4 : 0);
+  return static_cast<int64_t>(sm_count()) * TQ * D * 4 + wide_ints(items * splits) * 4 + (splits > 1 ? items * splits * TQ * (D + 2) * 4 : 0);
 }
 
 int attn_tc(const AttnArgs& a, int dtype, int bits, int D, cudaStream_t s) {
@@ -751,7 +970,8 @@ int attn_tc(const AttnArgs& a, int dtype, int bits, int D, cudaStream_t s) {
   ta.items = static_cast<int>(items * ta.splits);
   ta.x64 = 0x64006400u;
   ta.total = a.part;                                   // (used by fp32 calls)
-  ta.a.part = a.part + static_cast<int64_t>(sm_count()) * TQ * D;
+  ta.wide = reinterpret_cast<int*>(a.part + static_cast<int64_t>(sm_count()) * TQ * D);
+  ta.a.part = reinterpret_cast<float*>(ta.wide + wide_ints(ta.items));
   const bool f32 = dtype == CTDK_DTYPE_F32;
   if (bits == 4) {
     if (D == 64) return f32 ? launch<float, 64, 4>(ta, s) : launch<__nv_bfloat16, 64, 4>(ta, s);

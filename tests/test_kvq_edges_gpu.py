@@ -1,8 +1,10 @@
 """The quantised cache at the edges of what its calls take, on the GPU; against numpy in 64 bits (tests/kvq_ref.py) where there are values."""
+import numpy as np
 import pytest
 import torch
 
-from tests.test_kvq_gpu import K, _status_clean  # noqa: F401  (fixtures)
+from tests import kvq_bounds as B
+from tests.test_kvq_gpu import K, _status_clean, check, rnd  # noqa: F401  (fixtures among them)
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
@@ -15,3 +17,86 @@ def test_an_empty_batch(K, T, H):  # noqa: F811
     K.kvq_write(cache, rows, rows, 0)
     assert K.kvq_attention(torch.empty(0, T, H, 64, device="cuda"), cache, 0).shape == (0, T, H, 64)
     assert K.kvq_read(cache, 0, 8)[0].shape == (0, 2, 8, 64)
+
+
+# ---- values and keys of very different sizes ------------------------------------------------------
+def wrote(K, k, v, bits):  # noqa: F811
+    """A cache of exactly these rows [B, n, Hk, D]; what lies behind them is NaN."""
+    batch, n, Hk, D = k.shape
+    cache = K.kvq_cache(batch, Hk, n, D, bits)
+    for i in (0, 2):
+        cache.tensors[i].fill_(0xFF)
+        cache.tensors[i + 1].fill_(float("nan"))
+    K.kvq_write(cache, k.cuda(), v.cuda(), 0)
+    return cache
+
+
+SHAPES = [(1, 4, 2, 64), (3, 4, 2, 128), (40, 4, 2, 64), (129, 2, 2, 128), (150, 3, 1, 64)]   # T, H, Hk, D
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,H,Hk,D", SHAPES)
+@pytest.mark.parametrize("lo,hi", [(-30, 30), (30, -30), (0, 20), (20, 0), (-90, 0)])
+def test_values_that_grow_and_shrink_along_the_sequence(K, bits, dtype, T, H, Hk, D, lo, hi):  # noqa: F811
+    """By powers of two that fit one range of fp16 (the sums are rescaled on the way) and by ones that do not."""
+    n = 600
+    k, v = rnd((1, n, Hk, D), 11, 0.3), rnd((1, n, Hk, D), 12)
+    v = v * torch.exp2(torch.linspace(lo, hi, n).round()).reshape(1, n, 1, 1)
+    cache, q = wrote(K, k, v, bits), rnd((1, T, H, D), 13, 1.0, dtype).cuda()
+    check(K, cache, q, n - T)
+    check(K, cache, q, 0, n=n)
+    check(K, cache, q, 300 - T // 2, window=90, sinks=3, n=n)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("power", [20, 24, 25, 26, 27, 28, 40, 97])
+def test_a_row_does_not_depend_on_sizes_that_it_cannot_see(K, bits, dtype, power):  # noqa: F811
+    """One group of values, then one of keys, far larger than the others: the rows before it, and the ones whose window has left it,
+    are as without it."""
+    n, H, Hk, D, at = 256, 4, 2, 64, 100
+    q = rnd((1, n, H, D), 21, 1.0, dtype).cuda()
+    for which in (0, 1):
+        x = [rnd((1, n, Hk, D), 22, 0.5), rnd((1, n, Hk, D), 23)]
+        plain = wrote(K, *x, bits)
+        x[which][0, at, 1, 32:] *= 2.0 ** power
+        cache = wrote(K, *x, bits)
+        for window, sinks in ((0, 0), (40, 2)):
+            got = B.compare(K, cache, q, 0, window=window, sinks=sinks)
+            want = K.kvq_attention(q, plain, 0, window=window, sinks=sinks).double().cpu().numpy()
+            blind = [t for t in range(n) if t < at or (window and t >= at + window)]
+            # both are within that bound of the same numbers; what they may differ by is twice that, and 2^-8 (2^-15) is more
+            tol = 2.0 ** -7 if dtype == BF16 else 2.0 ** -14
+            assert np.abs(got[0, blind] - want[0, blind]).max() <= tol * np.abs(want).max()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,H,Hk,D", SHAPES)
+def test_keys_of_all_sizes(K, bits, dtype, T, H, Hk, D):  # noqa: F811
+    """Positions whose keys are far larger, in columns in which the queries are zeros: their scores come from the small ones."""
+    n = 500
+    k, v = rnd((2, n, Hk, D), 31, 0.5), rnd((2, n, Hk, D), 32)
+    q = rnd((2, T, H, D), 33, 1.0, dtype)
+    q[..., 32:] = 0
+    k[:, ::3, :, 32:] *= 2.0 ** 50
+    k[:, 1::7, :, 32:] *= 2.0 ** -60
+    cache = wrote(K, k, v, bits)
+    check(K, cache, q.cuda(), [n - T, 100], n=n)
+    check(K, cache, q.cuda(), [n - T, 200], [T, T // 2], window=130, sinks=2, n=n)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_sizes_that_differ_beside_split_work_and_nan(K, bits, dtype):  # noqa: F811
+    """Few row tiles over a long cache (parts that are joined), some sequences even and some not, and a NaN on top."""
+    n, T, H, Hk, D = 3000, 20, 2, 1, 64
+    k, v = rnd((3, n, Hk, D), 41, 0.3), rnd((3, n, Hk, D), 42)
+    v[1] *= torch.exp2(torch.linspace(-40, 40, n).round()).reshape(n, 1, 1)
+    v[2, 1500, 0, :32] *= 2.0 ** 60
+    v[2, 2990, 0, 40] = float("nan")
+    cache = wrote(K, k, v, bits)
+    q = rnd((3, T, H, D), 43, 1.0, dtype).cuda()
+    check(K, cache, q, n - T)
+    check(K, cache, q, [n - T, 1495, 2400], [T, 11, T], n=n)
