@@ -14,7 +14,11 @@
 //            by more than 2^8, so that most tiles need one vote instead of a reduction over the warp;
 //   output   O^T[16 columns, 8 rows] += V^T P^T: ldmatrix.trans pairs the codes of two positions, which become c * s in bfloat16; P
 //            comes from the scores' fragments by an 8 x 8 transposition (movmatrix). For fp32 outputs it enters as three bfloat16
-//            terms (24 bits), for bfloat16 outputs as one.
+//            terms (24 bits), for bfloat16 outputs as two: with one, the error of its rounding is as large as the output's own
+//            (2.3e-3 of the outputs' size against 1.65e-3). Up to four rows leave half of a tile of eight empty, and the second terms
+//            go there (FOLDED): row r + 4 has the query of row r, and so its probabilities, of which it keeps what the first term
+//            leaves over; a second product costs 4 to 10 %
+//            (32 ragged sequences of up to 32768 of 8 x 128 in 4 bits 168 -> 184 us; in the empty rows 170).
 // The floor is the cache's codes and scales, once. All tiles of all blocks lie on one line, which the CTAs cut into equal parts, so
 // that one long sequence keeps all SMs busy as a large batch does; blocks that were cut are joined by a second, small kernel.
 // Measured (B200, copy bandwidth 6.45 TB/s): 131072 positions of 8 x 64 in 8 bits, four fp32 rows a head, 143 MB: 45 us, 49 % of that
@@ -292,12 +296,14 @@ struct Part {
   static constexpr int kRows = 8 * NT, kFloats = kRows * (D + 2);
 };
 
-template <typename QT, int D, int BITS, int NT>
+template <typename QT, int D, int BITS, int NT, bool FOLDED>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
     kvq_token_kernel(const __grid_constant__ Maps maps, const TokenArgs ta) {
   using TL = Tile<D, BITS>;
   constexpr int KEYS = TL::kKeys, BLOCKS = KEYS / 16, GROUPS = D / kGroup, STEPS = D / 16, ROW = TL::kRow;
-  constexpr int NQ = sizeof(QT) == 4 ? 2 : 1, NP = sizeof(QT) == 4 ? 3 : 1;   // terms of a query, of a probability
+  constexpr int NQ = sizeof(QT) == 4 ? 2 : 1, NP = sizeof(QT) == 4 ? 3 : 2;   // terms of a query, of a probability
+  constexpr int NB = FOLDED ? 1 : NP;                  // products that the terms of a probability take
+  static_assert(!FOLDED || (NT == 1 && NP == 2), "two terms in a tile of eight rows");
   constexpr int SW = GROUPS / 2;                       // words of a position's scales
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t full[kStages], empty[kStages];
@@ -421,9 +427,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
     constexpr int kPer = D / 4, kAtOnce = kWarps * 32 / kPer;   // threads of a row: 16 or 32
 #pragma unroll 1
     for (int rr = static_cast<int>(threadIdx.x) / kPer; rr < 8 * NT; rr += kAtOnce) {
-      const int n = rr / 8, c4 = static_cast<int>(threadIdx.x) % kPer, r = r0 + rr;
+      const int n = rr / 8, c4 = static_cast<int>(threadIdx.x) % kPer, from = FOLDED ? rr & 3 : rr, r = r0 + from;
       float x[4] = {};
-      if (rr < rows) {
+      if (from < rows) {
         const int t = r / a.group;
         load_row<4>(static_cast<const QT*>(a.q) + ub * a.batch_stride + static_cast<int64_t>(t) * a.row_stride +
                         static_cast<int64_t>(uh * a.group + (r - t * a.group)) * D + 4 * c4, x);
@@ -491,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int r = 8 * n + 2 * tig + c;
+        const int r = FOLDED ? (2 * tig + c) & 3 : 8 * n + 2 * tig + c;
         at_row[n][c] = r < rows ? row_position(pos, count, (r0 + r) / a.group, a.c.capacity) : -1;
         m[n][c] = -INFINITY;
         l[n][c] = 0.0f;
@@ -623,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
         for (int c = 0; c < 2; ++c) ref[n][c] = m[n][c] == -INFINITY ? 0.0f : m[n][c];
 #pragma unroll
       for (int k = 0; k < BLOCKS; ++k) {
-        uint32_t pf[NT][NP][2];
+        uint32_t pf[NT][NB][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float p[4];
@@ -635,8 +641,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
           for (int hf = 0; hf < 2; ++hf) {
             uint32_t tt[NP];
             terms_bf16<NP>(p[2 * hf], p[2 * hf + 1], tt);
+            if constexpr (FOLDED) {
+              pf[n][0][hf] = movmatrix(tig < 2 ? tt[0] : tt[1]);
+            } else {
 #pragma unroll
-            for (int y = 0; y < NP; ++y) pf[n][y][hf] = movmatrix(tt[y]);
+              for (int y = 0; y < NP; ++y) pf[n][y][hf] = movmatrix(tt[y]);
+            }
           }
         }
         uint32_t s2[2][GROUPS];                        // scales of positions (2 tig, 2 tig + 1) and (2 tig + 8, 2 tig + 9)
@@ -663,8 +673,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
         auto product = [&](int i, const uint32_t (&f)[4]) {
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            if constexpr (NP == 1) {
-              mma_bf16(o[n][i], f, pf[n][0][0], pf[n][0][1]);
+            if constexpr (NP == 2) {
+#pragma unroll
+              for (int y = NB - 1; y >= 0; --y) mma_bf16(o[n][i], f, pf[n][y][0], pf[n][y][1]);
             } else {
               float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -784,7 +795,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
         for (int w = 0; w < kWarps; ++w) {
           const float f = ex2(row_m[w][rr] - rf);
           ll += f * row_l[w][rr];
-          sum += f * exchange[(w * 8 + r) * TL::kPitch + e];
+          float x = exchange[(w * 8 + r) * TL::kPitch + e];
+          if constexpr (FOLDED) x += exchange[(w * 8 + r + 4) * TL::kPitch + e];
+          sum += f * x;
         }
         // the column that lane e & 7 had in half (e >> 3) & 1 of tile e >> 4
         const int ti = e >> 4, gi = e & 7, hf = (e >> 3) & 1;
@@ -945,11 +958,11 @@ int64_t most_tiles(const AttnArgs& a, int D, int bits) {
 // are is not known on the host, and one long one among them has to be split: a unit's tiles decide, not their number in all).
 bool split_wanted(int64_t rows, int64_t tiles) { return rows <= 16 && tiles > 5 * kWarps; }
 
-template <typename QT, int D, int BITS, int NT>
+template <typename QT, int D, int BITS, int NT, bool FOLDED = false>
 int launch_token(const TokenArgs& ta, int ctas, cudaStream_t s) {
   using TL = Tile<D, BITS>;
   constexpr int kSmem = TL::kSmem;
-  auto* kernel = kvq_token_kernel<QT, D, BITS, NT>;
+  auto* kernel = kvq_token_kernel<QT, D, BITS, NT, FOLDED>;
   Maps maps;
   const Cache& c = ta.a.c;
   const uint64_t dims[3] = {TL::kRow, static_cast<uint64_t>(c.capacity), static_cast<uint64_t>(c.B) * c.Hk};
@@ -968,14 +981,16 @@ int launch_token(const TokenArgs& ta, int ctas, cudaStream_t s) {
   if (e != cudaSuccess) return fail(CTDK_ELAUNCH, "kvq_attn: %s", cudaGetErrorString(e));
   return check_launch("kvq_attn");
 }
+template <typename QT, int D, int BITS>
+int launch_rows(const TokenArgs& ta, int nt, int ctas, cudaStream_t s) {
+  if constexpr (sizeof(QT) == 2)
+    if (ta.rows <= 4) return launch_token<QT, D, BITS, 1, true>(ta, ctas, s);
+  return nt == 1 ? launch_token<QT, D, BITS, 1>(ta, ctas, s) : launch_token<QT, D, BITS, 2>(ta, ctas, s);
+}
 template <typename QT>
 int launch_any(const TokenArgs& ta, int D, int bits, int nt, int ctas, cudaStream_t s) {
-  if (D == 64) {
-    if (bits == 4) return nt == 1 ? launch_token<QT, 64, 4, 1>(ta, ctas, s) : launch_token<QT, 64, 4, 2>(ta, ctas, s);
-    return nt == 1 ? launch_token<QT, 64, 8, 1>(ta, ctas, s) : launch_token<QT, 64, 8, 2>(ta, ctas, s);
-  }
-  if (bits == 4) return nt == 1 ? launch_token<QT, 128, 4, 1>(ta, ctas, s) : launch_token<QT, 128, 4, 2>(ta, ctas, s);
-  return nt == 1 ? launch_token<QT, 128, 8, 1>(ta, ctas, s) : launch_token<QT, 128, 8, 2>(ta, ctas, s);
+  if (D == 64) return bits == 4 ? launch_rows<QT, 64, 4>(ta, nt, ctas, s) : launch_rows<QT, 64, 8>(ta, nt, ctas, s);
+  return bits == 4 ? launch_rows<QT, 128, 4>(ta, nt, ctas, s) : launch_rows<QT, 128, 8>(ta, nt, ctas, s);
 }
 
 int64_t part_bytes(int D, int64_t rows) {
