@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            s[k][n][c] *= factor[n][c & 1];
+            s[k][n][c] = __fmul_rn(s[k][n][c], factor[n][c & 1]);   // (rounded as its maximum is)
             if (!PLAIN && !sees(at_row[n][c & 1], j0 + 16 * k + g + 8 * (c >> 1), a.window, a.sinks)) s[k][n][c] = -INFINITY;
           }
       }

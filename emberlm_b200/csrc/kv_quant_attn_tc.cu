@@ -219,7 +219,7 @@ __device__ __forceinline__ void exact_rows(const TcArgs& ta, const Item& w, int 
 #pragma unroll
       for (int n = 0; n < N; ++n) {
         const bool sees_it = mine && sees(at[n], j, a.window, a.sinks);
-        const float z = sees_it ? x[n] * a.scale_log2 : -INFINITY, most = warp_max(z);
+        const float z = sees_it ? __fmul_rn(x[n], a.scale_log2) : -INFINITY, most = warp_max(z);
         if (most > m[n]) {
           const float f = ex2(m[n] - most);
           m[n] = most;
@@ -629,7 +629,8 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
           }
           float x[64];
           tmem_ld_32x64_nowait(ts, x);
-          const float sc = fmaxf(factor * scale_k[g % kRing], 0x1p-126f), shrink = shrink_o[g % kRing];
+          float sc = fmaxf(factor * scale_k[g % kRing], 0x1p-126f);
+          const float shrink = shrink_o[g % kRing];
           tmem_wait_ld();
           if (!plain) {
             // which of 32 positions the row sees, as bits: up to its own, from the window's first on or below the sinks
@@ -653,19 +654,26 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
               m2 = fmax3(m2, x[i + 4], x[i + 5]);
               m3 = fmax3(m3, x[i + 6], x[i + 7]);
             }
-            mx = fmax3(fmax3(m0, x[60], x[61]), fmax3(m1, x[62], x[63]), fmaxf(m2, m3));
+            mx = __fmul_rn(fmax3(fmax3(m0, x[60], x[61]), fmax3(m1, x[62], x[63]), fmaxf(m2, m3)), sc);
+          }
+          // What the reference point was rounded by, the difference below takes into the exponent, for all positions alike; from 2^23
+          // on that could leave fp16's range, and the scores are rounded first.
+          if (__builtin_expect(fabsf(mx) > 0x1p23f && mx != -INFINITY, 0)) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) x[i] = __fmul_rn(x[i], sc);
+            sc = 1.0f;
           }
           // Most tiles move no reference point: one barrier tells the two warps of these rows so.
           int move;
           asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, 64, p;\n selp.b32 %0, 1, 0, q;\n}"
-                       : "=r"(move) : "r"(static_cast<int>(mx * sc > m_ref + kSlack || shrink != 1.0f || !ok)), "r"(1 + quarter) : "memory");
+                       : "=r"(move) : "r"(static_cast<int>(mx - m_ref > kSlack || shrink != 1.0f || !ok)), "r"(1 + quarter) : "memory");
           if (move != 0) {
-            const float mxs = fmaxf(mx, other(mx)) * sc;
+            const float most = fmaxf(mx, other(mx));
             if (!ok) break;
             float c = 1.0f;
-            if (mxs > m_ref + kSlack) {
-              c = ex2(m_ref - mxs);
-              m_ref = mxs;
+            if (most - m_ref > kSlack) {
+              c = ex2(m_ref - most);
+              m_ref = most;
             }
             pending *= c * shrink;
             if (j != 0 && (NT == 1 || j % kTogether != 0)) {

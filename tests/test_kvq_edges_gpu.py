@@ -100,3 +100,22 @@ def test_sizes_that_differ_beside_split_work_and_nan(K, bits, dtype):  # noqa: F
     q = rnd((3, T, H, D), 43, 1.0, dtype).cuda()
     check(K, cache, q, n - T)
     check(K, cache, q, [n - T, 1495, 2400], [T, 11, T], n=n)
+
+
+# ---- scores of all sizes --------------------------------------------------------------------------
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,H,Hk,D", SHAPES)
+@pytest.mark.parametrize("power", [18, 22, 24, 26, 28, 31, 45, 80])
+def test_large_scores(K, bits, dtype, T, H, Hk, D, power):  # noqa: F811
+    """Scores far beyond the 24 bits in which fp32 holds a difference of one: one position has all the weight, or, where two keys are
+    alike, both have half of it, whatever sign the scores have."""
+    n = 400
+    k, v = rnd((2, n, Hk, D), 61, 0.7), rnd((2, n, Hk, D), 62)
+    k[:, 1::2] = k[:, ::2]
+    q = rnd((2, T, H, D), 63) * 2.0 ** power
+    cache = wrote(K, k, v, bits)
+    B.compare(K, cache, q.to(dtype).cuda(), n - T)
+    B.compare(K, cache, q.to(dtype).cuda(), [n - T, 150], window=70, sinks=2, n=n)
+    low = wrote(K, k.abs() + 0.1, v, bits)            # all scores far below zero
+    B.compare(K, low, -q.abs().to(dtype).cuda(), n - T)
