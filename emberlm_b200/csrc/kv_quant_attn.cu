@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
   __shared__ Feed feed;
   __shared__ Unit first_unit;
   __shared__ __align__(16) uint32_t q_terms[NT][NQ][32][2 * STEPS + 4];   // (rows of odd numbers of 16 bytes: no bank conflicts)
-  __shared__ float q_factor[8 * NT], q_init[8 * NT][GROUPS];
+  __shared__ float q_factor[8 * NT], q_more[8 * NT], q_init[8 * NT][GROUPS];
   __shared__ int64_t scan[kWarps + 1];
   __shared__ float row_m[kWarps][8 * NT], row_l[kWarps][8 * NT];
   const AttnArgs& a = ta.a;
@@ -438,7 +438,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
 #pragma unroll
       for (int o = 1; o < kPer; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
       const int e = static_cast<int>(__float_as_uint(most) >> 23) - 127;           // 128: not finite
-      const int up = most == 0.0f || e == 128 ? 0 : max(min(6 - e, 126), -100);    // most * 2^up is in [64, 128), or near it
+      int up = most == 0.0f || e == 128 ? 0 : min(6 - e, 126);                     // most * 2^up is in [64, 128), or below; from 2^107 on,
+      if (up < -100) up += 8;                                                      // for a smaller factor behind the products, in [2^14, 2^15)
       const float f = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] *= f;
@@ -446,7 +447,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if ((c4 & 7) == 0) q_init[rr][c4 / 8] = sum * (BITS == 4 ? -8.0f * 0x1p-24f : -128.0f * 0x1p-24f);
-      if (c4 == 0) q_factor[rr] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + (NQ == 1 ? 24 : 9) - up) << 23);   // up is from -100 to 126
+      if (c4 == 0) {                                   // 2^down, down from -117 to 122 (fp32) or 137; there, what exceeds 2^120 goes to the sums of the codes
+        const int down = (NQ == 1 ? 24 : 9) - up, first = NQ == 1 ? min(down, 120) : down;
+        q_factor[rr] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + first) << 23);
+        q_more[rr] = __uint_as_float(static_cast<uint32_t>(127 + down - first) << 23);
+      }
       if constexpr (BITS == 4) {                       // columns 8 tig + c of a group: pairs (c, c + 4); odd c times 2^-4 beside raw codes
         const int row_lane = (rr & 7) * 4 + ((c4 >> 1) & 3), half = c4 & 1, word = 4 * (c4 >> 3);
         uint32_t t01[NQ], t23[NQ];
@@ -508,9 +513,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
         for (int c = 0; c < 4; ++c) o[n][i][c] = 0.0f;
     }
 
-    // One tile; PLAIN: every valid row sees all of it.
-    auto tile = [&](auto plain, int j0, uint32_t kbase, uint32_t ksc) {
-      constexpr bool PLAIN = decltype(plain)::value;
+    // One tile; PLAIN: every valid row sees all of it; HUGE: there are queries whose factor is in two parts.
+    auto tile = [&](auto plain, auto some_huge, int j0, uint32_t kbase, uint32_t ksc) {
+      constexpr bool PLAIN = decltype(plain)::value, HUGE = decltype(some_huge)::value;
       const uint32_t vbase = kbase + kWarps * TL::kCodes, vsc = ksc + kWarps * TL::kScales;
       float s[BLOCKS][NT][4];
       // ---- scores
@@ -547,6 +552,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
             const float s1 = __uint_as_float(gr & 1 ? sc[1][gr / 2] & 0xffff0000u : sc[1][gr / 2] << 16);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
+              if constexpr (HUGE)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[n][c] *= q_more[8 * n + 2 * tig + (c & 1)];
 #pragma unroll
               for (int c = 0; c < 4; ++c) s[k][n][c] = gr == 0 ? acc[n][c] * (c < 2 ? s0 : s1) : fmaf(acc[n][c], c < 2 ? s0 : s1, s[k][n][c]);
             }
@@ -744,10 +752,18 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
         const uint32_t kbase = smem_u32(smem) + st * TL::kStageBytes + warp * TL::kCodes;
         const uint32_t ksc = smem_u32(smem) + st * TL::kStageBytes + 2 * kWarps * TL::kCodes + warp * TL::kScales;
         const int j0 = f.j + warp * KEYS;
-        if (j0 >= f.plain_lo && j0 <= f.plain_hi) {
-          tile(std::true_type{}, j0, kbase, ksc);
-        } else {
-          tile(std::false_type{}, j0, kbase, ksc);
+        bool huge = false;                             // (by the factors, which are at hand)
+        if constexpr (NQ == 1) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) huge |= fmaxf(fabsf(factor[n][0]), fabsf(factor[n][1])) > 0x1p105f;
+          huge = __any_sync(0xffffffffu, huge);
+        }
+        if (j0 >= f.plain_lo && j0 <= f.plain_hi && !huge) {
+          tile(std::true_type{}, std::false_type{}, j0, kbase, ksc);
+        } else if (!huge) {
+          tile(std::false_type{}, std::false_type{}, j0, kbase, ksc);
+        } else if constexpr (NQ == 1) {
+          tile(std::false_type{}, std::true_type{}, j0, kbase, ksc);
         }
       }
       __syncwarp();

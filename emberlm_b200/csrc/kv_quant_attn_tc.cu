@@ -582,9 +582,9 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
           }
         big = fmaxf(big, other(big));
         const int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;              // 128: not finite
-        const int up = big == 0.0f || e == 128 ? 0 : max(min(6 - e, 126), -100);
+        const int up = big == 0.0f || e == 128 ? 0 : min(6 - e, 126);
         const float f = a.scale_log2 < 0.0f ? -pow2(up) : pow2(up);
-        const float factor = fabsf(a.scale_log2) * pow2(-up);
+        const float factor = fabsf(a.scale_log2) * pow2(-up);   // 2^-126 to 2^121
 #pragma unroll 1
         for (int i = 0; i < D / 2; i += 32) {
           uint32_t q16[NT][16];
@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
           }
           float x[64];
           tmem_ld_32x64_nowait(ts, x);
-          float sc = fmaxf(factor * scale_k[g % kRing], 0x1p-126f);
+          float sc = fminf(fmaxf(factor * scale_k[g % kRing], 0x1p-126f), 0x1p127f);   // (finite: scores of zero stay)
           const float shrink = shrink_o[g % kRing];
           tmem_wait_ld();
           if (!plain) {

@@ -119,3 +119,21 @@ def test_large_scores(K, bits, dtype, T, H, Hk, D, power):  # noqa: F811
     B.compare(K, cache, q.to(dtype).cuda(), [n - T, 150], window=70, sinks=2, n=n)
     low = wrote(K, k.abs() + 0.1, v, bits)            # all scores far below zero
     B.compare(K, low, -q.abs().to(dtype).cuda(), n - T)
+
+
+# ---- queries of all sizes -------------------------------------------------------------------------
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,H,Hk,D", [(1, 4, 2, 64), (2, 6, 2, 128), (4, 6, 2, 64), (40, 4, 2, 128), (40, 4, 2, 64)])
+@pytest.mark.parametrize("power", [-120, -90, 99, 107, 113, 119, 125])
+def test_large_and_small_queries(K, bits, dtype, T, H, Hk, D, power):  # noqa: F811
+    """Finite queries up to the type's largest: over keys as small (or large) as they are large, with ordinary scores, and one huge head beside
+    ordinary ones."""
+    n = 300
+    k, v = rnd((2, n, Hk, D), 51, 0.7), rnd((2, n, Hk, D), 52)
+    q = rnd((2, T, H, D), 53, 1.0, F32).clamp(-3.5, 3.5)
+    cache = wrote(K, k * 2.0 ** -max(power, -90), v, bits)
+    B.compare(K, cache, (q * 2.0 ** power).to(dtype).cuda(), n - T)
+    if 0 < power < 120:
+        q[:, :, 1] *= 2.0 ** power
+        B.compare(K, wrote(K, k, v, bits), q.to(dtype).cuda(), n - T, window=100, sinks=3)
