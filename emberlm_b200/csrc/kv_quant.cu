@@ -234,8 +234,8 @@ int ctdk_kvq_write(const ctdk_kvq_cache* cache, const void* k, const void* v, in
   if (const int rc = kvq::check_cache(cache, "kvq_write"); rc != CTDK_OK) return rc;
   CTDK_REQUIRE(dtype == CTDK_DTYPE_F32 || dtype == CTDK_DTYPE_BF16, "kvq_write: dtype must be CTDK_DTYPE_F32 or CTDK_DTYPE_BF16");
   CTDK_REQUIRE(T >= 0 && T <= INT32_MAX, "kvq_write: bad T");
-  CTDK_REQUIRE(pos != nullptr || (pos_all >= 0 && pos_all + T <= cache->capacity), "kvq_write: positions %lld..%lld exceed the capacity %lld",
-               static_cast<long long>(pos_all), static_cast<long long>(pos_all + T), static_cast<long long>(cache->capacity));
+  CTDK_REQUIRE(pos != nullptr || (pos_all >= 0 && pos_all <= cache->capacity - T), "kvq_write: %lld positions from %lld on exceed the capacity %lld",
+               static_cast<long long>(T), static_cast<long long>(pos_all), static_cast<long long>(cache->capacity));
   if (T == 0 || cache->B == 0) return CTDK_OK;
   const int64_t unit = dtype == CTDK_DTYPE_F32 ? 4 : 8;   // elements in 16 bytes
   CTDK_REQUIRE(k != nullptr && v != nullptr && kvq::aligned(k, 16) && kvq::aligned(v, 16), "kvq_write: k and v must be 16-byte aligned");

@@ -1024,7 +1024,8 @@ extern "C" {
 
 int64_t ctdk_kvq_attn_workspace_bytes(const ctdk_kvq_cache* cache, int64_t T, int H) {
   if (const int rc = kvq::check_cache(cache, "kvq_attn"); rc != CTDK_OK) return rc;
-  CTDK_REQUIRE(T >= 0 && H > 0 && H % cache->Hk == 0, "kvq_attn: heads must be a multiple of kv heads");
+  CTDK_REQUIRE(H > 0 && H % cache->Hk == 0, "kvq_attn: heads must be a multiple of kv heads");
+  CTDK_REQUIRE(T >= 0 && T <= INT32_MAX / 2 / H, "kvq_attn: bad T");
   if (T == 0 || cache->B == 0) return 0;
   const int64_t rows = T * (H / cache->Hk);
   return rows <= 16 ? kvq::part_bytes(cache->D, rows) : kvq::attn_tc_bytes(cache->B, cache->Hk, cache->D, rows);
@@ -1038,8 +1039,8 @@ int ctdk_kvq_attn(const ctdk_kvq_cache* cache, const void* q, int dtype, int64_t
   CTDK_REQUIRE(H > 0 && H % cache->Hk == 0, "kvq_attn: heads must be a multiple of kv heads");
   CTDK_REQUIRE(window >= 0 && sinks >= 0, "kvq_attn: window and sinks must not be negative");
   CTDK_REQUIRE(T >= 0 && T <= INT32_MAX / 2 / H, "kvq_attn: bad T");
-  CTDK_REQUIRE(pos != nullptr || (pos_all >= 0 && pos_all + T <= cache->capacity), "kvq_attn: positions %lld..%lld exceed the capacity %lld",
-               static_cast<long long>(pos_all), static_cast<long long>(pos_all + T), static_cast<long long>(cache->capacity));
+  CTDK_REQUIRE(pos != nullptr || (pos_all >= 0 && pos_all <= cache->capacity - T), "kvq_attn: %lld positions from %lld on exceed the capacity %lld",
+               static_cast<long long>(T), static_cast<long long>(pos_all), static_cast<long long>(cache->capacity));
   if (T == 0 || cache->B == 0) return CTDK_OK;
   const int64_t unit = dtype == CTDK_DTYPE_F32 ? 4 : 8;   // elements in 16 bytes
   CTDK_REQUIRE(q != nullptr && out != nullptr, "kvq_attn: null pointer");

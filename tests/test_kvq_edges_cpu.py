@@ -31,3 +31,14 @@ def test_no_rows_need_no_workspace():
     d = desc()
     assert lib.raw().ctdk_kvq_attn_workspace_bytes(C.addressof(d), 0, 4) == 0
     assert lib.raw().ctdk_kvq_attn_workspace_bytes(C.addressof(d), 0, 64) == 0
+
+
+def test_positions_and_lengths_at_the_end_of_64_bits_are_refused():
+    L, d = lib.raw(), desc()
+    p = C.addressof(d)
+    for at in (2 ** 63 - 1, 2 ** 63 - 64, 127):
+        assert L.ctdk_kvq_write(p, 4096, 4096, 0, 128, 128, 64, None, at, None, None) == lib.CTDK_EINVAL
+        assert L.ctdk_kvq_attn(p, 4096, 0, 128, 128, 64, 4, None, at, None, 0, 0, 0.125, 4096, 4096, 1 << 30, None) == lib.CTDK_EINVAL
+    for T in (2 ** 63 - 1, 2 ** 62, 2 ** 40, -1):
+        assert L.ctdk_kvq_attn_workspace_bytes(p, T, 4) == lib.CTDK_EINVAL
+        assert L.ctdk_kvq_attn(p, 4096, 0, 128, 128, T, 4, 4096, 0, None, 0, 0, 0.125, 4096, 4096, 1 << 30, None) == lib.CTDK_EINVAL
