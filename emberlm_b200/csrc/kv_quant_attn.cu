@@ -25,7 +25,9 @@
 // bandwidth; 32 ragged sequences of up to 32768 of 8 x 128 in 4 bits, two bfloat16 rows a head, 680 MB: 163 us, 65 %; 64
 // windows of 1024 in 8 bits, 144 MB: 46 us, 49 %. What is left is instructions: turning codes into 16-bit numbers and, for fp32, two
 // and three terms a product.
+#include <cfloat>
 #include <climits>
+#include <cmath>
 #include <type_traits>
 
 #include "kv_quant_attn.h"
@@ -37,7 +39,7 @@ namespace {
 
 constexpr int kWarps = 7, kStages = 3;   // warps that compute (an eighth one loads: with 128 registers a thread, two CTAs fill an SM)
 constexpr int kThreads = (kWarps + 1) * 32;
-constexpr float kSlack = 8.0f;
+constexpr float kSlack = 8.0f, kLog2E = 1.4426950408889634f;
 
 template <int D, int BITS>
 struct Tile {
@@ -449,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
       if ((c4 & 7) == 0) q_init[rr][c4 / 8] = sum * (BITS == 4 ? -8.0f * 0x1p-24f : -128.0f * 0x1p-24f);
       if (c4 == 0) {                                   // 2^down, down from -117 to 122 (fp32) or 137; there, what exceeds 2^120 goes to the sums of the codes
         const int down = (NQ == 1 ? 24 : 9) - up, first = NQ == 1 ? min(down, 120) : down;
-        q_factor[rr] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + first) << 23);
+        q_factor[rr] = fminf(fmaxf(a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + first) << 23), -FLT_MAX), FLT_MAX);   // (scores of zero stay)
         q_more[rr] = __uint_as_float(static_cast<uint32_t>(127 + down - first) << 23);
       }
       if constexpr (BITS == 4) {                       // columns 8 tig + c of a group: pairs (c, c + 4); odd c times 2^-4 beside raw codes
@@ -1041,6 +1043,7 @@ int ctdk_kvq_attn(const ctdk_kvq_cache* cache, const void* q, int dtype, int64_t
   CTDK_REQUIRE(T >= 0 && T <= INT32_MAX / 2 / H, "kvq_attn: bad T");
   CTDK_REQUIRE(pos != nullptr || (pos_all >= 0 && pos_all <= cache->capacity - T), "kvq_attn: %lld positions from %lld on exceed the capacity %lld",
                static_cast<long long>(T), static_cast<long long>(pos_all), static_cast<long long>(cache->capacity));
+  CTDK_REQUIRE(std::isfinite(scale * kvq::kLog2E), "kvq_attn: scale must be finite");
   if (T == 0 || cache->B == 0) return CTDK_OK;
   const int64_t unit = dtype == CTDK_DTYPE_F32 ? 4 : 8;   // elements in 16 bytes
   CTDK_REQUIRE(q != nullptr && out != nullptr, "kvq_attn: null pointer");
@@ -1064,7 +1067,7 @@ int ctdk_kvq_attn(const ctdk_kvq_cache* cache, const void* q, int dtype, int64_t
   a.T = static_cast<int>(T);
   a.H = H;
   a.group = H / cache->Hk;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale * kvq::kLog2E;
   a.part = static_cast<float*>(workspace);
   a.status = device_status_word();
   if (a.status == nullptr) return fail(CTDK_ELAUNCH, "kvq_attn: no status word");

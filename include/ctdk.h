@@ -339,13 +339,14 @@ int ctdk_ce_row_weight(const float* loss_mask, const float* dy, const float* mas
  * ctdk_kvq_attn: query t of sequence b sits at i = pos + t and sees the positions j <= i (of the
  * cache) with i - j < window (window 0: all of them) or j < sinks:
  *   out[b, t, h] = sum_j softmax_j(scale * q[b, t, h] . k[b, h / (H / Hk), j]) v[b, h / (H / Hk), j]
- * q, out: fp32 or bfloat16, both of the same type; out is [B, T, H, D]. A row that sees nothing
- * (padding, and a row whose own position is outside the cache, among them) is zeros. Scores, maxima
- * and sums are fp32. fp32 queries enter the products with an error of 2^-22 of themselves or 2^-31
- * of the row's largest value; the probabilities of fp32 outputs with one of 2^-22, those of bfloat16
- * outputs with 2^-16 (up to 16 rows T * H / Hk) or 2^-11 (more), or, with more than 16 rows, 2^-32 of the
- * row's largest probability. What lies at positions that a query does not see matters for no more
- * than the rounding of its row, and not at all where no query sees them; equal calls give equal bits.
+ * q, out: fp32 or bfloat16, both of the same type; out is [B, T, H, D]. scale is finite, times log2(e)
+ * too. A row that sees nothing (padding, and a row whose own position is outside the cache, among
+ * them) is zeros. Scores, maxima and sums are fp32. fp32 queries enter the products with an error of
+ * 2^-22 of themselves or 2^-31 of the row's largest value; the probabilities of fp32 outputs with one of
+ * 2^-22, those of bfloat16 outputs with 2^-16 (up to 16 rows T * H / Hk) or 2^-11 (more), or, with more
+ * than 16 rows, 2^-32 of the row's largest probability. What lies at positions that a query does not see
+ * matters for no more than the rounding of its row, and not at all where no query sees them; equal calls
+ * give equal bits.
  * workspace: device memory, 16-byte aligned, of ctdk_kvq_attn_workspace_bytes(cache, T, H) bytes
  * (0: none needed), whose contents need not be kept; calls that may overlap need one each.
  * ------------------------------------------------------------------------------------ */

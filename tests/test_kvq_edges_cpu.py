@@ -42,3 +42,10 @@ def test_positions_and_lengths_at_the_end_of_64_bits_are_refused():
     for T in (2 ** 63 - 1, 2 ** 62, 2 ** 40, -1):
         assert L.ctdk_kvq_attn_workspace_bytes(p, T, 4) == lib.CTDK_EINVAL
         assert L.ctdk_kvq_attn(p, 4096, 0, 128, 128, T, 4, 4096, 0, None, 0, 0, 0.125, 4096, 4096, 1 << 30, None) == lib.CTDK_EINVAL
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 3e38])
+def test_a_scale_that_is_not_finite_is_refused(scale):
+    L, d = lib.raw(), desc()
+    for T in (1, 64):                                  # few and many rows
+        assert L.ctdk_kvq_attn(C.addressof(d), 4096, 0, 128, 128, T, 4, None, 0, None, 0, 0, scale, 4096, 4096, 1 << 30, None) == lib.CTDK_EINVAL

@@ -137,3 +137,19 @@ def test_large_and_small_queries(K, bits, dtype, T, H, Hk, D, power):  # noqa: F
     if 0 < power < 120:
         q[:, :, 1] *= 2.0 ** power
         B.compare(K, wrote(K, k, v, bits), q.to(dtype).cuda(), n - T, window=100, sinks=3)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,H,Hk,D", [(1, 4, 2, 64), (5, 4, 2, 128), (40, 4, 2, 64)])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-30, 1e30])
+def test_scales_of_all_sizes(K, bits, dtype, T, H, Hk, D, scale):  # noqa: F811
+    """Also where a factor of a row would overflow: its scores are zeros, queries and keys have no column in common."""
+    n = 200
+    k, v = rnd((1, n, Hk, D), 71, 0.7), rnd((1, n, Hk, D), 72)
+    q = rnd((1, T, H, D), 73)
+    if scale == 1e30:
+        k[..., 32:] = 0
+        q[..., :32] = 0
+        q *= 2.0 ** 100
+    B.compare(K, wrote(K, k, v, bits), q.to(dtype).cuda(), n - T, scale=scale)
