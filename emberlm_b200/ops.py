@@ -354,6 +354,17 @@ def _kvq_rows(x, name, cache, heads):
     return (st if T > 1 else 0), (sb if B > 1 else 0)
 
 
+def _kvq_whole(x, name):
+    """x as an int of 64 bits: ctypes would drop the bits above."""
+    try:
+        n = int(x)
+    except (TypeError, ValueError, OverflowError):
+        n = None
+    if n is None or n != x or not -2 ** 63 <= n < 2 ** 63:
+        raise RuntimeError(f"{name}: expected a whole number of 64 bits")
+    return n
+
+
 def _kvq_places(pos, count, cache, name):
     """(pos pointer, position of all, count pointer): pos an int or int32 [B] on the device, count None or the latter."""
     at = [None, 0, None]
@@ -363,7 +374,7 @@ def _kvq_places(pos, count, cache, name):
                 raise RuntimeError(f"{name}: positions and counts are int32 [B] on the cache's device")
             at[i] = t.data_ptr()
         elif i == 0:
-            at[1] = int(t)
+            at[1] = _kvq_whole(t, name)
         elif t is not None:
             raise RuntimeError(f"{name}: count must be a tensor or None")
     return at
@@ -405,7 +416,8 @@ def kvq_read(cache, start, length, group=1, dtype=torch.float32):
     """(k, v) [B, Hk * group, length, D]: what the cache holds at positions start .., each KV head `group` times (both types exact)."""
     if dtype not in _KVQ_DTYPES:
         raise RuntimeError("kvq_read: expected float32 or bfloat16")
-    if start < 0 or length < 0 or start + length > cache.capacity or group < 1:
+    start, length, group = (_kvq_whole(x, "kvq_read") for x in (start, length, group))
+    if start < 0 or length < 0 or start + length > cache.capacity or not 1 <= group < 2 ** 31:
         raise RuntimeError("kvq_read: positions out of range, or a group below 1")
     out = torch.empty(2, cache.B, cache.Hk * group, length, cache.D, device=cache.device, dtype=dtype)
     k, v = out[0], out[1]
@@ -423,6 +435,7 @@ def kvq_attention(q, cache, pos, count=None, window=0, sinks=0, scale=None):
     if H == 0 or H % cache.Hk:
         raise RuntimeError("kvq_attention: heads must be a multiple of kv heads")
     p, at, n = _kvq_places(pos, count, cache, "kvq_attention")
+    window, sinks = _kvq_whole(window, "kvq_attention"), _kvq_whole(sinks, "kvq_attention")
     with _kvq_device(cache):
         out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         need = lib.raw().ctdk_kvq_attn_workspace_bytes(cache.ref, T, H)

@@ -49,3 +49,30 @@ def test_a_scale_that_is_not_finite_is_refused(scale):
     L, d = lib.raw(), desc()
     for T in (1, 64):                                  # few and many rows
         assert L.ctdk_kvq_attn(C.addressof(d), 4096, 0, 128, 128, T, 4, None, 0, None, 0, 0, scale, 4096, 4096, 1 << 30, None) == lib.CTDK_EINVAL
+
+
+@pytest.mark.parametrize("value", [2 ** 64, 2 ** 63, -2 ** 63 - 1, 2 ** 64 + 5, 3.5, float("nan"), float("inf")])
+def test_numbers_that_a_call_would_change_are_refused(value):
+    """ctypes keeps the low 64 bits of a number: position 2^64 would be position 0, a window of 2^64 + 5 one of 5."""
+    from emberlm_b200 import ops
+
+    cache = type("Cache", (), {"B": 2, "device": None, "capacity": 64})()
+    with pytest.raises(RuntimeError, match="whole number"):
+        ops._kvq_places(value, None, cache, "kvq_write")
+    assert ops._kvq_places(7.0, None, cache, "kvq_write") == [None, 7, None]
+    assert ops._kvq_places(2 ** 62, None, cache, "kvq_write") == [None, 2 ** 62, None]
+
+
+def test_windows_and_groups_that_a_call_would_change_are_refused():
+    import torch
+
+    from emberlm_b200 import ops
+
+    cache = type("Cache", (), {"B": 2, "device": torch.device("cpu"), "capacity": 64, "Hk": 2, "D": 64})()
+    q = torch.zeros(2, 1, 4, 64)
+    for kw in ({"window": 2 ** 64 + 5}, {"sinks": 2 ** 64 + 5}, {"window": 2.5}):
+        with pytest.raises(RuntimeError, match="whole number"):
+            ops.kvq_attention(q, cache, 0, **kw)
+    for args in ((0, 1, 2 ** 32 + 1), (0.5, 1, 1), (0, 1, 2 ** 31)):
+        with pytest.raises(RuntimeError):
+            ops.kvq_read(cache, *args)
