@@ -157,8 +157,8 @@ struct Unit {
 
 struct TokenArgs {
   AttnArgs a;
-  int rows;            // T * group
-  int split;           // 0: one CTA a unit (and a block of 8 * NT rows); 1: equal spans of all tiles
+  int rows;            // T * group, 8 * NT at most
+  int split;           // 0: one CTA a unit; 1: equal spans of all tiles
   Patterns bits;
 };
 
@@ -184,14 +184,14 @@ __device__ __forceinline__ int64_t count_of(const AttnArgs& a, int b) {
   return a.count != nullptr ? min(static_cast<int64_t>(a.count[b]), static_cast<int64_t>(a.T)) : a.T;
 }
 template <int KEYS>
-__device__ __forceinline__ Visit visit(const AttnArgs& a, int b, int t0, int rows) {
-  return visit_of(pos_of(a, b), count_of(a, b), t0, rows, a.c.capacity, a.window, a.sinks, KEYS);
+__device__ __forceinline__ Visit visit(const AttnArgs& a, int b) {
+  return visit_of(pos_of(a, b), count_of(a, b), 0, a.T, a.c.capacity, a.window, a.sinks, KEYS);
 }
 template <int KEYS>
-__device__ __forceinline__ void visit_unit(const AttnArgs& a, Unit& u, int t0, int rows) {
+__device__ __forceinline__ void visit_unit(const AttnArgs& a, Unit& u) {
   u.pos = pos_of(a, u.b);
   u.count = count_of(a, u.b);
-  u.v = visit_of(u.pos, u.count, t0, rows, a.c.capacity, a.window, a.sinks, KEYS);
+  u.v = visit_of(u.pos, u.count, 0, a.T, a.c.capacity, a.window, a.sinks, KEYS);
 }
 // Moves to the next unit that has tiles.
 template <int KEYS>
@@ -205,7 +205,7 @@ __device__ __forceinline__ void next_unit(const AttnArgs& a, Unit& u) {
   u.h = 0;
   do {
     ++u.b;
-    visit_unit<KEYS>(a, u, 0, a.T);
+    visit_unit<KEYS>(a, u);
   } while (u.v.tiles == 0 && u.b + 1 < a.c.B);
   u.begin = u.end;
   u.end += u.v.tiles;
@@ -245,7 +245,7 @@ template <int KEYS>
 __device__ __forceinline__ bool span_of(const AttnArgs& a, int i, int n, Span& span, Unit& u, int64_t* smem) {
   u = {};
   if (a.pos == nullptr && a.count == nullptr) {
-    visit_unit<KEYS>(a, u, 0, a.T);
+    visit_unit<KEYS>(a, u);
     const int64_t all = static_cast<int64_t>(u.v.tiles) * a.c.B * a.c.Hk;
     n = sharing(all, n);
     if (i >= n) return false;
@@ -261,7 +261,7 @@ __device__ __forceinline__ bool span_of(const AttnArgs& a, int i, int n, Span& s
   // Tiles of a chunk of sequences, one a thread; more than one chunk: once for their sum, once more to find the place.
   auto mine = [&](int b0) {
     const int b = b0 + static_cast<int>(threadIdx.x);
-    return b < a.c.B ? static_cast<int64_t>(visit<KEYS>(a, b, 0, a.T).tiles) * a.c.Hk : 0;
+    return b < a.c.B ? static_cast<int64_t>(visit<KEYS>(a, b).tiles) * a.c.Hk : 0;
   };
   const int step = static_cast<int>(blockDim.x);
   int64_t x = mine(0), before, all = cta_sum(x, &before, smem);
@@ -281,7 +281,7 @@ __device__ __forceinline__ bool span_of(const AttnArgs& a, int i, int n, Span& s
   }
   __syncthreads();
   u.b = static_cast<int>(found[0]);
-  visit_unit<KEYS>(a, u, 0, a.T);
+  visit_unit<KEYS>(a, u);
   const int64_t h = quotient(span.lo - found[1], u.v.tiles);
   u.h = static_cast<int>(h);
   u.begin = found[1] + h * u.v.tiles;
@@ -337,23 +337,18 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
   // This CTA's tiles.
   Span span;
   Unit u = {};
-  int r0 = 0;                                          // first row of the block of rows
   if (ta.split) {
     if (!span_of<KEYS>(a, blockIdx.x, gridDim.x, span, u, scan)) return;
   } else {
-    const int blocks = (ta.rows + 8 * NT - 1) / (8 * NT);
-    const int64_t id = blockIdx.x, bh = id / blocks;
-    r0 = static_cast<int>(id - bh * blocks) * 8 * NT;
-    u.b = static_cast<int>(bh / a.c.Hk);
-    u.h = static_cast<int>(bh - static_cast<int64_t>(u.b) * a.c.Hk);
-    const int t0 = r0 / a.group, t1 = (min(r0 + 8 * NT, ta.rows) - 1) / a.group;
-    visit_unit<KEYS>(a, u, t0, t1 - t0 + 1);
+    u.b = static_cast<int>(blockIdx.x) / a.c.Hk;
+    u.h = static_cast<int>(blockIdx.x) - u.b * a.c.Hk;
+    visit_unit<KEYS>(a, u);
     u.begin = 0;
     u.end = u.v.tiles;
     span.lo = 0;
     span.hi = u.v.tiles;
   }
-  const int rows = min(8 * NT, ta.rows - r0);
+  const int rows = ta.rows;
 
   if (threadIdx.x == 0) {
     feed.u = first_unit = u;
@@ -429,9 +424,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
     constexpr int kPer = D / 4, kAtOnce = kWarps * 32 / kPer;   // threads of a row: 16 or 32
 #pragma unroll 1
     for (int rr = static_cast<int>(threadIdx.x) / kPer; rr < 8 * NT; rr += kAtOnce) {
-      const int n = rr / 8, c4 = static_cast<int>(threadIdx.x) % kPer, from = FOLDED ? rr & 3 : rr, r = r0 + from;
+      const int n = rr / 8, c4 = static_cast<int>(threadIdx.x) % kPer, r = FOLDED ? rr & 3 : rr;
       float x[4] = {};
-      if (from < rows) {
+      if (r < rows) {
         const int t = r / a.group;
         load_row<4>(static_cast<const QT*>(a.q) + ub * a.batch_stride + static_cast<int64_t>(t) * a.row_stride +
                         static_cast<int64_t>(uh * a.group + (r - t * a.group)) * D + 4 * c4, x);
@@ -505,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int r = FOLDED ? (2 * tig + c) & 3 : 8 * n + 2 * tig + c;
-        at_row[n][c] = r < rows ? row_position(pos, count, (r0 + r) / a.group, a.c.capacity) : -1;
+        at_row[n][c] = r < rows ? row_position(pos, count, r / a.group, a.c.capacity) : -1;
         m[n][c] = -INFINITY;
         l[n][c] = 0.0f;
       }
@@ -827,7 +822,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
             part[8 * NT * D + 8 * NT + rr] = ll;
           }
         } else {
-          const int t = (r0 + rr) / a.group, hg = (r0 + rr) - t * a.group;
+          const int t = rr / a.group, hg = rr - t * a.group;
           const bool valid = row_position(pos, count, t, a.c.capacity) >= 0;
           store_out(static_cast<QT*>(a.out) + ((static_cast<int64_t>(ub) * a.T + t) * a.H + uh * a.group + hg) * D + d, valid ? sum / ll : 0.0f);
         }
@@ -857,7 +852,7 @@ __global__ void __launch_bounds__(kJoinThreads) kvq_join_kernel(const TokenArgs 
   pdl_wait();
   const int b = blockIdx.x / a.c.Hk, h = blockIdx.x - b * a.c.Hk;
   const int64_t pos = pos_of(a, b), count = count_of(a, b);
-  const Visit v = visit<KEYS>(a, b, 0, a.T);
+  const Visit v = visit<KEYS>(a, b);
   int64_t all, begin;
   if (a.pos == nullptr && a.count == nullptr) {
     all = static_cast<int64_t>(v.tiles) * a.c.B * a.c.Hk;
@@ -865,7 +860,7 @@ __global__ void __launch_bounds__(kJoinThreads) kvq_join_kernel(const TokenArgs 
   } else {
     int64_t n = 0, before = 0;
     for (int i = threadIdx.x; i < a.c.B; i += kJoinThreads) {
-      const int64_t x = visit<KEYS>(a, i, 0, a.T).tiles;
+      const int64_t x = visit<KEYS>(a, i).tiles;
       n += x;
       if (i < b) before += x;
     }
@@ -884,8 +879,8 @@ __global__ void __launch_bounds__(kJoinThreads) kvq_join_kernel(const TokenArgs 
   const int64_t end = begin + v.tiles;
   const int c0 = static_cast<int>(quotient((begin + 1) * ctas - 1, all)), c1 = static_cast<int>(quotient(end * ctas - 1, all));
   if (c0 == c1) return;
-  // The first part is its CTA's last unit (or its only one, which began before), the others are their CTAs' first.
-  const float* first = a.part + (static_cast<int64_t>(c0) * 2 + (begin < span_start(all, c0, ctas) ? 0 : 1)) * Part<D, NT>::kFloats;
+  // The first part is its CTA's last unit, the others are their CTAs' first.
+  const float* first = a.part + (static_cast<int64_t>(c0) * 2 + 1) * Part<D, NT>::kFloats;
   auto part_of = [&](int c) { return c == c0 ? first : a.part + static_cast<int64_t>(c) * 2 * Part<D, NT>::kFloats; };
   float sum[kOut];
 #pragma unroll
@@ -941,8 +936,11 @@ __global__ void __launch_bounds__(kJoinThreads) kvq_join_kernel(const TokenArgs 
     for (int i = 0; i < kOut; ++i) {
       const int e = threadIdx.x + i * kJoinThreads, r = e / D;
       if (r >= ta.rows) continue;
+      int p = 0;
+      if (p0 == c0) sum[i] += weight[p++][r] * first[e];
+      const float* others = a.part + static_cast<int64_t>(p0 + p) * 2 * Part<D, NT>::kFloats + e;
 #pragma unroll 8
-      for (int p = 0; p < n; ++p) sum[i] += weight[p][r] * part_of(p0 + p)[e];
+      for (; p < n; ++p, others += 2 * Part<D, NT>::kFloats) sum[i] += weight[p][r] * others[0];
     }
   }
   __syncthreads();
@@ -956,7 +954,7 @@ __global__ void __launch_bounds__(kJoinThreads) kvq_join_kernel(const TokenArgs 
 }
 
 // CTAs of the split form: as many as run at a time, fewer where a CTA's warps would not get a tile each.
-int split_ctas(int D, int bits, int64_t rows, int64_t units, int64_t tiles) {
+int split_ctas(int64_t rows, int64_t units, int64_t tiles) {
   const int full = (rows <= 8 ? 2 : 1) * sm_count();
   const int64_t want = (units * tiles + kWarps - 1) / kWarps;
   return static_cast<int>(want < full ? (want < 1 ? 1 : want) : full);
@@ -974,7 +972,7 @@ int64_t most_tiles(const AttnArgs& a, int D, int bits) {
 // than they save. Split and unsplit, us, 8 bits, 8 x 128, two fp32 rows a head: one sequence of 15, 35, 49, 98 tiles 12.4 / 7.2,
 // 9.9 / 9.8, 10.5 / 12.2, 12.6 / 20.6; 32 sequences 18.3 / 9.7, 23.1 / 14.2, 25.8 / 17.7, 38.0 / 32.1 (which sequences there
 // are is not known on the host, and one long one among them has to be split: a unit's tiles decide, not their number in all).
-bool split_wanted(int64_t rows, int64_t tiles) { return rows <= 16 && tiles > 5 * kWarps; }
+bool split_wanted(int64_t tiles) { return tiles > 5 * kWarps; }
 
 template <typename QT, int D, int BITS, int NT, bool FOLDED = false>
 int launch_token(const TokenArgs& ta, int ctas, cudaStream_t s) {
@@ -1084,15 +1082,15 @@ int ctdk_kvq_attn(const ctdk_kvq_cache* cache, const void* q, int dtype, int64_t
   ta.bits = kvq::patterns(cache->bits);
   const int nt = rows <= 8 ? 1 : 2;
   const int64_t tiles = kvq::most_tiles(a, cache->D, cache->bits);
-  ta.split = kvq::split_wanted(rows, tiles) ? 1 : 0;
-  int64_t ctas = units * ((rows + 8 * nt - 1) / (8 * nt));
+  ta.split = kvq::split_wanted(tiles) ? 1 : 0;
+  int64_t ctas = units;
   if (ta.split) {
     CTDK_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 &&
                      workspace_bytes >= kvq::part_bytes(cache->D, rows),
                  "kvq_attn: the workspace needs %lld bytes, 16-byte aligned", static_cast<long long>(kvq::part_bytes(cache->D, rows)));
-    ctas = kvq::split_ctas(cache->D, cache->bits, rows, units, tiles);
+    ctas = kvq::split_ctas(rows, units, tiles);
   }
-  CTDK_REQUIRE(ctas <= INT32_MAX && units <= INT32_MAX, "kvq_attn: too many rows");
+  CTDK_REQUIRE(units <= INT32_MAX, "kvq_attn: too many rows");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == CTDK_DTYPE_F32 ? kvq::launch_any<float>(ta, cache->D, cache->bits, nt, static_cast<int>(ctas), s)
                                  : kvq::launch_any<__nv_bfloat16>(ta, cache->D, cache->bits, nt, static_cast<int>(ctas), s);
