@@ -153,3 +153,54 @@ def test_scales_of_all_sizes(K, bits, dtype, T, H, Hk, D, scale):  # noqa: F811
         q[..., :32] = 0
         q *= 2.0 ** 100
     B.compare(K, wrote(K, k, v, bits), q.to(dtype).cuda(), n - T, scale=scale)
+
+
+# ---- sizes at which work is shared out differently ------------------------------------------------
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_more_parts_than_the_join_holds_at_a_time(K, bits, dtype):  # noqa: F811
+    """One long sequence of one head on every CTA: more than 128 parts (the join takes them in rounds), with scores that grow."""
+    n, H, D = 150000, 4, 64
+    k, v = rnd((1, n, 1, D), 81, 0.4), rnd((1, n, 1, D), 82)
+    k *= torch.linspace(0.5, 6, n).reshape(1, n, 1, 1)
+    cache = wrote(K, k, v, bits)
+    B.compare(K, cache, rnd((1, 1, H, D), 83, 1.0, dtype).cuda(), n - 1)
+    B.compare(K, cache, rnd((1, 3, H, D), 84, 1.0, dtype).cuda(), n - 3)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_more_sequences_than_a_block_has_threads(K, dtype):  # noqa: F811
+    """700 ragged sequences, some empty, in a cache long enough for the work to be shared."""
+    batch, H, Hk, D = 700, 4, 2, 64
+    capacity = 1536
+    cache = K.kvq_cache(batch, Hk, capacity, D, 8)
+    g = torch.Generator().manual_seed(91)
+    lengths = torch.randint(0, 200, (batch,), generator=g)
+    lengths[::7] = 0
+    lengths[511], lengths[255], lengths[256] = 1500, 1100, 0
+    k, v = rnd((batch, 200, Hk, D), 92).cuda(), rnd((batch, 200, Hk, D), 93).cuda()
+    for at in range(0, capacity - 200, 200):
+        K.kvq_write(cache, k, v, at)
+    q = rnd((batch, 1, H, D), 94, 1.0, dtype).cuda()
+    pos = [int(n) - 1 for n in lengths]
+    got = K.kvq_attention(q, cache, torch.tensor(pos, dtype=torch.int32, device="cuda"))
+    for b in list(range(0, 30)) + [254, 255, 256, 257, 510, 511, 512, 513, 698, 699]:
+        one = K.KvqCache(*[t[b:b + 1].contiguous() for t in cache.tensors])
+        alone = B.compare(K, one, q[b:b + 1], [pos[b]], n=max(pos[b] + 1, 1))
+        assert torch.equal(got[b] == 0, torch.from_numpy(alone[0] == 0).cuda())
+    # every sequence against the others' way of being shared out: fp32 to its bound's size, a few roundings
+    far = (got.double() - torch.cat([K.kvq_attention(q[b:b + 1], K.KvqCache(*[t[b:b + 1].contiguous() for t in cache.tensors]), pos[b] if pos[b] >= 0 else
+                                                      torch.tensor([-1], dtype=torch.int32, device="cuda")) for b in range(batch)]).double()).abs().max()
+    assert far <= (2.0 ** -18 if dtype == F32 else 2.0 ** -6) * float(v.abs().max())
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("H,Hk,D", [(17, 1, 64), (32, 1, 128), (40, 2, 64), (160, 1, 64)])
+def test_one_token_of_many_heads(K, bits, dtype, H, Hk, D):  # noqa: F811
+    """More than 16 query heads a key/value head: single tokens go to the prompt kernel."""
+    n = 700
+    cache = wrote(K, rnd((2, n, Hk, D), 101, 0.5), rnd((2, n, Hk, D), 102), bits)
+    q = rnd((2, 1, H, D), 103, 1.0, dtype).cuda()
+    B.compare(K, cache, q, n - 1)
+    B.compare(K, cache, q, [0, 130], window=60, sinks=2, n=n)
