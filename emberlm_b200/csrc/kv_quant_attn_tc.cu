@@ -12,7 +12,7 @@
 //                values (the others) alike.
 //   warp 2       looks a tile's scales over, a tile ahead of those: exponents, NaN. (Warp 3 only fills a warpgroup.)
 // The products take fp16 operands. c * s is not exact in fp16 for every scale s, but c * s * 2^-e is, for the power of two that
-// brings a tile's largest scale near the top of the range, unless a scale is far smaller than that one (kSpanK, kSpanV below). Keys have
+// brings a tile's largest scale near the top of the range, unless a scale is far smaller than that one (Span below). Keys have
 // an e of their own in every tile (it joins the scores' factor), values one that O is rescaled for when a tile exceeds it. That one is
 // shared by the item's rows, whichever of them see the largest values; where an item's scales lie too far apart for it, warp 2 marks the
 // item, and its rows are formed once more from the cache in fp32 (exact_rows). fp32 queries
@@ -49,16 +49,22 @@ constexpr int kTogether = 4;
 constexpr int kRing = 8;
 constexpr int kRoom = 6;                 // powers of two by which values may grow before O is rescaled
 
+// Powers of two that a tile's scales of keys, an item's of values, may lie apart. All products of codes and scales are exact as long as
+// the smallest scale does not come below 2^-21 (4 bits: four significant bits, and fp16 has multiples of 2^-24) or 2^-24; that is enough
+// for bfloat16 outputs. The tensor cores, though, align products by the exponents that operands are held with, 2^-14 for all subnormal
+// ones, and cut off 26 bits below: for fp32 outputs, 22 bits are left down to 2^-18. Values may start kRoom lower.
+template <typename QT, int BITS>
+struct Span {
+  static constexpr int kTop = BITS == 4 ? 11 : 7;                    // the largest scale comes to [2^kTop, 2^(kTop + 1))
+  static constexpr int kK = kTop + (sizeof(QT) == 4 ? 18 : BITS == 4 ? 21 : 24), kV = kK - kRoom;
+};
+
 template <int D, int BITS>
 struct Cfg {
   static constexpr int kRow = D * BITS / 8, kGroups = D / kGroup, kChunks = D / 64;
   static constexpr int kCodes = KT * kRow, kScales = KT * kGroups * 2;
   static constexpr int kTile = kChunks * kChunk;                     // a converted tile
   static constexpr int kSmem = 1024 + 4 * kTile + 4 * kCodes + 4 * kScales;
-  static constexpr int kTop = BITS == 4 ? 11 : 7;                    // the largest scale comes to [2^kTop, 2^(kTop + 1))
-  // Powers of two between a tile's scales of keys, an item's of values, up to which all products of codes and scales are exact: fp16 has
-  // multiples of 2^-24, a scale four significant bits (4 bits) or one, and values may start kRoom lower.
-  static constexpr int kSpanK = kTop + (BITS == 4 ? 21 : 24), kSpanV = kSpanK - kRoom;
 };
 
 struct TcArgs {
@@ -486,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
             big = __reduce_max_sync(0xffffffffu, big);
             any = __any_sync(0xffffffffu, any != 0) ? 1u : 0u;
           }
-          const int e = big == 0 ? (which ? -120 : 0) : max(static_cast<int>(big >> 7) - 127 - C::kTop, -120);
+          const int e = big == 0 ? (which ? -120 : 0) : max(static_cast<int>(big >> 7) - 127 - Span<QT, BITS>::kTop, -120);
           if (which == 0) {
             exp_k[g % kRing] = e;                      // (all lanes: the same)
             scale_k[g % kRing] = pow2(e);
@@ -509,12 +515,12 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
           }
           if (big != 0) {                              // (behind what others wait for)
             const int top = static_cast<int>(big >> 7), bottom = static_cast<int>((__reduce_min_sync(0xffffffffu, min(least & 0xffffu, least >> 16)) + 1u) >> 7);
-            if (which == 0) wide |= top - bottom > C::kSpanK;
+            if (which == 0) wide |= top - bottom > Span<QT, BITS>::kK;
             else vtop = max(vtop, top), vlow = min(vlow, bottom);
           }
         }
       }
-      wide |= vtop - vlow > C::kSpanV;
+      wide |= vtop - vlow > Span<QT, BITS>::kV;
       marked |= wide;
       if (lane == 0) ta.wide[it] = wide ? 1 : 0;
     }

@@ -344,7 +344,7 @@ int ctdk_ce_row_weight(const float* loss_mask, const float* dy, const float* mas
  * them) is zeros. Scores, maxima and sums are fp32. fp32 queries enter the products with an error of
  * 2^-22 of themselves or 2^-31 of the row's largest value; the probabilities of fp32 outputs with one of
  * 2^-22, those of bfloat16 outputs with 2^-16 (up to 16 rows T * H / Hk) or 2^-11 (more), or, with more
- * than 16 rows, 2^-32 of the row's largest probability. What lies at positions that a query does not see
+ * than 16 rows, 2^-31 of the row's largest probability. What lies at positions that a query does not see
  * matters for no more than the rounding of its row, and not at all where no query sees them; equal calls
  * give equal bits.
  * workspace: device memory, 16-byte aligned, of ctdk_kvq_attn_workspace_bytes(cache, T, H) bytes

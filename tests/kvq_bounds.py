@@ -21,7 +21,9 @@ def attention(q, k, v, pos, count, window=0, sinks=0, scale=None, fp32=True, few
     what that does to the weights is formed position by position, from the scores moved up and down;
     a probability: the exponential is off by 2^-22 and its terms by 2^-22 (two of fp16, three of bfloat16 are less), in bfloat16 outputs
     by 2^-16 (two bfloat16 terms, few rows) or 2^-11 (one of fp16, many rows); fp16 terms, held times 2^7 beside a sum of 1 or more, lose
-    half a step of 2^-24, and what is below 2^-126 may be zero;
+    half a step of 2^-24 each where they are subnormal: 2^-25 / 2^7 = 2^-32 with one term; of two terms, the first is cut to 11 bits and
+    what is left is formed from that cut number, so that the rounding of neither makes up for the other's: 2^-31; what is below
+    2^-126 may be zero;
     sums over positions: of 16 products, in two or three terms, cut off by 2^-23 each; a new accumulator after 64 of them
     (fp32 outputs), then fp32 additions, through 64 joins at most and no more than there are steps; the same number of them for the sum of the probabilities;
     the result: half a step of its type."""
@@ -52,7 +54,7 @@ def attention(q, k, v, pos, count, window=0, sinks=0, scale=None, fp32=True, few
             steps = -(-len(z) // 16)
             sums = (min(3 * steps, 64) if fp32 else 3 * steps) * 2.0 ** -23 + 2 * u * (steps / 64 + min(steps, 64))
             tol[t, h] = (np.maximum(np.maximum(up, down), 0.0) @ np.abs(vv) + (p_off + sums) * (w @ np.abs(vv))
-                         + (2.0 ** -32 + 2.0 ** -126) * np.abs(vv).sum(0)) * (1 + half) + half * np.abs(out[t, h])
+                         + ((2.0 ** -31 if fp32 else 2.0 ** -32) + 2.0 ** -126) * np.abs(vv).sum(0)) * (1 + half) + half * np.abs(out[t, h])
     return out, tol
 
 
