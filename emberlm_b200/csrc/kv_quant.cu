@@ -26,20 +26,6 @@ struct RowArgs {
   int T, Hk;
 };
 
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-}
-
 // Eight 4-bit codes for the scale s, each value to the nearest whole number of steps, half to even, decided exactly, packed as they
 // are stored. The quotient is corrected once by its remainder (exact: both terms are whole multiples of the smaller one's last place
 // and their difference is short), which makes it exact wherever it is a half, a common case of bfloat16 values; adding 1.5 * 2^23

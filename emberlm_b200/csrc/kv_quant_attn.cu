@@ -86,14 +86,6 @@ __device__ __forceinline__ void lds_words(uint32_t (&w)[2], uint32_t a) {
 __device__ __forceinline__ void lds_words(uint32_t (&w)[4], uint32_t a) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
 }
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-__device__ __forceinline__ void unpack_f16(uint32_t w, float& lo, float& hi) {
-  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.f32.f16 %0, a;\n cvt.f32.f16 %1, b;\n}" : "=f"(lo), "=f"(hi) : "r"(w));
-}
 // (x, y) as N packed terms, each the rest of the ones before, rounded.
 template <int N>
 __device__ __forceinline__ void terms_f16(float x, float y, uint32_t (&t)[N]) {
@@ -141,12 +133,6 @@ __device__ __forceinline__ void load_row(const __nv_bfloat16* p, float* x) {
 struct Span {
   int64_t lo, hi;      // tiles of all units, numbered through
 };
-// As bulk_load of common.cuh, without a cache hint.
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
-               "r"(smem_u32(bar))
-               : "memory");
-}
 // A CTA's place in the list of units (sequence, key/value head): the unit it is at, and where that unit's tiles lie.
 struct Unit {
   int b, h;
@@ -288,9 +274,6 @@ __device__ __forceinline__ bool span_of(const AttnArgs& a, int i, int n, Span& s
   u.end = u.begin + u.v.tiles;
   return true;
 }
-
-__device__ __forceinline__ void store_out(float* p, float x) { *p = x; }
-__device__ __forceinline__ void store_out(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
 // Floats of a CTA's partial result for one unit: sums [rows][D], then the rows' reference points and denominators.
 template <int D, int NT>

@@ -82,6 +82,14 @@ __device__ __forceinline__ bool wait_w(uint64_t* bar, uint32_t parity, int* stat
   if (__builtin_expect(!ok, 0)) ok = wait_longer(bar, parity, status, where);
   return ok;
 }
+// As bulk_load of common.cuh, without a cache hint.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void store_out(float* p, float x) { *p = x; }
+__device__ __forceinline__ void store_out(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 // Position of row t of a sequence, or -1 if it is not valid.
 __device__ __forceinline__ int row_position(int64_t pos, int64_t count, int64_t t, int64_t capacity) {
   const int64_t i = pos + t;

@@ -101,14 +101,6 @@ __device__ __forceinline__ Item item_at(const TcArgs& ta, int it) { return item_
 __device__ __forceinline__ uint32_t idesc_f16(bool b_mn, int n) {
   return (1u << 4) | (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(TQ >> 4) << 24);
 }
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-__device__ __forceinline__ void unpack_f16(uint32_t w, float& lo, float& hi) {
-  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.f32.f16 %0, a;\n cvt.f32.f16 %1, b;\n}" : "=f"(lo), "=f"(hi) : "r"(w));
-}
 // The lowest n bits (n below 0: none; from 32 on: all).
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(max(-126, min(127, e)) + 127) << 23); }
@@ -118,35 +110,13 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r
                "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                : "memory");
 }
-__device__ __forceinline__ void bulk_in(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
-               "r"(smem_u32(bar))
-               : "memory");
-}
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-template <typename QT>
-__device__ __forceinline__ void load8(const QT* p, float (&x)[8]);
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
 }
 __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) { *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d); }
 __device__ __forceinline__ void store4(__nv_bfloat16* p, float a, float b, float c, float d) {
   *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(a, b), pack_bf16(c, d));
 }
-
-__device__ __forceinline__ void store1(float* p, float x) { *p = x; }
-__device__ __forceinline__ void store1(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
 // Rows r0 .. end - 1 of an item, by one warp, N at a time, from the codes and scales in the cache, in fp32 throughout: a lane a position
 // for the scores, a lane D / 32 columns for the output. For items whose scales no single power of two brings into fp16's range: right
@@ -275,7 +245,7 @@ __device__ __forceinline__ void exact_rows(const TcArgs& ta, const Item& w, int 
         const int r = w.r0 + r0 + n, t = r / a.group, hg = r - t * a.group;
         QT* dst = static_cast<QT*>(a.out) + ((static_cast<int64_t>(w.b) * a.T + t) * a.H + w.h * a.group + hg) * D + col;
 #pragma unroll
-        for (int c = 0; c < kOwn; ++c) store1(dst + c, at[n] >= 0 ? o[n][c] / l[n] : 0.0f);
+        for (int c = 0; c < kOwn; ++c) store_out(dst + c, at[n] >= 0 ? o[n][c] / l[n] : 0.0f);
       }
   }
 }
@@ -375,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) kvq_prompt_kernel(const __grid_co
             uint64_t* bar = &in_full[2 * st + i];
             mbar_expect_tx(bar, C::kCodes + there * C::kGroups * 2);
             tma_load_3d(codes_s + (2 * st + i) * C::kCodes, i ? &tm_v : &tm_k, bar, 0, j, bh);
-            bulk_in(scales_s + (2 * st + i) * C::kScales, a.c.scales[i] + sc, there * C::kGroups * 2, bar);
+            bulk_load(scales_s + (2 * st + i) * C::kScales, a.c.scales[i] + sc, there * C::kGroups * 2, bar);
           }
           __syncwarp();
         }
@@ -921,8 +891,7 @@ __global__ void __launch_bounds__(256) kvq_prompt_join_kernel(const TcArgs ta) {
     const int t = r / a.group, hg = r - t * a.group;
     const float x = row_position(pos, count, t, a.c.capacity) >= 0 ? s / l : 0.0f;
     QT* out = static_cast<QT*>(a.out) + ((static_cast<int64_t>(b) * a.T + t) * a.H + h * a.group + hg) * D + d;
-    if constexpr (sizeof(QT) == 4) *out = x;
-    else *out = __float2bfloat16_rn(x);
+    store_out(out, x);
   }
 }
 
