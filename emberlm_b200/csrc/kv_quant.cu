@@ -4,9 +4,13 @@
 // A thread takes sixteen neighbouring values, two threads a group; a row's threads are neighbours and consecutive rows
 // are consecutive positions of one head, so that the cache side is contiguous and the other side comes in whole head
 // rows of 128 to 512 bytes. (With eight values a thread the index arithmetic, not memory, was the limit.)
-// Measured (B200, copy bandwidth 6.45 TB/s): 4 x 4096 rows of 8 x 128, keys and values: bfloat16 to 4 bits 29 us (86 MB each way,
-// 3.0 TB/s), back 18 us (4.7 TB/s); fp32 to 8 bits 28 us (6.1 TB/s), back 33 us (5.1 TB/s). Writing 4 bits is bound by
-// the exact rounding (a quotient with its remainder a value), the others by memory.
+// Measured (B200, copy bandwidth 6.45 TB/s): 4 x 4096 rows of 8 x 128, keys and values, one call after the other over more data than
+// L2 holds, us and TB/s:
+//             fp32, 4 bits   bfloat16, 4 bits   fp32, 8 bits   bfloat16, 8 bits
+//   write     33.0  4.6      30.7  2.8          28.2  6.0      22.7  4.5
+//   read      32.6  4.7      21.6  4.0          33.4  5.1      20.6  5.0
+// Writing 4 bits spends its time on the exact rounding (a quotient with its remainder a value, from bfloat16 rows too, which would need
+// less); the others run at 62 to 93 % of the copy bandwidth.
 #include "kv_quant.cuh"
 
 namespace ctdk {

@@ -22,9 +22,11 @@
 // The floor is the cache's codes and scales, once. All tiles of all blocks lie on one line, which the CTAs cut into equal parts, so
 // that one long sequence keeps all SMs busy as a large batch does; blocks that were cut are joined by a second, small kernel.
 // Measured (B200, copy bandwidth 6.45 TB/s): 131072 positions of 8 x 64 in 8 bits, four fp32 rows a head, 143 MB: 45 us, 49 % of that
-// bandwidth; 32 ragged sequences of up to 32768 of 8 x 128 in 4 bits, two bfloat16 rows a head, 680 MB: 163 us, 65 %; 64
-// windows of 1024 in 8 bits, 144 MB: 46 us, 49 %. What is left is instructions: turning codes into 16-bit numbers and, for fp32, two
-// and three terms a product.
+// bandwidth; 32 ragged sequences of up to 32768 of 8 x 128 in 4 bits, two bfloat16 rows a head, 680 MB: 170 us, 62 %; 64
+// windows of 1024 in 8 bits, 144 MB: 46 us, 48 %. The bound is latency at low occupancy: with 128 registers a thread there are 3.6 to 3.7
+// warps a scheduler, which issue in half of the cycles (ALU pipe 34 to 48 %, tensor pipe 21 to 28 %, DRAM 42 to 45 %); of the
+// cycles between two issues of a warp, fixed latencies take 1.3 to 2.0, memory (spilled registers among it) 0.9 to 1.0, a busy math pipe 0.8 to
+// 0.9. At 128 registers fp32 rows over 128 columns spill 224 bytes (4 bits) and 32, bfloat16 rows up to 48.
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -953,8 +955,9 @@ int64_t most_tiles(const AttnArgs& a, int D, int bits) {
 }
 // Whether the work is split over all SMs: not where a unit has few tiles, for which the shares' beginnings and the second launch cost more
 // than they save. Split and unsplit, us, 8 bits, 8 x 128, two fp32 rows a head: one sequence of 15, 35, 49, 98 tiles 12.4 / 7.2,
-// 9.9 / 9.8, 10.5 / 12.2, 12.6 / 20.6; 32 sequences 18.3 / 9.7, 23.1 / 14.2, 25.8 / 17.7, 38.0 / 32.1 (which sequences there
-// are is not known on the host, and one long one among them has to be split: a unit's tiles decide, not their number in all).
+// 9.9 / 9.8, 10.5 / 12.2, 12.6 / 20.6; 32 sequences 18.3 / 9.7, 23.1 / 14.2, 25.8 / 17.7, 38.0 / 32.1. The rule asks a unit's tiles alone,
+// as it must where positions lie on the device: one long sequence among short ones has to be split. Where all units are known to be
+// alike and as many as the CTAs (pos_all, or a window), unsplit would be faster from 36 to some 100 tiles too; the rule does not ask that.
 bool split_wanted(int64_t tiles) { return tiles > 5 * kWarps; }
 
 template <typename QT, int D, int BITS, int NT, bool FOLDED = false>

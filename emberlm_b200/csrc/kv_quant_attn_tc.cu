@@ -19,10 +19,12 @@
 // enter as two fp16 terms (22 bits), and so do the probabilities of fp32 outputs; those of bfloat16 outputs as one.
 // With A from tensor memory the products read 64 bytes a clock of shared memory; with both operands there they would wait for it.
 // Every mbarrier wait is bounded.
-// Measured (B200): 2048 fp32 rows of 16 heads of 128 after 6144 positions in 4 bits (120 GFLOP, executed as two products each): 334 us, 360 TFLOP/s
-// of the 1635 that a bfloat16 product reaches; 4095 bfloat16 rows of 32 heads of 64 with a window of 512: 105 us. A tile is
-// bound by the softmax threads (two terms a probability: 17 cycles an element and thread) and the conversion beside them, which
-// share the instruction cache: code that was unrolled further ran slower (461 -> 297 us when the roles' loops were made small).
+// Measured (B200): 2048 fp32 rows of 16 heads of 128 after 6144 positions in 4 bits (120 GFLOP, executed as two products each): 320 us, 376 TFLOP/s
+// of the 1635 that a bfloat16 product reaches, 214 us in bfloat16; 4095 bfloat16 rows of 32 heads of 64 with a window of 512: 110 us. The
+// tensor pipe is active in 43 % of the cycles, a scheduler has five warps and issues in 52 %; of the cycles between two issues of a warp,
+// loads (of tensor memory, first of all) take 3.6, fixed latencies 1.1, barriers 0.9, missing instructions 0.8. A tile is bound by the softmax threads (two terms a probability: 17 cycles an element and thread) and the
+// conversion beside them, which share the instruction cache: code that was unrolled further ran slower (461 -> 297 us when the roles'
+// loops were made small). The fp32 softmax spills 72 (128 columns) or 92 bytes.
 #include <climits>
 
 #include "kv_quant_attn.h"
